@@ -290,6 +290,130 @@ int pulpnn_linear_out_32_static_scratch(const uint8_t *pInBuffer, const int32_t 
  */
 int pulpnn_selftest_wait_timeout(unsigned int limit_us);
 
+/* ---- attention over a paged cache of keys and values -------------------------
+ * What a decoder built on the 8-bit fully connected layers runs between them; no counterpart in the
+ * reference. pulp_nn_linear_out_32's accumulators become rotated queries and cached keys and values
+ * (pulpnn_kv_append), one new token per sequence reads the cache (pulpnn_attn_decode), a prompt is
+ * attended to as a whole (pulpnn_attn_prompt), cached rows come back as 16-bit rows (pulpnn_kv_gather),
+ * and both attentions can write the uint8 activations that pulp_nn_linear reads.
+ *
+ *  - Each call enqueues ONE kernel (pulpnn_attn_decode at most two) on the calling thread's stream, returns
+ *    a status (PULPNN_OK or an error code, also recorded for pulpnn_last_error) and may be captured
+ *    into a CUDA graph. The batch setting does not apply.
+ *  - Every buffer is device (or managed) memory of the context's GPU. Strides count elements; the channels of
+ *    a row lie side by side, and rows of queries, keys, values and outputs begin on 16-byte boundaries (uint8
+ *    outputs of the attentions: on 4-byte ones).
+ *  - head_dim: a multiple of 8 up to 128; of 16 where the cache holds 8 bits.
+ *  - Sizes come from the host; slots, positions, block tables, lengths and offsets are read from device
+ *    memory when the kernel runs. Values among them that point outside the buffers read and write nothing:
+ *    what each call does instead stands beside it.
+ */
+enum {
+  PULPNN_TYPE_F16 = 0, PULPNN_TYPE_BF16 = 1, PULPNN_TYPE_F32 = 2, PULPNN_TYPE_S32 = 3, PULPNN_TYPE_S8 = 4,
+  PULPNN_TYPE_U8 = 5
+};
+
+/* Keys and values in pages of page_size slots. Element (slot s, head h, channel c) of the keys is
+ * k[(s / page_size) * page_stride + (s % page_size) * slot_stride + h * head_stride + c]; the values and, for
+ * PULPNN_TYPE_S8, the scales (one float per slot and head) likewise. type: F16, BF16 or S8; an S8 row stands for
+ * code * scale, and a scale that is NaN makes its row NaN. */
+typedef struct {
+  void *k, *v;
+  float *k_scale, *v_scale;                 /* NULL unless type is PULPNN_TYPE_S8 */
+  int64_t page_stride, slot_stride, head_stride;
+  int64_t scale_page_stride, scale_slot_stride, scale_head_stride;
+  int32_t type, n_pages, page_size, n_heads, head_dim, reserved;
+} pulpnn_kv_cache_t;
+
+/*
+ * pulpnn_kv_append -- rotates queries and keys, and stores keys and values into the cache.
+ *
+ * Token t of head h: x = in (F16, BF16, F32) or in * step[h * head_dim + c] (S32). The first rotary_dim channels of
+ * q and k turn by the angle positions[t] * inv_freq[i], i < rotary_dim / 2: (a, b) -> (a cos - b sin,
+ * b cos + a sin) of the channels (i, i + rotary_dim / 2), or (2i, 2i + 1) where interleaved is set. The angle is
+ * computed in 64 bits. q_out receives q; row slots[t] of the cache receives k and v, rounded to its 16-bit type, or as
+ * S8 codes rint(x * 127 / max|x|) with the scale max|x| / 127 (rows below 2^-100 become 0; a row with a NaN or an
+ * infinity gets the scale NaN). k_out and v_out (may be NULL) receive the rows before they are cut to 8 bits.
+ *
+ *  - in_type: F16, BF16, F32 or S32. out_type: F16 or BF16, of q_out, k_out and v_out; a 16-bit cache has the same.
+ *  - q may be NULL (with q_out); positions and inv_freq may be NULL where rotary_dim is 0 (even, at most head_dim).
+ *  - q_out may be q (k_out k, v_out v) with the same strides and a type of the same size; other overlaps are undefined.
+ *  - A token whose slot lies outside the cache (-1: padding) is not stored; its q_out, k_out, v_out are written.
+ *    Slots of one call differ: what a slot that two tokens name holds afterwards is undefined.
+ */
+typedef struct {
+  const void *q, *k, *v;                    /* [n_tokens][heads][head_dim] */
+  void *q_out, *k_out, *v_out;
+  const float *q_step, *k_step, *v_step;    /* [heads * head_dim], S32 only */
+  const int64_t *slots;                     /* [n_tokens] */
+  const int32_t *positions;                 /* [n_tokens] */
+  const double *inv_freq;                   /* [rotary_dim / 2], radians per position */
+  int64_t q_stride[2], k_stride[2], v_stride[2];             /* token, head */
+  int64_t q_out_stride[2], k_out_stride[2], v_out_stride[2];
+  int32_t n_tokens, n_q_heads, rotary_dim, interleaved, in_type, out_type;
+} pulpnn_kv_append_t;
+int pulpnn_kv_append(const pulpnn_kv_cache_t *cache, const pulpnn_kv_append_t *args);
+
+/*
+ * pulpnn_kv_gather -- rows slots[0 .. n_tokens) of the cache as 16-bit rows (S8: code * scale, rounded once). A slot
+ * outside the cache gives a row of zeros. out_type: F16 or BF16; a 16-bit cache has the same. k_out or v_out may be NULL.
+ */
+typedef struct {
+  const int64_t *slots;                     /* [n_tokens] */
+  void *k_out, *v_out;                      /* [n_tokens][n_heads][head_dim] */
+  int64_t k_out_stride[2], v_out_stride[2]; /* token, head */
+  int32_t n_tokens, out_type;
+} pulpnn_kv_gather_t;
+int pulpnn_kv_gather(const pulpnn_kv_cache_t *cache, const pulpnn_kv_gather_t *args);
+
+/*
+ * pulpnn_attn_decode -- attention of one new token per sequence over the cache:
+ * out[b][h] = sum over t of softmax(scale * q[b][h] . k[t]) v[t], where t runs over tokens 0 .. seq_lens[b] - 1 of
+ * sequence b (the last `window` of them where window > 0), token t lies in slot t % page_size of page
+ * block_table[b * table_stride + t / page_size], and query head h reads key head h / (n_heads / cache heads).
+ * lse (may be NULL, [n_seqs][n_heads]) receives the natural logarithm of the softmax's sum. A sequence without tokens
+ * gives zeros, and minus infinity in lse.
+ *
+ *  - q_type: F16 or BF16, the cache's where that is 16 bits wide. out_type: q_type, or U8: rint(out / out_step) + out_zero,
+ *    cut to 0 .. 255.
+ *  - Lengths are cut to 0 .. max_pages * page_size. A token whose page lies outside the cache is left out, as if masked.
+ *  - Scores, sums and the softmax are held in 32 bits; a token's weight is rounded to 16 bits for its product with v.
+ */
+typedef struct {
+  const void *q;                            /* [n_seqs][n_heads][head_dim] */
+  void *out;
+  float *lse;
+  const int32_t *block_table, *seq_lens;    /* [n_seqs][max_pages], [n_seqs] */
+  int64_t q_stride[2], out_stride[2], table_stride;          /* sequence, head */
+  float scale, out_step;
+  int32_t out_zero, q_type, out_type, n_seqs, n_heads, max_pages, window, reserved;
+} pulpnn_attn_decode_t;
+int pulpnn_attn_decode(const pulpnn_kv_cache_t *cache, const pulpnn_attn_decode_t *args);
+
+/*
+ * pulpnn_attn_prompt -- attention over whole prompts, packed one behind the other: sequence b holds rows cu_q[b] ..
+ * cu_q[b + 1] - 1 of q and out and rows cu_k[b] .. cu_k[b + 1] - 1 of k and v; query head h reads key head
+ * h / (n_heads / n_kv_heads). Query i of a sequence of Lq queries and Lk keys has the position i + Lk - Lq (keys that
+ * lie before a prompt's first query are its cached beginning). causal: it sees the keys 0 .. position; window > 0
+ * (causal only): the last `window` of these. lse as above, [n_q_rows][n_heads]. A query that sees no key gives zeros, and
+ * minus infinity in lse.
+ *
+ *  - type: F16 or BF16, of q, k and v. out_type: type, or U8 as above. scale > 0.
+ *  - What a query does not see does not reach its result, infinities and NaN there included.
+ *  - Offsets are cut to the rows there are; rows of out and lse that no sequence holds are left as they were.
+ *  - Scores, sums and the softmax are held in 32 bits; weights are rounded to 16 bits for their product with v.
+ */
+typedef struct {
+  const void *q, *k, *v;                    /* [rows][heads][head_dim] */
+  void *out;
+  float *lse;
+  const int32_t *cu_q, *cu_k;               /* [n_seqs + 1] */
+  int64_t q_stride[2], k_stride[2], v_stride[2], out_stride[2];      /* row, head */
+  float scale, out_step;
+  int32_t out_zero, type, out_type, n_q_rows, n_k_rows, n_seqs, n_heads, n_kv_heads, head_dim, causal, window, reserved;
+} pulpnn_attn_prompt_t;
+int pulpnn_attn_prompt(const pulpnn_attn_prompt_t *args);
+
 /* ---- sequential network runner --------------------------------------------
  * The reference is a kernel library; its user chains the calls. This runner is
  * that chain for one GPU: layers are appended in order, parameters are copied

@@ -395,6 +395,232 @@ def pulpnn_linear_out_32_static_scratch(pInBuffer, bias, pOutBuffer, pWeights, d
         raise PulpNNError(rc, "pulpnn_linear_out_32_static_scratch failed")
 
 
+# ---- attention over a paged cache of keys and values ------------------------------------------
+# The arguments go over as the C structs of include/pulpnn_b200.h, packed in one step; tensors are torch tensors on
+# the context's GPU (anything with data_ptr, shape, stride and dtype). Shapes and types are checked here, alignment,
+# ranges and whose memory it is by the library.
+TYPE_F16, TYPE_BF16, TYPE_F32, TYPE_S32, TYPE_S8, TYPE_U8 = range(6)
+_type_of = {}
+
+
+def _type(x):
+    code = _type_of.get(x.dtype)
+    if code is None:
+        if not _type_of:
+            import torch
+            _type_of.update({torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16, torch.float32: TYPE_F32,
+                             torch.int32: TYPE_S32, torch.int8: TYPE_S8, torch.uint8: TYPE_U8, torch.int64: -2,
+                             torch.float64: -3})
+            return _type(x)
+        raise PulpNNError(ERR_INVALID_ARG, "type %s" % x.dtype)
+    return code
+
+
+_TYPE_S64, _TYPE_F64 = -2, -3
+
+
+def _need(ok, what):
+    if not ok:
+        raise PulpNNError(ERR_INVALID_ARG, what)
+
+
+def _rows(x, name, n, heads, dim, type_, out=False):
+    """Address, token and head stride of [n][heads][dim] rows; an axis of one has the stride 0."""
+    _need(x.shape == (n, heads, dim), "%s has shape %s, not %s" % (name, tuple(x.shape), (n, heads, dim)))
+    _need(_type(x) == type_, "%s has type %s" % (name, x.dtype))
+    a, b, c = x.stride()
+    _need(c == 1 or dim == 1, "the channels of %s do not lie side by side" % name)
+    a, b = a if n > 1 else 0, b if heads > 1 else 0
+    _need(not out or (a != 0 or n <= 1) and (b != 0 or heads <= 1), "rows of %s share memory" % name)
+    return x.data_ptr(), a, b
+
+
+def _vector(x, name, n, type_):
+    """Address of n contiguous values, 0 for None."""
+    if x is None:
+        return 0
+    _need(x.shape == (n,) and x.is_contiguous(), "%s has shape %s, not (%d,) in one piece" % (name, tuple(x.shape), n))
+    _need(_type(x) == type_, "%s has type %s" % (name, x.dtype))
+    return x.data_ptr()
+
+
+class _StructCall:
+    """A C entry point that takes structs: call(struct, ...) raises what it records."""
+
+    def __init__(self, name, n):
+        self.name, self.n, self.f = name, n, None
+
+    def __call__(self, *blocks):
+        f = self.f
+        if f is None:
+            f = getattr(_lib.load_library(), self.name)
+            f.restype, f.argtypes = C.c_int, [C.c_char_p] * self.n
+            self.f = f
+        if f(*blocks) != OK:
+            _check()
+
+
+class KVCache:
+    """Pages of keys and values (pulpnn_kv_cache_t): k and v are [pages][slots][heads][dim], or [pages][heads][slots][dim]
+    with heads_first, of type float16, bfloat16 or int8 with equal strides; int8 has k_scale and v_scale, float32
+    without the last axis. The tensors stay the caller's, who keeps them on the GPU while calls use them."""
+
+    _pack = struct.Struct("=4Q6q6i").pack
+
+    def __init__(self, k, v, k_scale=None, v_scale=None, heads_first=False):
+        _need(k.dim() == 4 and k.shape == v.shape, "keys and values of shapes %s and %s" % (tuple(k.shape), tuple(v.shape)))
+        _need(k.dtype == v.dtype and k.stride() == v.stride(), "keys and values of different types or strides")
+        _need(k.stride(3) == 1, "the channels of a row do not lie side by side")
+        self.type, self.heads_first, self.tensors = _type(k), heads_first, (k, v, k_scale, v_scale)
+        pages, slots, heads, self.head_dim = k.shape
+        s, axes = k.stride(), (0, 1, 2)
+        if heads_first:
+            slots, heads, axes = heads, slots, (0, 2, 1)
+        self.n_pages, self.page_size, self.n_heads, t = pages, slots, heads, (0, 0, 0)
+        _need(all(n == 1 or st != 0 for n, st in zip(k.shape, s)), "rows of the cache share memory")
+        if self.type == TYPE_S8:
+            _need(k_scale is not None and v_scale is not None, "an int8 cache without scales")
+            _need(k_scale.shape == k.shape[:3] and v_scale.shape == k.shape[:3], "scales are shaped as the cache without its last axis")
+            _need(_type(k_scale) == TYPE_F32 and _type(v_scale) == TYPE_F32, "scales are float32")
+            _need(k_scale.stride() == v_scale.stride(), "scales with different strides")
+            t = k_scale.stride()
+            _need(all(n == 1 or st != 0 for n, st in zip(k.shape, t)), "scales share memory")
+        else:
+            _need(k_scale is None and v_scale is None, "scales of a 16-bit cache")
+        s = [s[i] if k.shape[i] > 1 else 0 for i in axes]
+        self.block = self._pack(k.data_ptr(), v.data_ptr(), _addr_of(k_scale), _addr_of(v_scale), *s, *(t[i] for i in axes), self.type,
+                                pages, slots, heads, self.head_dim, 0)
+
+
+def _addr_of(x):
+    return 0 if x is None else x.data_ptr()
+
+
+_append_pack = struct.Struct("=12Q12q6i").pack
+_append_call = _StructCall("pulpnn_kv_append", 2)
+_gather_pack = struct.Struct("=3Q4q2i").pack
+_gather_call = _StructCall("pulpnn_kv_gather", 2)
+_NO_ROWS = (0, 0, 0)
+
+
+def pulpnn_kv_append(cache, slots, k, v, positions=None, inv_freq=None, interleaved=False, q=None, q_out=None, k_out=None,
+                     v_out=None, q_step=None, k_step=None, v_step=None):
+    """Rotates q and k ([tokens][heads][dim]; float16, bfloat16, float32, or int32 with a float32 step per channel) by
+    positions (int32) x inv_freq (float64, half as many as channels rotate), writes q to q_out and stores k and v in the
+    cache at slots (int64; one outside the cache stores nothing). k_out, v_out: the stored rows before a cut to 8 bits."""
+    n, heads, dim = k.shape[0], cache.n_heads, cache.head_dim
+    if n == 0:
+        return
+    in_type = _type(k)
+    out_type = cache.type if cache.type != TYPE_S8 else None
+    for o in (q_out, k_out, v_out):
+        if out_type is None and o is not None:
+            out_type = _type(o)
+    if out_type is None:
+        out_type = TYPE_BF16                                # nothing of that type is written
+    pk, pv = _rows(k, "k", n, heads, dim, in_type), _rows(v, "v", n, heads, dim, in_type)
+    _need((q is None) == (q_out is None), "q and q_out come together")
+    pq, oq, hq = _NO_ROWS, _NO_ROWS, 0
+    if q is not None:
+        hq = q.shape[1]
+        pq, oq = _rows(q, "q", n, hq, dim, in_type), _rows(q_out, "q_out", n, hq, dim, out_type, True)
+    ok = _NO_ROWS if k_out is None else _rows(k_out, "k_out", n, heads, dim, out_type, True)
+    ov = _NO_ROWS if v_out is None else _rows(v_out, "v_out", n, heads, dim, out_type, True)
+    half = 0 if inv_freq is None else inv_freq.shape[0]
+    steps = (0, 0, 0)
+    if in_type == TYPE_S32:
+        _need(k_step is not None and v_step is not None and (q is None or q_step is not None), "int32 rows without steps")
+        steps = (_vector(q_step, "q_step", hq * dim, TYPE_F32), _vector(k_step, "k_step", heads * dim, TYPE_F32),
+                 _vector(v_step, "v_step", heads * dim, TYPE_F32))
+    else:
+        _need(q_step is None and k_step is None and v_step is None, "steps are for int32 rows")
+    _need(half == 0 or positions is not None, "a rotation without positions")
+    _append_call(cache.block, _append_pack(
+        pq[0], pk[0], pv[0], oq[0], ok[0], ov[0], *steps, _vector(slots, "slots", n, _TYPE_S64),
+        _vector(positions, "positions", n, TYPE_S32), _vector(inv_freq, "inv_freq", half, _TYPE_F64), pq[1], pq[2], pk[1], pk[2],
+        pv[1], pv[2], oq[1], oq[2], ok[1], ok[2], ov[1], ov[2], n, hq, 2 * half, 1 if interleaved else 0, in_type, out_type))
+
+
+def pulpnn_kv_gather(cache, slots, k_out, v_out=None):
+    """Rows `slots` (int64) of the cache into k_out and v_out ([tokens][heads][dim], float16 or bfloat16; either may be
+    None). A slot outside the cache gives zeros."""
+    n = slots.shape[0]
+    if n == 0:
+        return
+    first = k_out if k_out is not None else v_out
+    _need(first is not None, "neither k_out nor v_out")
+    out_type = _type(first)
+    a, b = (_NO_ROWS if x is None else _rows(x, name, n, cache.n_heads, cache.head_dim, out_type, True)
+            for x, name in ((k_out, "k_out"), (v_out, "v_out")))
+    _gather_call(cache.block, _gather_pack(_vector(slots, "slots", n, _TYPE_S64), a[0], b[0], a[1], a[2], b[1], b[2], n, out_type))
+
+
+_decode_pack = struct.Struct("=5Q5q2f8i").pack
+_decode_call = _StructCall("pulpnn_attn_decode", 2)
+
+
+def _out_type(out, in_type, out_step):
+    """The type of an attention's output: the queries', or uint8 with a step."""
+    type_ = _type(out)
+    _need(type_ == in_type or type_ == TYPE_U8, "out has type %s" % out.dtype)
+    _need((type_ == TYPE_U8) == (out_step is not None), "uint8 outputs, and only these, have an out_step")
+    return type_
+
+
+def pulpnn_attn_decode(cache, q, block_table, seq_lens, out, scale=None, window=0, lse=None, out_step=None, out_zero=0):
+    """Attention of one new token per sequence: q and out [sequences][heads][dim], block_table int32 [sequences][pages],
+    seq_lens int32 [sequences]. scale: dim ** -0.5 unless given. window > 0: the last `window` tokens only. lse: float32
+    [sequences][heads]. out has q's type, or uint8 with out_step (and out_zero)."""
+    n, heads, dim = q.shape
+    if n == 0:
+        return
+    q_type = _type(q)
+    out_type = _out_type(out, q_type, out_step)
+    _need(dim == cache.head_dim, "q has %d channels, the cache %d" % (dim, cache.head_dim))
+    a, b = _rows(q, "q", n, heads, dim, q_type), _rows(out, "out", n, heads, dim, out_type, True)
+    _need(block_table.dim() == 2 and block_table.shape[0] == n and _type(block_table) == TYPE_S32, "block_table is int32 [sequences][pages]")
+    pages = block_table.shape[1]
+    _need(pages <= 1 or block_table.stride(1) == 1, "the pages of a sequence do not lie side by side in block_table")
+    _decode_call(cache.block, _decode_pack(
+        a[0], b[0], _lse(lse, n, heads), block_table.data_ptr() if pages else seq_lens.data_ptr(), _vector(seq_lens, "seq_lens", n, TYPE_S32),
+        a[1], a[2], b[1], b[2], block_table.stride(0) if n > 1 else 0, dim ** -0.5 if scale is None else scale,
+        out_step or 0., out_zero, q_type, out_type, n, heads, pages, window, 0))
+
+
+def _lse(lse, n, heads):
+    if lse is None:
+        return 0
+    _need(lse.shape == (n, heads) and lse.is_contiguous() and _type(lse) == TYPE_F32, "lse is float32 [%d][%d] in one piece" % (n, heads))
+    return lse.data_ptr()
+
+
+_prompt_pack = struct.Struct("=7Q8q2f12i").pack
+_prompt_call = _StructCall("pulpnn_attn_prompt", 1)
+
+
+def pulpnn_attn_prompt(q, k, v, cu_q, out, cu_k=None, causal=True, window=0, scale=None, lse=None, out_step=None, out_zero=0):
+    """Attention over whole prompts: sequence b holds rows cu_q[b] .. cu_q[b+1] of q and out ([rows][heads][dim]) and rows
+    cu_k[b] .. cu_k[b+1] (cu_q's unless given) of k and v. Its last query and its last key have the same position.
+    causal: no query sees a later position; window > 0 (causal only): nor one `window` or more before its own."""
+    n, heads, dim = q.shape
+    if n == 0:
+        return
+    nk, kv_heads = k.shape[0], k.shape[1]
+    type_ = _type(q)
+    out_type = _out_type(out, type_, out_step)
+    rows = [_rows(q, "q", n, heads, dim, type_), _rows(k, "k", nk, kv_heads, dim, type_), _rows(v, "v", nk, kv_heads, dim, type_),
+            _rows(out, "out", n, heads, dim, out_type, True)]
+    seqs = cu_q.shape[0] - 1
+    if cu_k is None:
+        _need(nk == n, "%d rows of keys for %d of queries, and no cu_k" % (nk, n))
+        cu_k = cu_q
+    _prompt_call(_prompt_pack(
+        rows[0][0], rows[1][0], rows[2][0], rows[3][0], _lse(lse, n, heads), _vector(cu_q, "cu_q", seqs + 1, TYPE_S32),
+        _vector(cu_k, "cu_k", seqs + 1, TYPE_S32), rows[0][1], rows[0][2], rows[1][1], rows[1][2], rows[2][1], rows[2][2], rows[3][1],
+        rows[3][2], dim ** -0.5 if scale is None else scale, out_step or 0., out_zero, type_, out_type, n, nk, seqs, heads, kv_heads, dim,
+        1 if causal else 0, window, 0))
+
+
 # ---- network runner --------------------------------------------------------------------------
 class LayerDesc(C.Structure):
     _fields_ = [(n, C.c_int) for n in (

@@ -1,0 +1,546 @@
+// attn_decode.cu -- pulpnn_attn_decode: one new token per sequence against a paged cache of keys and values.
+//
+//   o[b][h] = sum_t w_t v[t],  w = softmax over t of scale * (q[b][h] . k[t]),  t the last `window` tokens of sequence b.
+//
+// Every key and value is read once and used for the G query heads that share it: 4 G operations on 2 or 4 bytes, so the
+// kernel is bound by memory as long as the arithmetic stays out of the way. That is on the tensor cores
+// (mma.m16n8k16): S^T = K Q^T with 16 tokens as the rows and 8 query heads as the columns, and O^T = V^T P^T with 16
+// channels as the rows. With the heads as columns a group of up to 8 wastes half as much as it would as rows, and the
+// weights only have to be transposed in 8x8 blocks (movmatrix) on their way from the one product to the other. tcgen05
+// would want 128 rows, M = tokens, for 16 bytes of results each: it reads its operands from shared memory just the
+// same, and its accumulators would have to come back through TMEM for the running maximum.
+//
+// A warp works alone: tiles of 16 (8-bit: 32) tokens, fetched by itself with 16-byte cp.async into STAGES buffers of its own;
+// there is no barrier between warps until the end. Each lane looks up the page of one token, one tile ahead of
+// its fetch, so pages of any size may end anywhere in a tile, and tokens behind the end are filled with zeros
+// without being read. WARPS warps are a CTA, CTAs of a cluster share a sequence, and the partial results are joined
+// through (distributed) shared memory in a fixed order: no workspace, no atomics, the same result every time.
+//
+// Running maximum: the reference m only has to be near the true maximum, not equal to it. It is raised (and the sums
+// rescaled) when some score is more than 2^LAG above it, which one vote per tile finds out; the weights stay
+// below 2^LAG, far from the end of the 16-bit types' range, and the sums are kept in 32 bits.
+//
+// 8-bit caches: codes are exact in fp16, so K's product is exact but for q, whose rows are scaled by a power of two
+// to a maximum of 1 .. 2 (bf16 queries lose nothing that matters: 2^-24 of the row's maximum). The key's scale
+// multiplies the score. The value's scale multiplies the weight before it is rounded to fp16; such weights get a reference of
+// their own, the running maximum of score + log2(scale), so that they keep fp16's 11 bits whatever the scales are.
+#include <cooperative_groups.h>
+
+#include "attention.cuh"
+#include "sm100_primitives.cuh"
+
+namespace pulpnn {
+namespace attn {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int WARPS = 4, STAGES = 3;
+constexpr float LAG = 8.f, NOTHING = -1e30f;
+
+struct DecodeProblem {
+  const char *q;
+  char *out;
+  float *lse;
+  const int *table, *lens;
+  int64_t q_seq, q_head, out_seq, out_head;      // bytes
+  int64_t table_stride;
+  CacheView cache;
+  int hq, group, head_tiles, dim, max_pages, window, q_type, out_type;
+  float scale_log2, out_inv_step;
+  int out_zero, splits;
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool live)
+{
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, bool live)
+{
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldmatrix4(uint32_t a, unsigned (&r)[4])
+{
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t a, unsigned (&r)[4])
+{
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ unsigned transpose8(unsigned a)
+{
+  unsigned d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ unsigned lds32(uint32_t a)
+{
+  unsigned v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float ex2(float x)
+{
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T> __device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1);
+template <> __device__ __forceinline__ void mma<__half>(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1)
+{
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1)
+{
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Signed bytes as fp16: the byte plus 128 in the low bits of 1024 is 1152 + code, exactly.
+__device__ __forceinline__ unsigned widen(unsigned biased, unsigned select)
+{
+  const unsigned w = __byte_perm(biased, 0x64646464u, select), off = 0x64806480u;
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&w), *reinterpret_cast<const __half2 *>(&off));
+  return *reinterpret_cast<const unsigned *>(&r);
+}
+__device__ __forceinline__ float load_q(const char *p, int type)
+{
+  return type == PULPNN_TYPE_F16 ? __half2float(*reinterpret_cast<const __half *>(p)) : __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(p));
+}
+
+template <int DP, bool EIGHT> struct Tile {
+  static constexpr int SIZE = EIGHT ? 1 : 2;
+  static constexpr int TOKENS = EIGHT ? 32 : 16;
+  static constexpr int ROW = DP * SIZE + 16;                 // padded: 8 rows of one 16-byte column lie in different banks
+  static constexpr int CHUNKS = DP * SIZE / 16;              // of a row
+  static constexpr int STAGE = 2 * TOKENS * ROW + (EIGHT ? 2 * TOKENS * 4 : 0);
+  static constexpr int PIPE = WARPS * STAGES * STAGE;
+};
+// what the join needs, in the pipeline's place: per warp [heads][DP] sums, then the CTA's
+template <int DP, int NT> struct Join {
+  static constexpr int HEADS = NT * 8, PITCH = DP + 4;
+  static constexpr int WARP = HEADS * PITCH;                 // floats
+  static constexpr int STATS = 3 * HEADS;                    // m, l, reference of the sums
+  static constexpr int BYTES = (WARPS * (WARP + STATS) + WARP + STATS) * 4;
+};
+template <int DP, int NT, bool EIGHT> constexpr int decode_smem()
+{
+  return Tile<DP, EIGHT>::PIPE > Join<DP, NT>::BYTES ? Tile<DP, EIGHT>::PIPE : Join<DP, NT>::BYTES;
+}
+
+template <typename T, int DP, int NT, bool EIGHT>
+__global__ void __launch_bounds__(WARPS * 32) attn_decode_kernel(const DecodeProblem p)
+{
+  using TL = Tile<DP, EIGHT>;
+  using JN = Join<DP, NT>;
+  constexpr int KS = DP / 16, MT = TL::TOKENS / 16, COPIES = TL::TOKENS * TL::CHUNKS / 32;
+  extern __shared__ __align__(128) char smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = blockIdx.x % p.splits;
+  int rest = blockIdx.x / p.splits;
+  const int ht = rest % p.head_tiles; rest /= p.head_tiles;
+  const int kvh = rest % p.cache.n_heads, seq = rest / p.cache.n_heads;
+  const int h0 = kvh * p.group + ht * NT * 8, heads = min(NT * 8, p.group - ht * NT * 8);
+
+  if (p.dim < DP) {       // channels behind the head's own stay zero: a NaN there would spoil the product with q's zeros
+    for (int i = threadIdx.x; i < TL::PIPE / 16; i += WARPS * 32) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+  }
+  pdl_wait();
+  const int n = min(max(__ldg(p.lens + seq), 0), p.max_pages * p.cache.page_size);
+  const int first = p.window > 0 ? max(0, n - p.window) : 0;
+  const int tiles = (n - first + TL::TOKENS - 1) / TL::TOKENS;
+  const int lo = (int)((int64_t)tiles * rank / p.splits), hi = (int)((int64_t)tiles * (rank + 1) / p.splits);
+  const int mine = hi - lo > warp ? (hi - lo - warp + WARPS - 1) / WARPS : 0;       // tiles lo + warp + i * WARPS
+
+  const uint32_t pipe = sm100::smem_u32(smem) + warp * STAGES * TL::STAGE;
+  const int *table = p.table + seq * p.table_stride;
+  // the page of this lane's token of tile i; -1 where there is none
+  auto page_of = [&](int i, int &at) -> int {
+    const int token = first + (lo + warp + i * WARPS) * TL::TOKENS + (lane & (TL::TOKENS - 1));
+    at = 0;
+    if (i >= mine || token >= n) return -1;
+    const int in_row = p.cache.by_page.div(token), page = __ldg(table + in_row);
+    at = token - in_row * p.cache.page_size;
+    return page >= 0 && page < p.cache.n_pages ? page : -1;
+  };
+  unsigned live_ring = 0;      // STAGES words of bits would be as good: bit (stage) of lane's token
+  auto fetch = [&](int i, int page, int at) {
+    const int stage = i % STAGES;
+    const uint32_t base = pipe + stage * TL::STAGE;
+    const bool live = page >= 0;
+    const int64_t off = live ? row_of(p.cache, page, at, kvh) * TL::SIZE : 0;
+    live_ring = (live_ring & ~(1u << stage)) | (live ? 1u << stage : 0u);
+    if (i < mine) {
+#pragma unroll
+      for (int j = 0; j < COPIES; j++) {
+        const int item = lane + 32 * j, row = item / TL::CHUNKS, chunk = item % TL::CHUNKS;
+        const int64_t o = __shfl_sync(0xffffffffu, off, row);
+        const bool ok = __shfl_sync(0xffffffffu, live, row);
+        if (chunk * 16 < p.dim * TL::SIZE) {
+          cp_async16(base + row * TL::ROW + chunk * 16, p.cache.k + (ok ? o + chunk * 16 : 0), ok);
+          cp_async16(base + (TL::TOKENS + row) * TL::ROW + chunk * 16, p.cache.v + (ok ? o + chunk * 16 : 0), ok);
+        }
+      }
+      if (EIGHT) {
+        const int64_t s = live ? scale_of(p.cache, page, at, kvh) : 0;
+        cp_async4(base + 2 * TL::TOKENS * TL::ROW + lane * 4, p.cache.k_scale + s, live);
+        cp_async4(base + 2 * TL::TOKENS * TL::ROW + (32 + lane) * 4, p.cache.v_scale + s, live);
+      }
+    }
+    cp_commit();
+  };
+  int page_next, at_next;
+  {
+    int page[STAGES], at[STAGES];
+#pragma unroll
+    for (int i = 0; i < STAGES; i++) page[i] = page_of(i, at[i]);
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; i++) fetch(i, page[i], at[i]);
+    page_next = page[STAGES - 1]; at_next = at[STAGES - 1];
+  }
+
+  // q as the second operand: head g of each tile of 8, channels 16 ks + {2t, 2t+1} and {2t+8, 2t+9}; 8-bit: 4t .. 4t+3
+  unsigned qf[NT][KS][2];
+  float q_scale[NT][2];        // of this thread's heads 2t, 2t+1 in the accumulators
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    const bool live = nt * 8 + g < heads;
+    const char *row = p.q + seq * p.q_seq + (int64_t)(h0 + nt * 8 + g) * p.q_head;
+    if (!EIGHT) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          const int c = ks * 16 + half * 8 + 2 * t;
+          qf[nt][ks][half] = live && c < p.dim ? *reinterpret_cast<const unsigned *>(row + c * 2) : 0u;
+        }
+      q_scale[nt][0] = q_scale[nt][1] = p.scale_log2;
+    } else {
+      float x[KS][4], most = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int c = ks * 16 + 4 * t + e;
+          x[ks][e] = live && c < p.dim ? load_q(row + c * 2, p.q_type) : 0.f;
+          most = fmaxf(most, fabsf(x[ks][e]));
+        }
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      // the power of two at or below the row's maximum (1 for a row of zeros, infinities or the smallest numbers)
+      const unsigned e = (__float_as_uint(most) >> 23) & 255u;
+      const float up = e >= 1 && e <= 253 ? __uint_as_float((254u - e) << 23) : 1.f, down = e >= 1 && e <= 253 ? __uint_as_float(e << 23) : 1.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+        for (int half = 0; half < 2; half++) qf[nt][ks][half] = pack2<__half>(x[ks][2 * half] * up, x[ks][2 * half + 1] * up);
+#pragma unroll
+      for (int c = 0; c < 2; c++) q_scale[nt][c] = __shfl_sync(0xffffffffu, down, (2 * t + c) * 4) * p.scale_log2;
+    }
+  }
+
+  float o[NT][KS][4], m[NT][2], l[NT][2], ref[NT][2];       // ref: the reference of the sums o; m's own where a cache is 16 bits wide
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[nt][ks][e] = 0.f;
+    m[nt][0] = m[nt][1] = ref[nt][0] = ref[nt][1] = NOTHING;
+    l[nt][0] = l[nt][1] = 0.f;
+  }
+
+  for (int i = 0; i < mine; i++) {
+    fetch(i + STAGES - 1, page_next, at_next);
+    page_next = page_of(i + STAGES, at_next);
+    cp_wait<STAGES - 1>();
+    __syncwarp();
+    const uint32_t base = pipe + (i % STAGES) * TL::STAGE, vbase = base + TL::TOKENS * TL::ROW, sbase = base + 2 * TL::TOKENS * TL::ROW;
+    const unsigned live = __ballot_sync(0xffffffffu, (live_ring >> (i % STAGES)) & 1u);
+
+    // S^T: tokens 16 mt + {g, g + 8} x heads 8 nt + {2t, 2t + 1}
+    float s[MT][NT][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[mt][nt][e] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) {
+        unsigned a[4];
+        if (EIGHT) {
+          const unsigned w0 = lds32(base + (mt * 16 + g) * TL::ROW + ks * 16 + 4 * t) ^ 0x80808080u;
+          const unsigned w1 = lds32(base + (mt * 16 + 8 + g) * TL::ROW + ks * 16 + 4 * t) ^ 0x80808080u;
+          a[0] = widen(w0, 0x4140); a[1] = widen(w1, 0x4140); a[2] = widen(w0, 0x4342); a[3] = widen(w1, 0x4342);
+        } else {
+          ldmatrix4(base + (mt * 16 + (lane & 15)) * TL::ROW + ks * 32 + (lane >> 4) * 16, a);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) mma<T>(s[mt][nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+      }
+    }
+    float vs[MT][2], lvs[MT][2];
+    bool over = false;
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const int token = mt * 16 + r * 8 + g;
+        const bool ok = (live >> token) & 1u;
+        float ks_ = 1.f;
+        if (EIGHT) {
+          ks_ = __uint_as_float(lds32(sbase + token * 4));
+          vs[mt][r] = __uint_as_float(lds32(sbase + (32 + token) * 4));
+          lvs[mt][r] = __log2f(fabsf(vs[mt][r]));
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            float &x = s[mt][nt][2 * r + c];
+            x = ok ? x * (EIGHT ? q_scale[nt][c] * ks_ : q_scale[nt][c]) : -INFINITY;
+            over |= x > m[nt][c] + LAG;
+            if (EIGHT) over |= x + lvs[mt][r] > ref[nt][c] + LAG;
+          }
+      }
+    if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          float a = m[nt][c], b = ref[nt][c];
+#pragma unroll
+          for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+              a = fmaxf(a, s[mt][nt][2 * r + c]);
+              if (EIGHT) b = fmaxf(b, s[mt][nt][2 * r + c] + lvs[mt][r]);
+            }
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2) {
+            a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
+            if (EIGHT) b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, d));
+          }
+          if (!EIGHT) b = a;
+          l[nt][c] *= ex2(m[nt][c] - a);
+          const float f = ex2(ref[nt][c] - b);
+          m[nt][c] = a; ref[nt][c] = b;
+          // column 2t + c of the accumulators is this thread's in every row
+#pragma unroll
+          for (int ks = 0; ks < KS; ks++) { o[nt][ks][c] *= f; o[nt][ks][2 + c] *= f; }
+        }
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+      unsigned b[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          float w[2];
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            const float x = s[mt][nt][2 * r + c], e = ex2(x - m[nt][c]);
+            l[nt][c] += e;
+            // rounded to 16 bits for the product with V: off by 2^-8 (bf16) or 2^-11 (fp16) at most; the sum l takes it unrounded
+            w[c] = EIGHT ? (vs[mt][r] == vs[mt][r] ? ex2(x + lvs[mt][r] - ref[nt][c]) : vs[mt][r]) : e;
+            if (EIGHT && vs[mt][r] < 0.f) w[c] = -w[c];
+          }
+          b[nt][r] = transpose8(pack2<T>(w[0], w[1]));
+        }
+      // O^T += V^T P^T
+      if (EIGHT) {
+#pragma unroll
+        for (int blk = 0; blk < DP / 32; blk++) {
+          const uint32_t v = vbase + (mt * 16 + 2 * t) * TL::ROW + blk * 32 + 4 * g;
+          const unsigned w0 = lds32(v) ^ 0x80808080u, w1 = lds32(v + TL::ROW) ^ 0x80808080u;
+          const unsigned w2 = lds32(v + 8 * TL::ROW) ^ 0x80808080u, w3 = lds32(v + 9 * TL::ROW) ^ 0x80808080u;
+          const unsigned x0 = __byte_perm(w0, w1, 0x5140), x1 = __byte_perm(w0, w1, 0x7362);
+          const unsigned y0 = __byte_perm(w2, w3, 0x5140), y1 = __byte_perm(w2, w3, 0x7362);
+          const unsigned a0[4] = {widen(x0, 0x4140), widen(x0, 0x4342), widen(y0, 0x4140), widen(y0, 0x4342)};
+          const unsigned a1[4] = {widen(x1, 0x4140), widen(x1, 0x4342), widen(y1, 0x4140), widen(y1, 0x4342)};
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) {
+            mma<T>(o[nt][2 * blk], a0, b[nt][0], b[nt][1]);
+            mma<T>(o[nt][2 * blk + 1], a1, b[nt][0], b[nt][1]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+          unsigned a[4];
+          // matrices: (tokens 0-7, channels 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15), each transposed
+          ldmatrix4_trans(vbase + (mt * 16 + (lane & 7) + (lane >> 4) * 8) * TL::ROW + ks * 32 + ((lane >> 3) & 1) * 16, a);
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) mma<T>(o[nt][ks], a, b[nt][0], b[nt][1]);
+        }
+      }
+    }
+    __syncwarp();          // the buffer is free for the fetch of the next turn
+  }
+  cp_wait<0>();
+
+  // ---- join: warps, then CTAs of the cluster -----------------------------------------------------
+  __syncthreads();         // the pipeline's memory is free
+  float *sums = reinterpret_cast<float *>(smem), *stats = sums + WARPS * JN::WARP;
+  float *cta_sums = stats + WARPS * JN::STATS, *cta_stats = cta_sums + JN::WARP;
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      float x = l[nt][c];
+#pragma unroll
+      for (int d = 4; d < 32; d *= 2) x += __shfl_xor_sync(0xffffffffu, x, d);
+      const int head = nt * 8 + 2 * t + c;
+      float *st = stats + warp * JN::STATS;
+      if (g == 0) { st[head] = m[nt][c]; st[JN::HEADS + head] = x; st[2 * JN::HEADS + head] = ref[nt][c]; }
+      float *dst = sums + warp * JN::WARP + head * JN::PITCH;
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          const int ch = EIGHT ? (ks >> 1) * 32 + 4 * g + 2 * (ks & 1) + r : ks * 16 + r * 8 + g;
+          dst[ch] = o[nt][ks][2 * r + c];
+        }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < JN::HEADS * DP / 4; i += WARPS * 32) {
+    const int head = i / (DP / 4), ch = i % (DP / 4) * 4;
+    if (head >= heads) continue;
+    float M = NOTHING, R = NOTHING, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+      M = fmaxf(M, stats[w * JN::STATS + head]);
+      R = fmaxf(R, stats[w * JN::STATS + 2 * JN::HEADS + head]);
+    }
+    float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+      const float *st = stats + w * JN::STATS;
+      L += st[JN::HEADS + head] * ex2(st[head] - M);
+      const float f = ex2(st[2 * JN::HEADS + head] - R);
+      const float4 x = *reinterpret_cast<const float4 *>(sums + w * JN::WARP + head * JN::PITCH + ch);
+      acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
+    }
+    *reinterpret_cast<float4 *>(cta_sums + head * JN::PITCH + ch) = acc;
+    if (ch == 0) { cta_stats[head] = M; cta_stats[JN::HEADS + head] = L; cta_stats[2 * JN::HEADS + head] = R; }
+  }
+  cluster.sync();
+  // each CTA writes its share of the outputs, from every CTA's sums
+  for (int i = threadIdx.x + rank * WARPS * 32; i < heads * (p.dim / 4); i += p.splits * WARPS * 32) {
+    const int head = i / (p.dim / 4), ch = i % (p.dim / 4) * 4;
+    float M = NOTHING, R = NOTHING, L = 0.f;
+    for (int r = 0; r < p.splits; r++) {
+      const float *st = cluster.map_shared_rank(cta_stats, r);
+      M = fmaxf(M, st[head]);
+      R = fmaxf(R, st[2 * JN::HEADS + head]);
+    }
+    float4 acc = make_float4(0, 0, 0, 0);
+    for (int r = 0; r < p.splits; r++) {
+      const float *st = cluster.map_shared_rank(cta_stats, r);
+      L += st[JN::HEADS + head] * ex2(st[head] - M);
+      const float f = ex2(st[2 * JN::HEADS + head] - R);
+      const float4 x = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(cta_sums, r) + head * JN::PITCH + ch);
+      acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
+    }
+    const float f = L == 0.f ? 0.f : (EIGHT ? ex2(R - M) : 1.f) / L;      // a row that sees nothing is zero
+    const float y[4] = {acc.x * f, acc.y * f, acc.z * f, acc.w * f};
+    char *dst = p.out + seq * p.out_seq + (int64_t)(h0 + head) * p.out_head;
+    store4(dst, ch, p.out_type, y, p.out_inv_step, p.out_zero);
+    if (p.lse && ch == 0) p.lse[(int64_t)seq * p.hq + h0 + head] = (M + log2f(L)) * 0.69314718055994530942f;
+  }
+  cluster.sync();          // no CTA leaves while another reads its sums
+}
+
+template <typename T, int DP, int NT, bool EIGHT>
+bool decode_go(Context &c, const DecodeProblem &p, int64_t pairs)
+{
+  constexpr int smem = decode_smem<DP, NT, EIGHT>();
+  auto k = attn_decode_kernel<T, DP, NT, EIGHT>;
+  static PerDeviceInt ready;
+  if (!ready.get(c.device)) {
+    if (!cuda_ok(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute(attn_decode)")) return false;
+    ready.set(c.device, 1);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(pairs * p.splits)); cfg.blockDim = dim3(WARPS * 32); cfg.dynamicSmemBytes = smem; cfg.stream = c.stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr; cfg.numAttrs = 2;
+  if (!cuda_ok(cudaLaunchKernelEx(&cfg, k, p), "pulpnn_attn_decode")) return false;
+  count_launch("attn_decode_kernel");
+  return true;
+}
+template <typename T, bool EIGHT>
+bool decode_dim(Context &c, const DecodeProblem &p, int64_t pairs, bool two)
+{
+  if (p.dim <= 64) return two ? decode_go<T, 64, 2, EIGHT>(c, p, pairs) : decode_go<T, 64, 1, EIGHT>(c, p, pairs);
+  if (p.dim <= 96) return two ? decode_go<T, 96, 2, EIGHT>(c, p, pairs) : decode_go<T, 96, 1, EIGHT>(c, p, pairs);
+  return two ? decode_go<T, 128, 2, EIGHT>(c, p, pairs) : decode_go<T, 128, 1, EIGHT>(c, p, pairs);
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace pulpnn
+
+using namespace pulpnn;
+using namespace pulpnn::attn;
+
+extern "C" int pulpnn_attn_decode(const pulpnn_kv_cache_t *cache, const pulpnn_attn_decode_t *a)
+{
+  const char *who = "pulpnn_attn_decode";
+  Context &c = ctx();
+  if (const int e = check_cache(who, cache)) return e;
+  ATTN_REQUIRE(a && a->n_seqs >= 0, PULPNN_ERR_INVALID_ARG, "%s: %d sequences", who, a ? a->n_seqs : -1);
+  if (a->n_seqs == 0) return PULPNN_OK;
+  ATTN_REQUIRE(a->q && a->out && a->block_table && a->seq_lens, PULPNN_ERR_INVALID_ARG, "%s: NULL pointer", who);
+  ATTN_REQUIRE(is_wide(a->q_type) && (cache->type == PULPNN_TYPE_S8 || cache->type == a->q_type), PULPNN_ERR_UNSUPPORTED,
+               "%s: q_type %d with a cache of type %d", who, a->q_type, cache->type);
+  ATTN_REQUIRE(a->out_type == a->q_type || a->out_type == PULPNN_TYPE_U8, PULPNN_ERR_UNSUPPORTED, "%s: out_type %d is neither q_type nor U8", who, a->out_type);
+  ATTN_REQUIRE(a->n_heads > 0 && a->n_heads % cache->n_heads == 0, PULPNN_ERR_INVALID_ARG, "%s: %d query heads for %d key heads", who,
+               a->n_heads, cache->n_heads);
+  ATTN_REQUIRE(a->max_pages >= 0 && a->window >= 0, PULPNN_ERR_INVALID_ARG, "%s: max_pages %d, window %d", who, a->max_pages, a->window);
+  ATTN_REQUIRE((int64_t)a->max_pages * cache->page_size <= 0x7fffff00, PULPNN_ERR_UNSUPPORTED, "%s: sequences of 2^31 tokens", who);
+  if (const int e = check_scale(who, a->scale)) return e;
+  if (const int e = check_out(who, a->out_type, a->out_step, a->out_zero)) return e;
+  ATTN_REQUIRE(rows_aligned(a->q, 2, {a->q_stride[0], a->q_stride[1]}) &&
+               out_aligned(a->out, a->out_type, a->out_stride[0], a->out_stride[1]), PULPNN_ERR_UNSUPPORTED,
+               "%s: rows that do not begin on 16-byte boundaries", who);
+  ATTN_REQUIRE(aligned(a->block_table, 4) && aligned(a->seq_lens, 4) && aligned(a->lse, 4), PULPNN_ERR_INVALID_ARG, "%s: unaligned table, lengths or lse", who);
+  if (!ensure_device(c)) return c.err;
+  if (!on_device(c, who, {cache->k, cache->v, cache->k_scale, cache->v_scale, a->q, a->out, a->lse, a->block_table, a->seq_lens})) return c.err;
+
+  DecodeProblem p;
+  p.q = static_cast<const char *>(a->q); p.out = static_cast<char *>(a->out); p.lse = a->lse;
+  p.table = a->block_table; p.lens = a->seq_lens;
+  const int os = type_size(a->out_type);
+  p.q_seq = a->q_stride[0] * 2; p.q_head = a->q_stride[1] * 2; p.out_seq = a->out_stride[0] * os; p.out_head = a->out_stride[1] * os;
+  p.table_stride = a->table_stride;
+  p.cache = view_of(*cache);
+  p.hq = a->n_heads; p.group = a->n_heads / cache->n_heads; p.dim = cache->head_dim; p.max_pages = a->max_pages; p.window = a->window;
+  p.q_type = a->q_type; p.out_type = a->out_type;
+  p.scale_log2 = a->scale * 1.4426950408889634074f;
+  p.out_inv_step = a->out_type == PULPNN_TYPE_U8 ? 1.f / a->out_step : 1.f; p.out_zero = a->out_zero;
+  const bool two = p.group > 8;
+  p.head_tiles = (p.group + (two ? 15 : 7)) / (two ? 16 : 8);
+  const int64_t pairs = (int64_t)a->n_seqs * cache->n_heads * p.head_tiles;
+  ATTN_REQUIRE(pairs <= 0x0fffffff, PULPNN_ERR_UNSUPPORTED, "%s: %d sequences of %d heads", who, a->n_seqs, a->n_heads);
+  // CTAs of a sequence: no more than leave each warp two tiles of the longest one
+  int64_t most = (int64_t)a->max_pages * cache->page_size;
+  if (a->window > 0 && a->window < most) most = a->window;
+  const int tile = cache->type == PULPNN_TYPE_S8 ? 32 : 16;
+  p.splits = 1;
+  while (p.splits < 8 && most > (int64_t)p.splits * WARPS * tile * 2) p.splits *= 2;
+  const bool ok = cache->type == PULPNN_TYPE_S8 ? decode_dim<__half, true>(c, p, pairs, two)
+                  : (a->q_type == PULPNN_TYPE_F16 ? decode_dim<__half, false>(c, p, pairs, two) : decode_dim<__nv_bfloat16, false>(c, p, pairs, two));
+  return ok ? PULPNN_OK : c.err;
+}
