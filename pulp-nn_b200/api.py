@@ -426,12 +426,13 @@ def _need(ok, what):
 
 def _rows(x, name, n, heads, dim, type_, out=False):
     """Address, token and head stride of [n][heads][dim] rows; an axis of one has the stride 0."""
-    _need(x.shape == (n, heads, dim), "%s has shape %s, not %s" % (name, tuple(x.shape), (n, heads, dim)))
-    _need(_type(x) == type_, "%s has type %s" % (name, x.dtype))
     a, b, c = x.stride()
-    _need(c == 1 or dim == 1, "the channels of %s do not lie side by side" % name)
+    if x.shape != (n, heads, dim) or _type_of.get(x.dtype) != type_ or c != 1:
+        raise PulpNNError(ERR_INVALID_ARG, "%s: %s %s with strides %s, where rows of %s are wanted" % (
+            name, x.dtype, tuple(x.shape), x.stride(), (n, heads, dim)))
     a, b = a if n > 1 else 0, b if heads > 1 else 0
-    _need(not out or (a != 0 or n <= 1) and (b != 0 or heads <= 1), "rows of %s share memory" % name)
+    if out and (a == 0 and n > 1 or b == 0 and heads > 1):
+        raise PulpNNError(ERR_INVALID_ARG, "rows of %s share memory" % name)
     return x.data_ptr(), a, b
 
 
@@ -439,8 +440,8 @@ def _vector(x, name, n, type_):
     """Address of n contiguous values, 0 for None."""
     if x is None:
         return 0
-    _need(x.shape == (n,) and x.is_contiguous(), "%s has shape %s, not (%d,) in one piece" % (name, tuple(x.shape), n))
-    _need(_type(x) == type_, "%s has type %s" % (name, x.dtype))
+    if x.shape != (n,) or not x.is_contiguous() or _type(x) != type_:
+        raise PulpNNError(ERR_INVALID_ARG, "%s: %s %s, where %d values in one piece are wanted" % (name, x.dtype, tuple(x.shape), n))
     return x.data_ptr()
 
 
@@ -562,7 +563,7 @@ _decode_call = _StructCall("pulpnn_attn_decode", 2)
 def _out_type(out, in_type, out_step):
     """The type of an attention's output: the queries', or uint8 with a step."""
     type_ = _type(out)
-    _need(type_ == in_type or type_ == TYPE_U8, "out has type %s" % out.dtype)
+    _need(type_ == in_type or type_ == TYPE_U8, "out is neither of q's type nor uint8")
     _need((type_ == TYPE_U8) == (out_step is not None), "uint8 outputs, and only these, have an out_step")
     return type_
 
@@ -576,7 +577,7 @@ def pulpnn_attn_decode(cache, q, block_table, seq_lens, out, scale=None, window=
         return
     q_type = _type(q)
     out_type = _out_type(out, q_type, out_step)
-    _need(dim == cache.head_dim, "q has %d channels, the cache %d" % (dim, cache.head_dim))
+    _need(dim == cache.head_dim, "q and the cache have different numbers of channels")
     a, b = _rows(q, "q", n, heads, dim, q_type), _rows(out, "out", n, heads, dim, out_type, True)
     _need(block_table.dim() == 2 and block_table.shape[0] == n and _type(block_table) == TYPE_S32, "block_table is int32 [sequences][pages]")
     pages = block_table.shape[1]
@@ -590,7 +591,7 @@ def pulpnn_attn_decode(cache, q, block_table, seq_lens, out, scale=None, window=
 def _lse(lse, n, heads):
     if lse is None:
         return 0
-    _need(lse.shape == (n, heads) and lse.is_contiguous() and _type(lse) == TYPE_F32, "lse is float32 [%d][%d] in one piece" % (n, heads))
+    _need(lse.shape == (n, heads) and lse.is_contiguous() and _type(lse) == TYPE_F32, "lse is float32 [rows][heads] in one piece")
     return lse.data_ptr()
 
 
@@ -612,7 +613,7 @@ def pulpnn_attn_prompt(q, k, v, cu_q, out, cu_k=None, causal=True, window=0, sca
             _rows(out, "out", n, heads, dim, out_type, True)]
     seqs = cu_q.shape[0] - 1
     if cu_k is None:
-        _need(nk == n, "%d rows of keys for %d of queries, and no cu_k" % (nk, n))
+        _need(nk == n, "other numbers of rows of keys than of queries, and no cu_k")
         cu_k = cu_q
     _prompt_call(_prompt_pack(
         rows[0][0], rows[1][0], rows[2][0], rows[3][0], _lse(lse, n, heads), _vector(cu_q, "cu_q", seqs + 1, TYPE_S32),

@@ -136,6 +136,14 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(unsigned w)
 {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
+// Signed bytes as fp16: a byte plus 128 in the low bits of 1024 is 1152 + code, exactly. `biased` holds bytes ^ 0x80, two of
+// which `select` puts into the low bytes of the halves.
+__device__ __forceinline__ unsigned widen(unsigned biased, unsigned select)
+{
+  const unsigned w = __byte_perm(biased, 0x64646464u, select), off = 0x64806480u;
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&w), *reinterpret_cast<const __half2 *>(&off));
+  return *reinterpret_cast<const unsigned *>(&r);
+}
 // four adjacent channels of an output row; uint8: rint(y / step) + zero, cut to 0 .. 255 (a NaN gives the zero point)
 __device__ __forceinline__ unsigned to_u8(float y, float inv_step, int zero)
 {

@@ -98,13 +98,6 @@ template <> __device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], co
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Signed bytes as fp16: the byte plus 128 in the low bits of 1024 is 1152 + code, exactly.
-__device__ __forceinline__ unsigned widen(unsigned biased, unsigned select)
-{
-  const unsigned w = __byte_perm(biased, 0x64646464u, select), off = 0x64806480u;
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&w), *reinterpret_cast<const __half2 *>(&off));
-  return *reinterpret_cast<const unsigned *>(&r);
-}
 __device__ __forceinline__ float load_q(const char *p, int type)
 {
   return type == PULPNN_TYPE_F16 ? __half2float(*reinterpret_cast<const __half *>(p)) : __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(p));
@@ -539,7 +532,8 @@ extern "C" int pulpnn_attn_decode(const pulpnn_kv_cache_t *cache, const pulpnn_a
   if (a->window > 0 && a->window < most) most = a->window;
   const int tile = cache->type == PULPNN_TYPE_S8 ? 32 : 16;
   p.splits = 1;
-  while (p.splits < 8 && most > (int64_t)p.splits * WARPS * tile * 2) p.splits *= 2;
+  while (p.splits < 8 && most > (int64_t)p.splits * WARPS * tile * 2 && pairs * p.splits < 8 * 2 * c.sm_count) p.splits *= 2;
+  if (c.opt_split_k > 0) p.splits = c.opt_split_k >= 8 ? 8 : (c.opt_split_k >= 4 ? 4 : (c.opt_split_k >= 2 ? 2 : 1));
   const bool ok = cache->type == PULPNN_TYPE_S8 ? decode_dim<__half, true>(c, p, pairs, two)
                   : (a->q_type == PULPNN_TYPE_F16 ? decode_dim<__half, false>(c, p, pairs, two) : decode_dim<__nv_bfloat16, false>(c, p, pairs, two));
   return ok ? PULPNN_OK : c.err;

@@ -2,20 +2,24 @@
 //
 //   O = softmax(scale * Q K^T, masked) V   per sequence and query head, in tiles of 128 queries x 128 keys.
 //
-// A CTA holds two tiles of queries ("units") and walks over the keys that either sees; both multiply with every K and V
-// tile it loads. The units of a key head are its 128-row tiles times the G query heads that share it, heads
-// fastest, and a CTA takes two that follow one another: two heads of the same rows where G > 1 (the same causal
-// range, and both busy however short the sequence is), two neighbouring row tiles where G = 1.
+// Work comes in items of two tiles of queries ("units"), which walk together over the keys that either sees; both
+// multiply with every K and V tile that is loaded. The units of a key head are its 128-row tiles times the G query heads
+// that share it, heads fastest, and an item is two that follow one another: two heads of the same rows where G > 1 (the
+// same causal range, and both busy however short the sequence is), two neighbouring row tiles where G = 1.
+//
+// One CTA an SM. It begins with the item of its own block index and takes further ones from blocks that have not
+// started yet (clusterlaunchcontrol), so that nothing is set up twice and no SM waits at the end of a fixed share; a
+// sequence's last rows, which see the most keys, come first.
 //
 //   warps 0-3, 4-7  softmax of unit 0 and 1: a thread is a row. S comes from TMEM, the weights go back there as the 16-bit
-//                   operand of the second product, in the columns S had.
+//                   operand of the second product, in the columns S had. At an item's end they also write its rows.
 //   warp 8          loads Q, then K and V tiles in turn, by TMA into a ring of stages
 //   warp 9          issues the MMAs: S = Q K^T (both from shared memory), O += P V (P from TMEM). While one unit's weights
-//                   are computed, the other unit's products run.
-//   warps 10, 11    guard the V tiles in which some query of the CTA does not see some key: a weight of 0 does
-//                   not keep an infinity or a NaN out of a sum of products, so rows behind the sequence's end (another sequence's)
-//                   become 0, and so do infinities and NaN among the rest, which the epilogue then adds to
-//                   the rows that do see them.
+//                   are computed, the other unit's products run; an item's first S follow the last O of the one before.
+//   warps 10, 11    guard the V tiles in which some query of the item does not see some key: a weight of 0 does
+//                   not keep an infinity or a NaN out of a sum of products, so rows behind the sequence's end (another
+//                   sequence's) become 0, and so do infinities and NaN among the rest, which the epilogue then adds to
+//                   the rows that do see them. Warp 10 also fetches the items, one ahead.
 //
 // TMEM: S of unit 0 and 1 (128 columns each), O of unit 0 and 1 (64 or 128 each).
 // The running maximum is a reference that has to be near the true one only: it is raised, and O rescaled in TMEM by
@@ -55,13 +59,38 @@ template <int DP> struct Shape {
   static constexpr int SMEM = (2 + STAGES) * TILE + 1024 /* barriers */ + 1024 /* alignment */;
 };
 
+struct Item { int end, q0, k0, lq, lk, pair, kvh, dirty; };
+constexpr int ITEMS = 3;
+
 struct Control {
-  uint64_t q_full[2], kv_full[8], kv_empty[8], clean[4], s_full[2], p_full[2], drain;
+  uint64_t q_full[2], q_empty[2], kv_full[8], kv_empty[8], clean[4], s_full[2], p_full[2], o_full[2], item_full[ITEMS], item_empty[ITEMS], next, drain;
+  uint4 answer;                    // to the request for another block's work
+  Item item[ITEMS];
   uint32_t tmem;
-  int abort_flag, dirty;
-  int warp_total[THREADS / 32];
-  int found, q0, k0, lq, lk, pair;
+  int abort_flag;
 };
+
+// The work of a block that has not started: asks for it, and reads the answer (false: there is none left).
+__device__ __forceinline__ void ask_for_block(uint4 *answer, uint64_t *bar)
+{
+  mbar_arrive_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+               ::"r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool block_of(const uint4 *answer, int &x, int &y)
+{
+  uint32_t got, bx, by;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t.reg .b32 z;\n\t"
+      "ld.shared.b128 r, [%3];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, z, _}, r;\n\t}"
+      : "=&r"(got), "=&r"(bx), "=&r"(by) : "r"(smem_u32(answer)) : "memory");
+  x = (int)bx; y = (int)by;
+  return got != 0;
+}
 
 // D(tmem) (+)= A(smem) * B(smem)^T and A(tmem) * B(smem), 16-bit operands, 32-bit sums
 __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
@@ -111,248 +140,249 @@ template <> struct Kind<__nv_bfloat16> { static constexpr bool BF16 = true; stat
 
 // A tile of queries: rows row0 .. row0 + rows - 1 of head `head`, the first at position pos; it sees the key tiles lo .. hi - 1.
 struct Unit { int row0, rows, head, pos, lo, hi, keys; };
+// An item's units and the key tiles lo .. hi - 1 that either sees.
+struct Work { Unit u[2]; int q0, k0, lk, kvh, lo, hi; };
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(THREADS, 1)
-attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                   const __grid_constant__ CUtensorMap map_v, const PromptProblem p)
+__device__ __forceinline__ Work work_of(const Item &it, const PromptProblem &p)
 {
-  using SH = Shape<DP>;
-  extern __shared__ char raw[];
-  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
-  char *smem = raw + (base - smem_u32(raw));
-  const uint32_t s_q = base, s_kv = base + 2 * SH::TILE;
-  Control &ct = *reinterpret_cast<Control *>(smem + (2 + SH::STAGES) * SH::TILE);
-  static_assert(sizeof(Control) <= 1024, "control block");
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  volatile int *abort_flag = &ct.abort_flag;
-
-  if (threadIdx.x == 0) {
-    ct.abort_flag = 0; ct.dirty = 0; ct.found = 0;
-    for (int x = 0; x < 2; x++) { mbar_init(&ct.q_full[x], 1); mbar_init(&ct.s_full[x], 1); mbar_init(&ct.p_full[x], 4); }
-    for (int s = 0; s < SH::STAGES; s++) { mbar_init(&ct.kv_full[s], 1); mbar_init(&ct.kv_empty[s], 1); }
-    for (int s = 0; s < SH::STAGES / 2; s++) mbar_init(&ct.clean[s], 2);
-    mbar_init(&ct.drain, 1);
-    mbar_fence_init();
-  }
-  pdl_wait();
-  // ---- which two units: the sequence whose pairs of units hold number blockIdx.x ----
-  {
-    int before = 0;
-    __syncthreads();
-    for (int s0 = 0; s0 < p.seqs; s0 += THREADS) {
-      const int b = s0 + threadIdx.x;
-      int count = 0, q0 = 0, lq = 0;
-      if (b < p.seqs) {
-        q0 = min(max(__ldg(p.cu_q + b), 0), p.nq);
-        lq = min(max(__ldg(p.cu_q + b + 1), q0), p.nq) - q0;
-        count = (int)(((int64_t)((lq + BQ - 1) / BQ) * p.group + 1) / 2);
-      }
-      int incl = count;
-#pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const int y = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += y;
-      }
-      if (lane == 31) ct.warp_total[warp] = incl;
-      __syncthreads();
-      int total = 0, off = before;
-      for (int w = 0; w < THREADS / 32; w++) { if (w < warp) off += ct.warp_total[w]; total += ct.warp_total[w]; }
-      const int at = (int)blockIdx.x - (off + incl - count);
-      if (at >= 0 && at < count) {
-        const int k0 = min(max(__ldg(p.cu_k + b), 0), p.nk);
-        ct.q0 = q0; ct.lq = lq; ct.k0 = k0; ct.lk = min(max(__ldg(p.cu_k + b + 1), k0), p.nk) - k0;
-        ct.pair = count - 1 - at;          // the last rows of a causal sequence see the most keys: they begin first
-        ct.found = 1;
-      }
-      before += total;
-      __syncthreads();
-      if (ct.found) break;
-    }
-  }
-  if (!ct.found) return;
-  if (warp == WARP_MMA) tmem_alloc(&ct.tmem, 512);
-  const int q0 = ct.q0, k0 = ct.k0, lq = ct.lq, lk = ct.lk, kvh = blockIdx.y;
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = ct.tmem;
-
-  Unit un[2];
+  Work w;
+  w.q0 = it.q0; w.k0 = it.k0; w.lk = it.lk; w.kvh = it.kvh;
 #pragma unroll
   for (int x = 0; x < 2; x++) {
-    const int u = 2 * ct.pair + x, rt = u / p.group;
-    Unit &w = un[x];
-    w.row0 = rt * BQ; w.head = kvh * p.group + u - rt * p.group;
-    w.rows = min(max(lq - w.row0, 0), BQ);
-    w.pos = w.row0 + lk - lq;
-    w.keys = w.rows == 0 ? 0 : (p.causal ? min(lk, max(w.pos + w.rows, 0)) : lk);       // it sees none from here on
-    const int from = p.window > 0 ? max(0, w.pos - p.window + 1) : 0;
-    w.lo = from / BK; w.hi = (w.keys + BK - 1) / BK;
-    if (from >= w.keys) w.lo = w.hi = 0;
+    const int n = 2 * it.pair + x, rt = n / p.group;
+    Unit &u = w.u[x];
+    u.row0 = rt * BQ; u.head = it.kvh * p.group + n - rt * p.group;
+    u.rows = min(max(it.lq - u.row0, 0), BQ);
+    u.pos = u.row0 + it.lk - it.lq;
+    u.keys = u.rows == 0 ? 0 : (p.causal ? min(it.lk, max(u.pos + u.rows, 0)) : it.lk);       // it sees none from here on
+    const int from = p.window > 0 ? max(0, u.pos - p.window + 1) : 0;
+    u.lo = from / BK; u.hi = (u.keys + BK - 1) / BK;
+    if (from >= u.keys) u.lo = u.hi = 0;
   }
-  const bool any0 = un[0].hi > un[0].lo, any1 = un[1].hi > un[1].lo;
-  const int lo = !any0 ? un[1].lo : (!any1 ? un[0].lo : min(un[0].lo, un[1].lo)), hi = max(un[0].hi, un[1].hi);
-  auto sees = [](const Unit &u, int j) { return j >= u.lo && j < u.hi; };
-  // whether some row of the unit does not see some key of tile j
-  auto masked = [&](const Unit &u, int j) {
-    const int k = j * BK, end = p.causal ? min(lk, u.pos + 1) : lk;
-    return k + BK > end || (p.window > 0 && k < u.pos + u.rows - p.window);
-  };
-  auto guarded = [&](int j) { return (sees(un[0], j) && masked(un[0], j)) || (sees(un[1], j) && masked(un[1], j)); };
+  const bool any0 = w.u[0].hi > w.u[0].lo, any1 = w.u[1].hi > w.u[1].lo;
+  w.lo = !any0 ? w.u[1].lo : (!any1 ? w.u[0].lo : min(w.u[0].lo, w.u[1].lo));
+  w.hi = max(w.u[0].hi, w.u[1].hi);
+  return w;
+}
+__device__ __forceinline__ bool sees(const Unit &u, int j) { return j >= u.lo && j < u.hi; }
+// whether some row of the unit does not see some key of tile j
+__device__ __forceinline__ bool masked(const Unit &u, int j, int lk, const PromptProblem &p)
+{
+  const int k = j * BK, end = p.causal ? min(lk, u.pos + 1) : lk;
+  return k + BK > end || (p.window > 0 && k < u.pos + u.rows - p.window);
+}
+__device__ __forceinline__ bool guarded(const Work &w, int j, const PromptProblem &p)
+{
+  return (sees(w.u[0], j) && masked(w.u[0], j, w.lk, p)) || (sees(w.u[1], j) && masked(w.u[1], j, w.lk, p));
+}
 
-  if (warp >= WARP_LOAD) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == WARP_LOAD) {
-      if (lane == 0) {
-        int issued = 0;
-        bool ok = true;
+// Finds pair number x of the units of all sequences. The search goes on where the last one stopped: `before` pairs lie
+// ahead of sequence s0. A whole warp; false where there are not so many pairs.
+__device__ __forceinline__ bool find_item(const PromptProblem &p, int x, int lane, int &s0, int &before, Item &it)
+{
+  for (; s0 < p.seqs; s0 += 256) {              // eight sequences a lane
+    int at[9], count[8], sum = 0;
+    const int b0 = s0 + lane * 8;
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-          if (un[x].hi <= un[x].lo) continue;
-          mbar_arrive_expect_tx(&ct.q_full[x], SH::TILE);
-          for (int b = 0; b < SH::BOXES; b++)
-            tma_load_3d(smem + x * SH::TILE + b * SH::BOX, &map_q, &ct.q_full[x], b * 64, un[x].head, q0 + un[x].row0);
-        }
-        for (int e = 0; e < 2 * (hi - lo) && ok; e++) {
-          const int st = e % SH::STAGES, j = lo + (e >> 1);
-          if (!(ok = mbar_wait(&ct.kv_empty[st], ((e / SH::STAGES) & 1) ^ 1, abort_flag, p.status, ST_LOAD))) break;
-          mbar_arrive_expect_tx(&ct.kv_full[st], SH::TILE);
-          for (int b = 0; b < SH::BOXES; b++)
-            tma_load_3d(smem + (2 + st) * SH::TILE + b * SH::BOX, e & 1 ? &map_v : &map_k, &ct.kv_full[st], b * 64, kvh, k0 + j * BK);
-          issued = e + 1;
-        }
-        if (!ok) {        // given up: the copies in flight must land before the CTA's shared memory is given away
-          volatile int never = 0;
+    for (int k = 0; k < 9; k++) at[k] = b0 + k <= p.seqs ? min(max(__ldg(p.cu_q + b0 + k), 0), p.nq) : 0;
 #pragma unroll
-          for (int x = 0; x < 2; x++)
-            if (un[x].hi > un[x].lo) mbar_wait(&ct.q_full[x], 0, &never, nullptr, 0);
-          for (int e = max(0, issued - SH::STAGES); e < issued; e++)
-            mbar_wait(&ct.kv_full[e % SH::STAGES], (e / SH::STAGES) & 1, &never, nullptr, 0);
-        }
-      }
-    } else if (warp == WARP_MMA) {
-      if (lane == 0) {
-        const int ksteps = (p.dim + 15) / 16;
-        const uint32_t id_s = idesc16(Kind<T>::BF16, false, BK), id_o = idesc16(Kind<T>::BF16, true, ksteps * 16);
-        int pcount[2] = {0, 0};
-        bool ok = true, have_q[2] = {false, false};
-        auto issue_s = [&](int x, int j) {      // the caller has waited for K(j)
-          if (!have_q[x]) { have_q[x] = true; if (!(ok = mbar_wait(&ct.q_full[x], 0, abort_flag, p.status, ST_MMA))) return; }
-          const uint32_t a = s_q + x * SH::TILE, b = s_kv + ((2 * (j - lo)) % SH::STAGES) * SH::TILE;
-          tc_fence_after();
-          for (int ks = 0; ks < ksteps; ks++) {
-            const uint32_t off = (ks >> 2) * SH::BOX + (ks & 3) * 32;
-            umma_ss(tmem + x * 128, umma_smem_desc<128>(a + off), umma_smem_desc<128>(b + off), id_s, ks > 0);
-          }
-          umma_commit(&ct.s_full[x]);
-        };
-        auto wait_kv = [&](int e) { return mbar_wait(&ct.kv_full[e % SH::STAGES], (e / SH::STAGES) & 1, abort_flag, p.status, ST_MMA); };
-        if (lo < hi) {
-          ok = wait_kv(0);
-#pragma unroll
-          for (int x = 0; x < 2; x++)
-            if (ok && sees(un[x], lo)) issue_s(x, lo);
-          if (ok) umma_commit(&ct.kv_empty[0]);
-        }
-        for (int j = lo; j < hi && ok; j++) {
-          const int ev = 2 * (j - lo) + 1, ek = ev + 1;
-          bool have_v = false, have_k = false;
-#pragma unroll
-          for (int x = 0; x < 2; x++) {
-            if (ok && sees(un[x], j)) {
-              if (!have_v) {
-                have_v = true;
-                ok = wait_kv(ev) && mbar_wait(&ct.clean[(ev % SH::STAGES) >> 1], (ev / SH::STAGES) & 1, abort_flag, p.status, ST_MMA);
-                if (!ok) break;
-              }
-              if (!(ok = mbar_wait(&ct.p_full[x], pcount[x] & 1, abort_flag, p.status, ST_MMA))) break;
-              pcount[x]++;
-              tc_fence_after();
-              const uint32_t b = s_kv + (ev % SH::STAGES) * SH::TILE;
-              const int parts = min(BK / 16, (un[x].keys - j * BK + 15) / 16);      // keys that none of its rows sees are left out
-              for (int kk = 0; kk < parts; kk++)
-                umma_ts(tmem + 256 + x * DP, tmem + x * 128 + kk * 8, desc_v(b + kk * 2048), id_o, j > un[x].lo || kk > 0);
-            }
-            if (ok && sees(un[x], j + 1)) {
-              if (!have_k) { have_k = true; if (!(ok = wait_kv(ek))) break; }
-              issue_s(x, j + 1);
-            } else if (ok && sees(un[x], j)) {
-              umma_commit(&ct.s_full[x]);         // O is complete
-            }
-          }
-          if (!ok) break;
-          umma_commit(&ct.kv_empty[ev % SH::STAGES]);
-          if (j + 1 < hi) umma_commit(&ct.kv_empty[ek % SH::STAGES]);
-        }
-        if (!ok) {        // given up: the MMAs in flight must end before TMEM is given back
-          volatile int never = 0;
-          umma_commit(&ct.drain);
-          mbar_wait(&ct.drain, 0, &never, nullptr, 0);
-        }
-      }
-    } else {
-      const int id = threadIdx.x - WARP_GUARD * 32;
-      for (int j = lo; j < hi; j++) {
-        const int e = 2 * (j - lo) + 1, st = e % SH::STAGES;
-        if (!mbar_wait(&ct.kv_full[st], (e / SH::STAGES) & 1, abort_flag, p.status, ST_GUARD)) break;
-        if (guarded(j)) {
-          const int rows = lk - j * BK;
-          bool odd = false;
-          for (int i = id; i < SH::TILE / 16; i += GUARD_THREADS) {
-            uint4 *at = reinterpret_cast<uint4 *>(smem + (2 + st) * SH::TILE) + i;
-            if (((i >> 3) & 127) >= rows) { *at = make_uint4(0, 0, 0, 0); continue; }
-            const uint4 w = *at;
-            constexpr unsigned E = Kind<T>::EXP;
-            // the exponent's bits all set: adding one at their lowest place carries into the sign's
-            auto bad = [](unsigned v) { return ((v & (E * 0x10001u)) + (E & (~E + 1u)) * 0x10001u) & 0x80008000u; };
-            const unsigned x = bad(w.x), y = bad(w.y), z = bad(w.z), t = bad(w.w);
-            if (x | y | z | t) {
-              auto keep = [](unsigned v, unsigned b) { return v & ~((b >> 15) * 0xffffu); };
-              *at = make_uint4(keep(w.x, x), keep(w.y, y), keep(w.z, z), keep(w.w, t));
-              odd = true;
-            }
-          }
-          if (odd) *reinterpret_cast<volatile int *>(&ct.dirty) = 1;
-          fence_proxy_async();
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ct.clean[st >> 1]);
-      }
+    for (int k = 0; k < 8; k++) {
+      const int tiles = b0 + k < p.seqs ? (max(at[k + 1] - at[k], 0) + BQ - 1) / BQ : 0;
+      count[k] = (int)(((int64_t)tiles * p.group + 1) / 2);
+      sum += count[k];
     }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const int x = warp >> 2, r = threadIdx.x & 127;
-    const Unit w = x == 0 ? un[0] : un[1];
-    const uint32_t rowbase = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t t_s = rowbase + x * 128, t_o = rowbase + 256 + x * DP;
+    int incl = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += v;
+    }
+    int off = before + incl - sum, which = -1, q0 = 0, lq = 0, pair = 0;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      if (x >= off && x < off + count[k]) {
+        which = b0 + k;
+        // the last rows of a causal sequence see the most keys: they begin first
+        q0 = at[k]; lq = at[k + 1] - at[k]; pair = count[k] - 1 - (x - off);
+      }
+      off += count[k];
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, which >= 0);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      which = __shfl_sync(0xffffffffu, which, src);
+      it.q0 = __shfl_sync(0xffffffffu, q0, src); it.lq = __shfl_sync(0xffffffffu, lq, src); it.pair = __shfl_sync(0xffffffffu, pair, src);
+      it.k0 = min(max(__ldg(p.cu_k + which), 0), p.nk);
+      it.lk = min(max(__ldg(p.cu_k + which + 1), it.k0), p.nk) - it.k0;
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return false;
+}
+
+// Warps 10 and 11: the guards of the V tiles; warp 10 also fetches the items.
+template <typename T, int DP>
+__device__ __forceinline__ void guard_warp(Control &ct, char *smem, const PromptProblem &p, bool fetches, int id)
+{
+  using SH = Shape<DP>;
+  constexpr int ST = SH::STAGES;
+  constexpr unsigned E = Kind<T>::EXP;
+  volatile int *abort_flag = &ct.abort_flag;
+  const int lane = id & 31;
+  int s0 = 0, before = 0, row = blockIdx.y, asked = 0;
+  bool ok = true, pending = false;
+  // publishes item number i
+  auto publish = [&](int i) {
+    ok = __all_sync(0xffffffffu, mbar_wait(&ct.item_empty[i % ITEMS], ((i / ITEMS) & 1) ^ 1, abort_flag, p.status, ST_GUARD));
+    Item it = {1, 0, 0, 0, 0, 0, 0, 0};
+    bool own = i == 0;
+    while (ok) {
+      int x = blockIdx.x, y = blockIdx.y;
+      bool got = true;
+      if (!own) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&ct.next, (asked - 1) & 1, abort_flag, p.status, ST_GUARD));
+        if (!ok) break;
+        pending = false;
+        got = block_of(&ct.answer, x, y);
+        fence_proxy_async();                   // the next answer comes behind these reads
+        __syncwarp();
+      }
+      own = false;
+      if (!got) break;                         // nothing is left, and nothing may be asked for again
+      if (lane == 0) ask_for_block(&ct.answer, &ct.next);
+      asked++; pending = true;
+      if (y != row || x < before) { row = y; s0 = 0; before = 0; }
+      it.kvh = y;
+      if (find_item(p, x, lane, s0, before, it)) { it.end = 0; break; }
+      // a block beyond the last pair: the grid is made for the most there can be
+    }
+    if (lane == 0) {
+      ct.item[i % ITEMS] = it;
+      mbar_arrive(&ct.item_full[i % ITEMS]);
+    }
+    __syncwarp();
+  };
+  if (fetches) publish(0);
+  int e = 1;                                   // the ring's number of the next V tile
+  for (int i = 0; ok; i++) {
+    ok = __all_sync(0xffffffffu, mbar_wait(&ct.item_full[i % ITEMS], (i / ITEMS) & 1, abort_flag, p.status, ST_GUARD));
+    if (!ok || ct.item[i % ITEMS].end) break;
+    const Work w = work_of(ct.item[i % ITEMS], p);
+    if (fetches) publish(i + 1);
+    for (int j = w.lo; j < w.hi && ok; j++, e += 2) {
+      const int st = e % ST;
+      ok = __all_sync(0xffffffffu, mbar_wait(&ct.kv_full[st], (e / ST) & 1, abort_flag, p.status, ST_GUARD));
+      if (!ok) break;
+      if (guarded(w, j, p)) {
+        const int rows = w.lk - j * BK;
+        bool odd = false;
+        for (int k = id; k < SH::TILE / 16; k += GUARD_THREADS) {
+          uint4 *at = reinterpret_cast<uint4 *>(smem + (2 + st) * SH::TILE) + k;
+          if (((k >> 3) & 127) >= rows) { *at = make_uint4(0, 0, 0, 0); continue; }
+          const uint4 v = *at;
+          // the exponent's bits all set: adding one at their lowest place carries into the sign's
+          auto bad = [](unsigned v) { return ((v & (E * 0x10001u)) + (E & (~E + 1u)) * 0x10001u) & 0x80008000u; };
+          const unsigned a = bad(v.x), b = bad(v.y), c = bad(v.z), d = bad(v.w);
+          if (a | b | c | d) {
+            auto keep = [](unsigned v, unsigned b) { return v & ~((b >> 15) * 0xffffu); };
+            *at = make_uint4(keep(v.x, a), keep(v.y, b), keep(v.z, c), keep(v.w, d));
+            odd = true;
+          }
+        }
+        if (odd) *reinterpret_cast<volatile int *>(&ct.item[i % ITEMS].dirty) = 1;
+        fence_proxy_async();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ct.clean[st >> 1]);
+    }
+    if (lane == 0) mbar_arrive(&ct.item_empty[i % ITEMS]);
+  }
+  if (pending) {          // given up with a request under way: its answer must land first
+    volatile int never = 0;
+    mbar_wait(&ct.next, (asked - 1) & 1, &never, nullptr, 0);
+  }
+}
+
+// two values in a register pair, one instruction for both
+__device__ __forceinline__ uint64_t pair2(float a, float b)
+{
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 both(uint64_t v)
+{
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Warps 0 to 7: the softmax of a unit, a row a thread.
+template <typename T, int DP>
+__device__ __forceinline__ void softmax_warps(Control &ct, uint32_t tmem, const PromptProblem &p)
+{
+  volatile int *abort_flag = &ct.abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, x = warp >> 2, r = threadIdx.x & 127;
+  const uint32_t rowbase = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+  const uint32_t t_s = rowbase + x * 128, t_o = rowbase + 256 + x * DP;
+  const int cols = (p.dim + 15) / 16;
+  const uint64_t scale2 = pair2(p.scale_log2, p.scale_log2);
+  uint32_t s_phase = 0, o_phase = 0;
+  bool ok = true;
+  for (int i = 0; ok; i++) {
+    if (!(ok = mbar_wait(&ct.item_full[i % ITEMS], (i / ITEMS) & 1, abort_flag, p.status, ST_SOFTMAX))) break;
+    const Item &it = ct.item[i % ITEMS];
+    if (it.end) break;
+    Unit w;
+    int q0, k0, lk, kvh;
+    {
+      const Work all = work_of(it, p);
+      w = x == 0 ? all.u[0] : all.u[1];
+      q0 = all.q0; k0 = all.k0; lk = all.lk; kvh = all.kvh;
+    }
     const int pos = w.pos + r;
     const int last = p.causal ? min(lk - 1, pos) : lk - 1, first = p.window > 0 ? pos - p.window + 1 : 0;
-    const int cols = (p.dim + 15) / 16;
     float m = NOTHING, l = 0.f;
-    bool ok = true;
-    uint32_t phase = 0;
     for (int j = w.lo; j < w.hi; j++) {
-      if (!(ok = mbar_wait(&ct.s_full[x], phase, abort_flag, p.status, ST_SOFTMAX))) break;
-      phase ^= 1;
+      if (!(ok = mbar_wait(&ct.s_full[x], s_phase, abort_flag, p.status, ST_SOFTMAX))) break;
+      s_phase ^= 1;
       tc_fence_after();
       uint32_t s[4][32];
 #pragma unroll
-      for (int i = 0; i < 4; i++) tmem_ld_32(t_s + i * 32, s[i]);
+      for (int k = 0; k < 4; k++) tmem_ld_32(t_s + k * 32, s[k]);
       tmem_wait_ld();
-      if (masked(w, j)) {
+      if (masked(w, j, lk, p)) {
         const int a = first - j * BK, b = last - j * BK;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int k = 0; k < 4; k++)
 #pragma unroll
           for (int c = 0; c < 32; c++)
-            if (i * 32 + c < a || i * 32 + c > b) s[i][c] = 0xff800000u;
+            if (k * 32 + c < a || k * 32 + c > b) s[k][c] = 0xff800000u;
       }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 32; c++)
+      for (int c = 0; c < 32; c += 2)
 #pragma unroll
-        for (int i = 0; i < 4; i++) top[i] = fmaxf(top[i], __uint_as_float(s[i][c]));
+        for (int k = 0; k < 4; k++) top[k] = max3(top[k], __uint_as_float(s[k][c]), __uint_as_float(s[k][c + 1]));
       const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
       if (__any_sync(0xffffffffu, most > m + LAG)) {
         const float to = fmaxf(m, most), f = ex2(m - to);
@@ -364,76 +394,256 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             tmem_ld_16(t_o + c * 16, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
             tmem_st_16(t_o + c * 16, o);
           }
         }
       }
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t off2 = pair2(-m, -m);
+      uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
+      for (int k = 0; k < 4; k++) {
         uint32_t w16[16];
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
-          const float e0 = ex2(fmaf(__uint_as_float(s[i][c]), p.scale_log2, -m)), e1 = ex2(fmaf(__uint_as_float(s[i][c + 1]), p.scale_log2, -m));
-          sum[i] += e0 + e1;
+          const float2 a = both(fma2(pair2(__uint_as_float(s[k][c]), __uint_as_float(s[k][c + 1])), scale2, off2));
+          const float e0 = ex2(a.x), e1 = ex2(a.y);
+          sum[k] = add2(sum[k], pair2(e0, e1));
           w16[c / 2] = pack2<T>(e0, e1);       // off by 2^-8 (bf16) or 2^-11 (fp16) of each weight at most; their sum is taken unrounded
         }
-        tmem_st_16(t_s + i * 16, w16);
+        tmem_st_16(t_s + k * 16, w16);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      const float2 total = both(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+      l += total.x + total.y;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&ct.p_full[x]);
     }
-    // ---- epilogue ----
+    if (!ok) break;
+    // ---- the rows ----
     const bool any = w.hi > w.lo;
-    if (ok && any) ok = mbar_wait(&ct.s_full[x], phase, abort_flag, p.status, ST_EPI);
-    if (ok) {
+    if (any) {
+      if (!(ok = mbar_wait(&ct.o_full[x], o_phase, abort_flag, p.status, ST_EPI))) break;
+      o_phase ^= 1;
       tc_fence_after();
-      const bool live = r < w.rows;
-      const int64_t row = q0 + w.row0 + r;
-      const float inv = l == 0.f ? 0.f : 1.f / l;         // a row that sees nothing is zero
-      char *dst = p.out + row * p.out_row + (int64_t)w.head * p.out_head;
-      const bool dirty = any && *reinterpret_cast<volatile int *>(&ct.dirty);
-      for (int c = 0; c < cols; c++) {
-        float y[16];
-        if (any) {
-          uint32_t o[16];
-          tmem_ld_16(t_o + c * 16, o);
-          tmem_wait_ld();
+    }
+    const bool live = r < w.rows;
+    const int64_t row = q0 + w.row0 + r;
+    const float inv = l == 0.f ? 0.f : 1.f / l;         // a row that sees nothing is zero
+    char *dst = p.out + row * p.out_row + (int64_t)w.head * p.out_head;
+    const bool dirty = any && *reinterpret_cast<const volatile int *>(&it.dirty);
+    for (int c = 0; c < cols; c++) {
+      float y[16];
+      if (any) {
+        uint32_t o[16];
+        tmem_ld_16(t_o + c * 16, o);
+        tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 16; i++) y[i] = inv == 0.f ? 0.f : __uint_as_float(o[i]) * inv;
-        } else {
+        for (int k = 0; k < 16; k++) y[k] = inv == 0.f ? 0.f : __uint_as_float(o[k]) * inv;
+      } else {
 #pragma unroll
-          for (int i = 0; i < 16; i++) y[i] = 0.f;
-        }
-        if (dirty && live) {      // the infinities and NaN that the guards took out of the tiles, where this row sees them
-          for (int j = w.lo; j < w.hi; j++) {
-            if (!guarded(j)) continue;
-            for (int k = max(first, j * BK); k <= min(last, j * BK + BK - 1); k++) {
-              const T *v = reinterpret_cast<const T *>(p.v + (int64_t)(k0 + k) * p.v_row + (int64_t)kvh * p.v_head) + c * 16;
+        for (int k = 0; k < 16; k++) y[k] = 0.f;
+      }
+      if (dirty && live) {      // the infinities and NaN that the guards took out of the tiles, where this row sees them
+        const Work all = work_of(it, p);
+        for (int j = w.lo; j < w.hi; j++) {
+          if (!guarded(all, j, p)) continue;
+          for (int k = max(first, j * BK); k <= min(last, j * BK + BK - 1); k++) {
+            const T *v = reinterpret_cast<const T *>(p.v + (int64_t)(k0 + k) * p.v_row + (int64_t)kvh * p.v_head) + c * 16;
 #pragma unroll
-              for (int i = 0; i < 16; i++)
-                if (c * 16 + i < p.dim) {
-                  const float z = (float)v[i];
-                  if (!(fabsf(z) <= 3.402823466e38f)) y[i] += z;
-                }
-            }
+            for (int n = 0; n < 16; n++)
+              if (c * 16 + n < p.dim) {
+                const float z = (float)v[n];
+                if (!(fabsf(z) <= 3.402823466e38f)) y[n] += z;
+              }
           }
         }
-        if (live) {
+      }
+      if (live) {
 #pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            if (c * 16 + i < p.dim) {
-              const float z[4] = {y[i], y[i + 1], y[i + 2], y[i + 3]};
-              store4(dst, c * 16 + i, p.out_type, z, p.out_inv_step, p.out_zero);
-            }
+        for (int k = 0; k < 16; k += 4)
+          if (c * 16 + k < p.dim) {
+            const float z[4] = {y[k], y[k + 1], y[k + 2], y[k + 3]};
+            store4(dst, c * 16 + k, p.out_type, z, p.out_inv_step, p.out_zero);
+          }
+      }
+    }
+    if (live && p.lse) p.lse[row * p.hq + w.head] = (m + log2f(l)) * 0.69314718055994530942f;
+    tc_fence_before();          // O has been read: the next item's first P, behind this, lets it be written over
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ct.item_empty[i % ITEMS]);
+  }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(THREADS, 1)
+attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v, const PromptProblem p)
+{
+  using SH = Shape<DP>;
+  constexpr int ST = SH::STAGES;
+  extern __shared__ char raw[];
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+  char *smem = raw + (base - smem_u32(raw));
+  const uint32_t s_q = base, s_kv = base + 2 * SH::TILE;
+  Control &ct = *reinterpret_cast<Control *>(smem + (2 + ST) * SH::TILE);
+  static_assert(sizeof(Control) <= 1024, "control block");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int *abort_flag = &ct.abort_flag;
+
+  if (threadIdx.x == 0) {
+    ct.abort_flag = 0;
+    for (int x = 0; x < 2; x++) {
+      mbar_init(&ct.q_full[x], 1); mbar_init(&ct.q_empty[x], 1); mbar_init(&ct.s_full[x], 1); mbar_init(&ct.p_full[x], 4); mbar_init(&ct.o_full[x], 1);
+    }
+    for (int s = 0; s < ST; s++) { mbar_init(&ct.kv_full[s], 1); mbar_init(&ct.kv_empty[s], 1); }
+    for (int s = 0; s < ST / 2; s++) mbar_init(&ct.clean[s], 2);
+    for (int s = 0; s < ITEMS; s++) { mbar_init(&ct.item_full[s], 1); mbar_init(&ct.item_empty[s], 12); }      // every warp is done with an item
+    mbar_init(&ct.next, 1); mbar_init(&ct.drain, 1);
+    mbar_fence_init();
+  }
+  if (warp == WARP_MMA) tmem_alloc(&ct.tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ct.tmem;
+  pdl_wait();
+
+  // item number i, false where an error ends the kernel; lanes that do not wait must not read
+  auto wait_item = [&](int i, int code) { return mbar_wait(&ct.item_full[i % ITEMS], (i / ITEMS) & 1, abort_flag, p.status, code); };
+
+  if (warp >= WARP_LOAD) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == WARP_LOAD) {
+      if (lane == 0) {
+        int e = 0, nq[2] = {0, 0};
+        bool ok = true;
+        for (int i = 0; ok; i++) {
+          if (!(ok = wait_item(i, ST_LOAD)) || ct.item[i % ITEMS].end) break;
+          const Work w = work_of(ct.item[i % ITEMS], p);
+#pragma unroll
+          for (int x = 0; x < 2; x++) {
+            if (!ok || w.u[x].hi <= w.u[x].lo) continue;
+            if (nq[x] > 0 && !(ok = mbar_wait(&ct.q_empty[x], (nq[x] - 1) & 1, abort_flag, p.status, ST_LOAD))) continue;
+            mbar_arrive_expect_tx(&ct.q_full[x], SH::TILE);
+            for (int b = 0; b < SH::BOXES; b++)
+              tma_load_3d(smem + x * SH::TILE + b * SH::BOX, &map_q, &ct.q_full[x], b * 64, w.u[x].head, w.q0 + w.u[x].row0);
+            nq[x]++;
+          }
+          for (int j2 = 2 * w.lo; j2 < 2 * w.hi && ok; j2++) {
+            const int st = e % ST;
+            if (!(ok = mbar_wait(&ct.kv_empty[st], ((e / ST) & 1) ^ 1, abort_flag, p.status, ST_LOAD))) break;
+            mbar_arrive_expect_tx(&ct.kv_full[st], SH::TILE);
+            for (int b = 0; b < SH::BOXES; b++)
+              tma_load_3d(smem + (2 + st) * SH::TILE + b * SH::BOX, e & 1 ? &map_v : &map_k, &ct.kv_full[st], b * 64, w.kvh, w.k0 + (j2 >> 1) * BK);
+            e++;
+          }
+          mbar_arrive(&ct.item_empty[i % ITEMS]);
+        }
+        if (!ok) {        // given up: the copies in flight must land before the CTA's shared memory is given away
+          volatile int never = 0;
+#pragma unroll
+          for (int x = 0; x < 2; x++)
+            if (nq[x] > 0) mbar_wait(&ct.q_full[x], (nq[x] - 1) & 1, &never, nullptr, 0);
+          for (int k = max(0, e - ST); k < e; k++) mbar_wait(&ct.kv_full[k % ST], (k / ST) & 1, &never, nullptr, 0);
         }
       }
-      if (live && p.lse) p.lse[row * p.hq + w.head] = (m + log2f(l)) * 0.69314718055994530942f;
+    } else if (warp == WARP_MMA) {
+      if (lane == 0) {
+        const int ksteps = (p.dim + 15) / 16;
+        const uint32_t id_s = idesc16(Kind<T>::BF16, false, BK), id_o = idesc16(Kind<T>::BF16, true, ksteps * 16);
+        int i = -1, np[2] = {0, 0}, nq[2] = {0, 0}, e = 0;        // e: the ring's number of the current key tile
+        bool ok = true;
+        Work cur, nxt;
+        // the next item that has key tiles; those without need nothing here. False: there is none, or an error (ok)
+        auto next_item = [&](Work &w) {
+          while (true) {
+            i++;
+            if (!(ok = wait_item(i, ST_MMA)) || ct.item[i % ITEMS].end) return false;
+            w = work_of(ct.item[i % ITEMS], p);
+            mbar_arrive(&ct.item_empty[i % ITEMS]);
+            if (w.lo < w.hi) return true;
+          }
+        };
+        auto wait_kv = [&](int k) { return mbar_wait(&ct.kv_full[k % ST], (k / ST) & 1, abort_flag, p.status, ST_MMA); };
+        auto issue_s = [&](int x, const Unit &u, int j, int k) {      // K, number k of the ring, has landed
+          if (j == u.lo) {
+            if (!(ok = mbar_wait(&ct.q_full[x], nq[x] & 1, abort_flag, p.status, ST_MMA))) return;
+            nq[x]++;
+          }
+          const uint32_t a = s_q + x * SH::TILE, b = s_kv + (k % ST) * SH::TILE;
+          tc_fence_after();
+          for (int ks = 0; ks < ksteps; ks++) {
+            const uint32_t off = (ks >> 2) * SH::BOX + (ks & 3) * 32;
+            umma_ss(tmem + x * 128, umma_smem_desc<128>(a + off), umma_smem_desc<128>(b + off), id_s, ks > 0);
+          }
+          umma_commit(&ct.s_full[x]);
+          if (j == u.hi - 1) umma_commit(&ct.q_empty[x]);
+        };
+        bool more = next_item(cur);
+        int j = 0;
+        if (more) {
+          j = cur.lo;
+          ok = wait_kv(0);
+#pragma unroll
+          for (int x = 0; x < 2; x++)
+            if (ok && sees(cur.u[x], j)) issue_s(x, cur.u[x], j, 0);
+          if (ok) umma_commit(&ct.kv_empty[0]);
+        }
+        while (more && ok) {
+          // the tile after this one, of this item or the next
+          const bool same = j + 1 < cur.hi;
+          int jn = j + 1;
+          if (same) {
+            nxt = cur;
+          } else {
+            more = next_item(nxt);
+            if (!ok) break;
+            jn = nxt.lo;
+          }
+          bool have_v = false, have_k = false;
+#pragma unroll
+          for (int x = 0; x < 2; x++) {
+            const Unit &u = cur.u[x];
+            if (ok && sees(u, j)) {
+              if (!have_v) {
+                have_v = true;
+                ok = wait_kv(e + 1) && mbar_wait(&ct.clean[((e + 1) % ST) >> 1], ((e + 1) / ST) & 1, abort_flag, p.status, ST_MMA);
+                if (!ok) break;
+              }
+              if (!(ok = mbar_wait(&ct.p_full[x], np[x] & 1, abort_flag, p.status, ST_MMA))) break;
+              np[x]++;
+              tc_fence_after();
+              const uint32_t b = s_kv + ((e + 1) % ST) * SH::TILE;
+              const int parts = min(BK / 16, (u.keys - j * BK + 15) / 16);      // keys that none of its rows sees are left out
+              for (int kk = 0; kk < parts; kk++)
+                umma_ts(tmem + 256 + x * DP, tmem + x * 128 + kk * 8, desc_v(b + kk * 2048), id_o, j > u.lo || kk > 0);
+              if (j == u.hi - 1) umma_commit(&ct.o_full[x]);
+            }
+            if (ok && more && sees(nxt.u[x], jn)) {
+              if (!have_k) { have_k = true; if (!(ok = wait_kv(e + 2))) break; }
+              issue_s(x, nxt.u[x], jn, e + 2);
+            }
+          }
+          if (!ok) break;
+          umma_commit(&ct.kv_empty[(e + 1) % ST]);
+          if (more) umma_commit(&ct.kv_empty[(e + 2) % ST]);
+          e += 2;
+          j = jn;
+          if (!same) cur = nxt;
+        }
+        // the MMAs issued so far end before TMEM is given back
+        volatile int never = 0;
+        umma_commit(&ct.drain);
+        mbar_wait(&ct.drain, 0, &never, p.status, ST_MMA);
+      }
+    } else {
+      guard_warp<T, DP>(ct, smem, p, warp == WARP_GUARD, threadIdx.x - WARP_GUARD * 32);
     }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    softmax_warps<T, DP>(ct, tmem, p);
   }
 
   __syncwarp();

@@ -1,9 +1,9 @@
 // kv_cache.cu -- rows into and out of a paged cache of keys and values: pulpnn_kv_append (position rotation of
 // queries and keys, storing with a cut to 8 bits) and pulpnn_kv_gather.
 //
-// Both move bytes: 48 rows of 128 channels a token at 32 query and 8 key heads, some 4 operations a channel. A row is
-// held by 16 lanes (8 for heads of up to 64 channels), 8 channels each, so that a warp loads and stores whole rows in
-// 16-byte pieces and a row's largest value is 4 (3) shuffles away.
+// Both move bytes: 48 rows of 128 channels a token at 32 query and 8 key heads, some 4 operations a channel. A warp of the
+// append holds whole rows, as many as fit at 8 channels a lane (3 of 80 channels), so that it loads and stores them in
+// 16-byte pieces and a row's largest value is 4 shuffles away.
 #include "attention.cuh"
 
 namespace pulpnn {
@@ -31,7 +31,8 @@ int check_cache(const char *who, const pulpnn_kv_cache_t *c)
 
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 256;               // of a gather's block
+constexpr int WARPS = 4;                   // of an append's
 
 struct AppendProblem {
   const char *in[3];          // q, k, v
@@ -42,36 +43,37 @@ struct AppendProblem {
   const int *positions;
   const double *inv_freq;
   CacheView cache;
-  int n, hq, rows, dim, rot, half;
+  int first, heads[3], dim, half, chunks, per_warp;      // chunks of 8 channels in a row; rows of a warp
 };
 
 struct S32 {};
 struct F32 {};
-template <typename IN> struct InSize { static constexpr int v = 2; };
-template <> struct InSize<S32> { static constexpr int v = 4; };
-template <> struct InSize<F32> { static constexpr int v = 4; };
 
-// one channel, and eight from a 16-byte boundary (S32 before the step)
+// eight channels as they come
+template <typename IN> struct Raw { uint4 a; };
+template <> struct Raw<S32> { uint4 a, b; };
+template <> struct Raw<F32> { uint4 a, b; };
+template <typename IN> struct Width { static constexpr int v = sizeof(Raw<IN>) / 8; };
+
+template <typename IN> __device__ __forceinline__ Raw<IN> load8(const char *p) { return *reinterpret_cast<const Raw<IN> *>(p); }
+template <typename IN> __device__ __forceinline__ void values(const Raw<IN> &w, float (&x)[8])
+{
+  const float2 a = unpack2<IN>(w.a.x), b = unpack2<IN>(w.a.y), c = unpack2<IN>(w.a.z), d = unpack2<IN>(w.a.w);
+  x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y; x[4] = c.x; x[5] = c.y; x[6] = d.x; x[7] = d.y;
+}
+template <> __device__ __forceinline__ void values<S32>(const Raw<S32> &w, float (&x)[8])
+{
+  x[0] = (float)(int)w.a.x; x[1] = (float)(int)w.a.y; x[2] = (float)(int)w.a.z; x[3] = (float)(int)w.a.w;
+  x[4] = (float)(int)w.b.x; x[5] = (float)(int)w.b.y; x[6] = (float)(int)w.b.z; x[7] = (float)(int)w.b.w;
+}
+template <> __device__ __forceinline__ void values<F32>(const Raw<F32> &w, float (&x)[8])
+{
+  x[0] = __uint_as_float(w.a.x); x[1] = __uint_as_float(w.a.y); x[2] = __uint_as_float(w.a.z); x[3] = __uint_as_float(w.a.w);
+  x[4] = __uint_as_float(w.b.x); x[5] = __uint_as_float(w.b.y); x[6] = __uint_as_float(w.b.z); x[7] = __uint_as_float(w.b.w);
+}
 template <typename IN> __device__ __forceinline__ float load1(const char *p) { return (float)*reinterpret_cast<const IN *>(p); }
 template <> __device__ __forceinline__ float load1<S32>(const char *p) { return (float)*reinterpret_cast<const int *>(p); }
 template <> __device__ __forceinline__ float load1<F32>(const char *p) { return *reinterpret_cast<const float *>(p); }
-template <typename IN> __device__ __forceinline__ void load8(const char *p, float (&x)[8])
-{
-  const uint4 w = *reinterpret_cast<const uint4 *>(p);
-  const float2 a = unpack2<IN>(w.x), b = unpack2<IN>(w.y), c = unpack2<IN>(w.z), d = unpack2<IN>(w.w);
-  x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y; x[4] = c.x; x[5] = c.y; x[6] = d.x; x[7] = d.y;
-}
-template <> __device__ __forceinline__ void load8<S32>(const char *p, float (&x)[8])
-{
-  const int4 a = reinterpret_cast<const int4 *>(p)[0], b = reinterpret_cast<const int4 *>(p)[1];
-  x[0] = (float)a.x; x[1] = (float)a.y; x[2] = (float)a.z; x[3] = (float)a.w;
-  x[4] = (float)b.x; x[5] = (float)b.y; x[6] = (float)b.z; x[7] = (float)b.w;
-}
-template <> __device__ __forceinline__ void load8<F32>(const char *p, float (&x)[8])
-{
-  const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
 // times the real value of a step, channel by channel
 __device__ __forceinline__ void times8(const float *step, float (&x)[8])
 {
@@ -86,137 +88,161 @@ __device__ __forceinline__ void times8(const float *step, float (&x)[8])
 #pragma unroll
   for (int i = 0; i < 8; i++) x[i] *= s[i];
 }
+// x * inv to the nearest integer, ties to even, in the low byte: 1.5 * 2^23 leaves the sum no bits below one
+__device__ __forceinline__ unsigned code(float x, float inv) { return __float_as_uint(fmaf(x, inv, 12582912.f)); }
 
-// One block: the rows blockIdx.y, blockIdx.y + gridDim.y, ... (in groups of THREADS / LANES) of one token.
-template <typename IN, typename WIDE, bool EIGHT, int LANES, bool INTERLEAVED>
-__global__ void __launch_bounds__(THREADS) kv_append_kernel(const AppendProblem p)
+// One block: the queries, the keys or the values (blockIdx.y) of one token, so that everything but the head is the same for
+// the whole block. A warp holds per_warp whole rows; BATCH loads of a thread are under way together, the first of them
+// while the token's angles are computed.
+template <typename IN, typename WIDE, bool EIGHT, bool INTERLEAVED>
+__global__ void __launch_bounds__(WARPS * 32, Width<IN>::v == 2 ? 8 : 6) kv_append_kernel(const AppendProblem p)
 {
-  constexpr int SIZE = InSize<IN>::v, PER = THREADS / LANES;
-  __shared__ float2 turn[MAX_HEAD_DIM / 2];
-  const int token = blockIdx.x, lane = threadIdx.x % LANES, sub = threadIdx.x / LANES, c0 = lane * 8;
+  constexpr int SIZE = Width<IN>::v, BATCH = SIZE == 2 ? 4 : 2;
+  __shared__ __align__(16) float2 turn[MAX_HEAD_DIM / 2];
+  const int token = blockIdx.x, which = blockIdx.y + p.first, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sub = lane / p.chunks, c0 = (lane - sub * p.chunks) * 8, first_lane = sub * p.chunks;
+  const int heads = p.heads[which], half = which < 2 ? p.half : 0;
+  const bool side_by_side = !INTERLEAVED && (half & 7) == 0, low = c0 < half, turns = c0 < 2 * half;
+  const int mate = (lane + (low ? half >> 3 : -(half >> 3))) & 31;      // holds the other channels of this lane's eight pairs
+  const int64_t in_head = p.in_head[which], out_head = p.out_head[which];
+  const char *in = p.in[which] + token * p.in_token[which] + c0 * SIZE;
+  char *out = p.out[which] ? p.out[which] + token * p.out_token[which] + c0 * 2 : nullptr;
+  const float *steps = sizeof(IN) == 1 ? p.step[which] : nullptr;       // of S32 only
   pdl_wait();
-  if (threadIdx.x < p.half) {
-    // The angle in turns, in 64 bits: a position of 10^5 times a frequency near 1 leaves 32 bits with errors of 10^-2.
-    // Its fraction of a turn keeps 24 bits, and sincospif takes multiples of pi.
-    const double turns = (double)__ldg(p.positions + token) * __ldg(p.inv_freq + threadIdx.x) * 0.15915494309189533577;
-    float s, c;
-    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-    turn[threadIdx.x] = make_float2(c, s);
-  }
-  const long long slot = __ldg(p.slots + token);
+  const long long slot = which ? __ldg(p.slots + token) : -1;
   const bool stored = slot >= 0 && slot < p.cache.n_slots;
   const int page = stored ? p.cache.by_page.div((int)slot) : 0, at = stored ? (int)slot - page * p.cache.page_size : 0;
-  __syncthreads();
-  // the bound is a whole number of warps: all lanes of a row stay together
-  for (int row0 = blockIdx.y * PER; row0 < p.rows; row0 += gridDim.y * PER) {
-    const int row = row0 + sub;
-    const bool live = row < p.rows && c0 < p.dim;
-    const int which = row < p.hq ? 0 : (row < p.hq + p.cache.n_heads ? 1 : 2);
-    const int head = row - (which == 0 ? 0 : (which == 1 ? p.hq : p.hq + p.cache.n_heads));
-    float x[8], y[8];
-    if (live) {
-      const char *src = p.in[which] + token * p.in_token[which] + head * p.in_head[which] + c0 * SIZE;
-      const float *step = sizeof(IN) == 1 && p.step[which] ? p.step[which] + (int64_t)head * p.dim + c0 : nullptr;
-      load8<IN>(src, x);
-      if (step) times8(step, x);
-      if (which < 2 && c0 < p.rot) {
-        if (INTERLEAVED) {
+  char *held = (which == 1 ? p.cache.k : p.cache.v) + (row_of(p.cache, page, at, 0) + c0) * (EIGHT ? 1 : 2);
+  const int64_t held_head = p.cache.head_stride * (EIGHT ? 1 : 2);
+  for (int head0 = warp * p.per_warp + sub, done = 0; done < heads; done += BATCH * WARPS * p.per_warp, head0 += BATCH * WARPS * p.per_warp) {
+    Raw<IN> own[BATCH];
+    bool live[BATCH];
 #pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            if (c0 + i < p.rot) {
-              const float2 t = turn[(c0 + i) >> 1];
-              y[i] = x[i] * t.x - x[i + 1] * t.y;
-              y[i + 1] = x[i + 1] * t.x + x[i] * t.y;
-            } else { y[i] = x[i]; y[i + 1] = x[i + 1]; }
-          }
-        } else if ((p.half & 7) == 0) {
-          // the other channels of the eight pairs are eight of one other lane, which has loaded them too
-          const bool low = c0 < p.half;
-          const int other = low ? p.half : -p.half, i0 = low ? c0 : c0 - p.half;
-          float z[8];
-          load8<IN>(src + other * SIZE, z);
-          if (step) times8(step + other, z);
+    for (int b = 0; b < BATCH; b++) {
+      const int head = head0 + b * WARPS * p.per_warp;
+      live[b] = sub < p.per_warp && head < heads;
+      if (live[b]) own[b] = load8<IN>(in + head * in_head);
+    }
+    if (done == 0 && half) {
+      if (threadIdx.x < half) {
+        // The angle in turns, in 64 bits: a position of 10^5 times a frequency near 1 leaves 32 bits with errors of 10^-2.
+        // Its fraction of a turn keeps 24 bits, and sincospif takes multiples of pi.
+        const double t = (double)__ldg(p.positions + token) * __ldg(p.inv_freq + threadIdx.x) * 0.15915494309189533577;
+        float s, c;
+        sincospif(2.f * (float)(t - rint(t)), &s, &c);
+        turn[threadIdx.x] = make_float2(c, s);
+      }
+      __syncthreads();
+    }
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const float2 t = turn[i0 + i];
-            y[i] = x[i] * t.x + (low ? -z[i] : z[i]) * t.y;
-          }
+    for (int b = 0; b < BATCH; b++) {
+      const int head = head0 + b * WARPS * p.per_warp;
+      if (!__any_sync(0xffffffffu, live[b])) break;
+      float x[8], y[8], z[8];
+      if (!live[b]) own[b] = Raw<IN>{};
+      values<IN>(own[b], x);
+      if (sizeof(IN) == 1 && steps && live[b]) times8(steps + head * p.dim + c0, x);
+      if (side_by_side && half) {
+        if (SIZE == 2) {
+          Raw<IN> w;
+          w.a.x = __shfl_sync(0xffffffffu, own[b].a.x, mate); w.a.y = __shfl_sync(0xffffffffu, own[b].a.y, mate);
+          w.a.z = __shfl_sync(0xffffffffu, own[b].a.z, mate); w.a.w = __shfl_sync(0xffffffffu, own[b].a.w, mate);
+          values<IN>(w, z);
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const int c = c0 + i;
-            y[i] = x[i];
-            if (c < p.rot) {
-              const bool low = c < p.half;
-              const int other = low ? p.half : -p.half;
-              float z = load1<IN>(src + (i + other) * SIZE);
-              if (step) z *= __ldg(step + i + other);
-              const float2 t = turn[low ? c : c - p.half];
-              y[i] = x[i] * t.x + (low ? -z : z) * t.y;
-            }
-          }
+          for (int i = 0; i < 8; i++) z[i] = __shfl_sync(0xffffffffu, x[i], mate);
+        }
+      }
+      if (!turns) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = x[i];
+      } else if (INTERLEAVED) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const bool in_rot = c0 + i < 2 * half;
+          const float2 t = in_rot ? turn[(c0 + i) >> 1] : make_float2(1.f, 0.f);
+          y[i] = in_rot ? x[i] * t.x - x[i + 1] * t.y : x[i];
+          y[i + 1] = in_rot ? x[i + 1] * t.x + x[i] * t.y : x[i + 1];
+        }
+      } else if (side_by_side) {
+        const float sign = low ? -1.f : 1.f;
+        const float4 *t = reinterpret_cast<const float4 *>(turn + (low ? c0 : c0 - half));
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const float4 u = t[i / 2];
+          y[i] = x[i] * u.x + z[i] * (sign * u.y);
+          y[i + 1] = x[i + 1] * u.z + z[i + 1] * (sign * u.w);
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) y[i] = x[i];
+        for (int i = 0; i < 8; i++) {
+          const int c = c0 + i;
+          y[i] = x[i];
+          if (c < 2 * half && live[b]) {
+            const bool lower = c < half;
+            const int to = lower ? half : -half;
+            float other = load1<IN>(in + head * in_head + (i + to) * SIZE);
+            if (sizeof(IN) == 1 && steps) other *= __ldg(steps + head * p.dim + c + to);
+            const float2 t = turn[lower ? c : c - half];
+            y[i] = x[i] * t.x + (lower ? -other : other) * t.y;
+          }
+        }
       }
-    }
-    __syncwarp();              // in place: every lane of the row has read what another lane now writes over
-    const uint4 wide = live ? make_uint4(pack2<WIDE>(y[0], y[1]), pack2<WIDE>(y[2], y[3]), pack2<WIDE>(y[4], y[5]),
-                                         pack2<WIDE>(y[6], y[7])) : make_uint4(0, 0, 0, 0);
-    if (live && p.out[which])
-      *reinterpret_cast<uint4 *>(p.out[which] + token * p.out_token[which] + head * p.out_head[which] + c0 * 2) = wide;
-    if (EIGHT) {
-      float most = 0.f;
-      bool odd = false;
-      if (live) {
+      if (!INTERLEAVED && !side_by_side) __syncwarp();        // in place: every lane of the row has read what another lane now writes over
+      const uint4 wide = make_uint4(pack2<WIDE>(y[0], y[1]), pack2<WIDE>(y[2], y[3]), pack2<WIDE>(y[4], y[5]), pack2<WIDE>(y[6], y[7]));
+      if (live[b] && out) *reinterpret_cast<uint4 *>(out + head * out_head) = wide;
+      if (which == 0) continue;
+      if (EIGHT) {
+        float most = 0.f;
+        bool odd = false;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
           most = fmaxf(most, fabsf(y[i]));
           odd |= !(fabsf(y[i]) <= 3.402823466e38f);
         }
-      }
-      if (odd) most = __int_as_float(0x7f800000);
+        if (odd) most = __int_as_float(0x7f800000);
+        // around the row's lanes: after steps of 1, 2, 4 and 8 each of up to 16 has met all others
 #pragma unroll
-      for (int d = 1; d < LANES; d *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-      if (live && which > 0 && stored) {
-        const bool fine = most <= 3.402823466e38f, any = most >= 7.888609e-31f && fine;     // 2^-100
-        const float inv = any ? 127.f / most : 0.f;
-        int q[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) q[i] = any ? min(max(__float2int_rn(y[i] * inv), -127), 127) : 0;
-        uint2 w;
-        w.x = (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | (unsigned)q[3] << 24;
-        w.y = (q[4] & 255) | (q[5] & 255) << 8 | (q[6] & 255) << 16 | (unsigned)q[7] << 24;
-        char *base = which == 1 ? p.cache.k : p.cache.v;
-        *reinterpret_cast<uint2 *>(base + row_of(p.cache, page, at, head) + c0) = w;
-        if (lane == 0)
-          (which == 1 ? p.cache.k_scale : p.cache.v_scale)[scale_of(p.cache, page, at, head)] =
-              any ? most / 127.f : (fine ? 0.f : __int_as_float(0x7fffffff));
+        for (int d = 1; d < 16; d *= 2) {
+          int from = lane - first_lane + d;
+          if (from >= p.chunks) from %= p.chunks;
+          most = fmaxf(most, __shfl_sync(0xffffffffu, most, (first_lane + from) & 31));
+        }
+        if (live[b] && stored) {
+          const bool fine = most <= 3.402823466e38f, any = most >= 7.888609e-31f && fine;     // 2^-100
+          const float inv = any ? 127.f / most : 0.f;
+          uint2 w = make_uint2(0, 0);
+          if (any) {
+            w.x = __byte_perm(__byte_perm(code(y[0], inv), code(y[1], inv), 0x0040), __byte_perm(code(y[2], inv), code(y[3], inv), 0x0040), 0x5410);
+            w.y = __byte_perm(__byte_perm(code(y[4], inv), code(y[5], inv), 0x0040), __byte_perm(code(y[6], inv), code(y[7], inv), 0x0040), 0x5410);
+          }
+          *reinterpret_cast<uint2 *>(held + head * held_head) = w;
+          if (c0 == 0)
+            (which == 1 ? p.cache.k_scale : p.cache.v_scale)[scale_of(p.cache, page, at, head)] =
+                any ? most / 127.f : (fine ? 0.f : __int_as_float(0x7fffffff));
+        }
+      } else if (live[b] && stored) {
+        *reinterpret_cast<uint4 *>(held + head * held_head) = wide;
       }
-    } else if (live && which > 0 && stored) {
-      char *base = which == 1 ? p.cache.k : p.cache.v;
-      *reinterpret_cast<uint4 *>(base + (row_of(p.cache, page, at, head) + c0) * 2) = wide;
     }
   }
 }
 
 template <typename IN, typename WIDE, bool EIGHT>
-cudaError_t append_go(const AppendProblem &p, bool interleaved, dim3 grid, cudaStream_t s)
+cudaError_t append_go(const AppendProblem &p, int n, bool interleaved, cudaStream_t s)
 {
-  const bool narrow = p.dim <= 64;
-  auto k = narrow ? (interleaved ? kv_append_kernel<IN, WIDE, EIGHT, 8, true> : kv_append_kernel<IN, WIDE, EIGHT, 8, false>)
-                  : (interleaved ? kv_append_kernel<IN, WIDE, EIGHT, 16, true> : kv_append_kernel<IN, WIDE, EIGHT, 16, false>);
-  return launch_pdl(k, grid, dim3(THREADS), 0, s, p);
+  const dim3 grid((unsigned)n, (unsigned)(3 - p.first));
+  return interleaved ? launch_pdl(kv_append_kernel<IN, WIDE, EIGHT, true>, grid, dim3(WARPS * 32), 0, s, p)
+                     : launch_pdl(kv_append_kernel<IN, WIDE, EIGHT, false>, grid, dim3(WARPS * 32), 0, s, p);
 }
 template <typename WIDE, bool EIGHT>
-cudaError_t append_in(int in_type, const AppendProblem &p, bool interleaved, dim3 grid, cudaStream_t s)
+cudaError_t append_in(int in_type, const AppendProblem &p, int n, bool interleaved, cudaStream_t s)
 {
   switch (in_type) {
-    case PULPNN_TYPE_F16: return append_go<__half, WIDE, EIGHT>(p, interleaved, grid, s);
-    case PULPNN_TYPE_BF16: return append_go<__nv_bfloat16, WIDE, EIGHT>(p, interleaved, grid, s);
-    case PULPNN_TYPE_F32: return append_go<F32, WIDE, EIGHT>(p, interleaved, grid, s);
-    default: return append_go<S32, WIDE, EIGHT>(p, interleaved, grid, s);
+    case PULPNN_TYPE_F16: return append_go<__half, WIDE, EIGHT>(p, n, interleaved, s);
+    case PULPNN_TYPE_BF16: return append_go<__nv_bfloat16, WIDE, EIGHT>(p, n, interleaved, s);
+    case PULPNN_TYPE_F32: return append_go<F32, WIDE, EIGHT>(p, n, interleaved, s);
+    default: return append_go<S32, WIDE, EIGHT>(p, n, interleaved, s);
   }
 }
 
@@ -225,44 +251,74 @@ struct GatherProblem {
   char *out[2];
   int64_t out_token[2], out_head[2];      // bytes
   CacheView cache;
-  int n, dim;
+  int n, dim, chunks, per_block, heads, whole;   // chunks of 16 bytes in a cached row; rows of a block at a time
+  FastDiv by_heads;
 };
 
-// One row of 8 channels a lane; blockIdx.y is the head, blockIdx.z keys or values.
-template <typename WIDE, bool EIGHT, int LANES>
+// Rows (token, head), heads fastest, a chunk of 16 cached bytes a thread; blockIdx.y is keys or values. A thread takes BATCH
+// rows, a block's rows apart, and has all their loads under way before it stores the first.
+template <typename WIDE, bool EIGHT>
 __global__ void __launch_bounds__(THREADS) kv_gather_kernel(const GatherProblem p)
 {
-  constexpr int PER = THREADS / LANES;
-  const int lane = threadIdx.x % LANES, c0 = lane * 8, head = blockIdx.y, which = p.out[0] ? blockIdx.z : 1;
-  const int64_t token = (int64_t)blockIdx.x * PER + threadIdx.x / LANES;
+  constexpr int BATCH = 4;
+  const int sub = threadIdx.x / p.chunks, chunk = threadIdx.x - sub * p.chunks, which = p.out[0] ? blockIdx.y : 1;
+  const char *from = which == 0 ? p.cache.k : p.cache.v;
+  const float *scales = which == 0 ? p.cache.k_scale : p.cache.v_scale;
   pdl_wait();
-  if (token >= p.n || c0 >= p.dim) return;
-  const long long slot = __ldg(p.slots + token);
-  uint4 w = make_uint4(0, 0, 0, 0);
-  if (slot >= 0 && slot < p.cache.n_slots) {
-    const int page = p.cache.by_page.div((int)slot), at = (int)slot - page * p.cache.page_size;
-    const char *base = which == 0 ? p.cache.k : p.cache.v;
-    if (EIGHT) {
-      const uint2 q = *reinterpret_cast<const uint2 *>(base + row_of(p.cache, page, at, head) + c0);
-      const float s = (which == 0 ? p.cache.k_scale : p.cache.v_scale)[scale_of(p.cache, page, at, head)];
-      float x[8];
+  if (sub >= p.per_block) return;
+  uint4 w[BATCH];
+  float scale[BATCH];
+  int64_t to[BATCH];
 #pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = (float)(signed char)((i < 4 ? q.x : q.y) >> (8 * (i & 3))) * s;
-      w = make_uint4(pack2<WIDE>(x[0], x[1]), pack2<WIDE>(x[2], x[3]), pack2<WIDE>(x[4], x[5]), pack2<WIDE>(x[6], x[7]));
+  for (int b = 0; b < BATCH; b++) {
+    const int row = (blockIdx.x * BATCH + b) * p.per_block + sub;
+    to[b] = -1;
+    w[b] = make_uint4(0, 0, 0, 0);
+    scale[b] = 0.f;
+    const int token = p.by_heads.div(row), head = row - token * p.heads;
+    if (token >= p.n) continue;
+    to[b] = token * p.out_token[which] + head * p.out_head[which] + chunk * (EIGHT ? 32 : 16);
+    const long long slot = __ldg(p.slots + token);
+    if (slot < 0 || slot >= p.cache.n_slots) continue;
+    const int page = p.cache.by_page.div((int)slot), at = (int)slot - page * p.cache.page_size;
+    w[b] = *reinterpret_cast<const uint4 *>(from + row_of(p.cache, page, at, head) * (EIGHT ? 1 : 2) + chunk * 16);
+    if (EIGHT) scale[b] = scales[scale_of(p.cache, page, at, head)];
+  }
+#pragma unroll
+  for (int b = 0; b < BATCH; b++) {
+    if (to[b] < 0) continue;
+    uint4 *dst = reinterpret_cast<uint4 *>(p.out[which] + to[b]);
+    if (!EIGHT) { *dst = w[b]; continue; }
+    const unsigned q[4] = {w[b].x, w[b].y, w[b].z, w[b].w};
+    unsigned y[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const unsigned u = q[i] ^ 0x80808080u;
+      const float2 a = unpack2<__half>(widen(u, 0x4140)), c = unpack2<__half>(widen(u, 0x4342));
+      y[2 * i] = pack2<WIDE>(a.x * scale[b], a.y * scale[b]);
+      y[2 * i + 1] = pack2<WIDE>(c.x * scale[b], c.y * scale[b]);
+    }
+    if (p.whole) {       // a full 32-byte sector per lane and instruction
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]), "r"(y[4]),
+                   "r"(y[5]), "r"(y[6]), "r"(y[7]) : "memory");
     } else {
-      w = *reinterpret_cast<const uint4 *>(base + (row_of(p.cache, page, at, head) + c0) * 2);
+      dst[0] = make_uint4(y[0], y[1], y[2], y[3]);
+      dst[1] = make_uint4(y[4], y[5], y[6], y[7]);
     }
   }
-  *reinterpret_cast<uint4 *>(p.out[which] + token * p.out_token[which] + head * p.out_head[which] + c0 * 2) = w;
 }
 
 template <typename WIDE, bool EIGHT>
-cudaError_t gather_go(const GatherProblem &p, cudaStream_t s)
+cudaError_t gather_go(GatherProblem &p, cudaStream_t s)
 {
-  const int lanes = p.dim <= 64 ? 8 : 16, per = THREADS / lanes;
-  const dim3 grid((unsigned)((p.n + per - 1) / per), (unsigned)p.cache.n_heads, p.out[0] && p.out[1] ? 2 : 1);
-  return lanes == 8 ? launch_pdl(kv_gather_kernel<WIDE, EIGHT, 8>, grid, dim3(THREADS), 0, s, p)
-                    : launch_pdl(kv_gather_kernel<WIDE, EIGHT, 16>, grid, dim3(THREADS), 0, s, p);
+  p.chunks = p.dim * (EIGHT ? 1 : 2) / 16; p.per_block = THREADS / p.chunks; p.heads = p.cache.n_heads;
+  p.by_heads.set((unsigned)p.heads);
+  p.whole = 1;
+  for (int i = 0; i < 2; i++)
+    if (p.out[i] && (!aligned(p.out[i], 32) || p.out_token[i] % 32 || p.out_head[i] % 32)) p.whole = 0;
+  const int64_t rows = (int64_t)p.n * p.heads, per = 4 * p.per_block;
+  const dim3 grid((unsigned)((rows + per - 1) / per), p.out[0] && p.out[1] ? 2 : 1);
+  return launch_pdl(kv_gather_kernel<WIDE, EIGHT>, grid, dim3(THREADS), 0, s, p);
 }
 
 }  // namespace
@@ -317,16 +373,13 @@ extern "C" int pulpnn_kv_append(const pulpnn_kv_cache_t *cache, const pulpnn_kv_
   }
   p.slots = reinterpret_cast<const long long *>(a->slots); p.positions = a->positions; p.inv_freq = a->inv_freq;
   p.cache = view_of(*cache);
-  p.n = a->n_tokens; p.hq = a->q ? a->n_q_heads : 0; p.rows = p.hq + 2 * cache->n_heads; p.dim = cache->head_dim;
-  p.rot = a->rotary_dim; p.half = a->rotary_dim / 2;
-  // Few tokens: a block for every group of rows, so that a single token's rows are in flight together. Many: one block
-  // a token, which computes the token's angles once.
-  const int per = THREADS / (p.dim <= 64 ? 8 : 16), groups = (p.rows + per - 1) / per;
-  const dim3 grid((unsigned)p.n, (unsigned)(p.n < 4 * c.sm_count ? groups : 1));
+  p.first = a->q ? 0 : 1; p.heads[0] = a->q ? a->n_q_heads : 0; p.heads[1] = p.heads[2] = cache->n_heads; p.dim = cache->head_dim;
+  p.half = a->rotary_dim / 2;
+  p.chunks = p.dim / 8; p.per_warp = 32 / p.chunks;
   const bool il = a->interleaved != 0, f16 = a->out_type == PULPNN_TYPE_F16;
   const cudaError_t e = cache->type == PULPNN_TYPE_S8
-      ? (f16 ? append_in<__half, true>(a->in_type, p, il, grid, c.stream) : append_in<__nv_bfloat16, true>(a->in_type, p, il, grid, c.stream))
-      : (f16 ? append_in<__half, false>(a->in_type, p, il, grid, c.stream) : append_in<__nv_bfloat16, false>(a->in_type, p, il, grid, c.stream));
+      ? (f16 ? append_in<__half, true>(a->in_type, p, a->n_tokens, il, c.stream) : append_in<__nv_bfloat16, true>(a->in_type, p, a->n_tokens, il, c.stream))
+      : (f16 ? append_in<__half, false>(a->in_type, p, a->n_tokens, il, c.stream) : append_in<__nv_bfloat16, false>(a->in_type, p, a->n_tokens, il, c.stream));
   if (!cuda_ok(e, who)) return c.err;
   count_launch("kv_append_kernel");
   return PULPNN_OK;
@@ -347,6 +400,8 @@ extern "C" int pulpnn_kv_gather(const pulpnn_kv_cache_t *cache, const pulpnn_kv_
                (!a->v_out || rows_aligned(a->v_out, 2, {a->v_out_stride[0], a->v_out_stride[1]})),
                PULPNN_ERR_UNSUPPORTED, "%s: rows that do not begin on 16-byte boundaries", who);
   ATTN_REQUIRE(aligned(a->slots, 8), PULPNN_ERR_INVALID_ARG, "%s: unaligned slots", who);
+  // rows are counted in 32 bits, up to a block's rows beyond the last
+  ATTN_REQUIRE((int64_t)a->n_tokens * cache->n_heads <= 0x7fffffff - 4 * THREADS, PULPNN_ERR_UNSUPPORTED, "%s: %d tokens of %d heads", who, a->n_tokens, cache->n_heads);
   if (!ensure_device(c)) return c.err;
   if (!on_device(c, who, {cache->k, cache->v, cache->k_scale, cache->v_scale, a->slots, a->k_out, a->v_out})) return c.err;
 
