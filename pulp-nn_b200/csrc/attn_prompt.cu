@@ -22,8 +22,8 @@
 //                   the rows that do see them. Warp 10 also fetches the items, one ahead.
 //
 // TMEM: S of unit 0 and 1 (128 columns each), O of unit 0 and 1 (64 or 128 each).
-// The running maximum is a reference that has to be near the true one only: it is raised, and O rescaled in TMEM by
-// the softmax warps themselves, when a score is more than 2^LAG above it, which after the first tiles is rare.
+// The running maximum is a reference that has to be near the true one only: it is taken from an item's first tile, and raised
+// (O being rescaled in TMEM by the softmax warps themselves) when a weight comes out above 2^15, which is rare.
 // Between the commit that announces S(j) and its own arrival with P(j), a softmax group has O to itself: the
 // commit comes behind the MMAs of tile j - 1.
 #include "attention.cuh"
@@ -37,7 +37,7 @@ using namespace sm100;
 
 constexpr int BQ = 128, BK = 128, THREADS = 384;
 constexpr int WARP_LOAD = 8, WARP_MMA = 9, WARP_GUARD = 10, GUARD_THREADS = 64;
-constexpr float LAG = 8.f, NOTHING = -1e30f;
+constexpr float NOTHING = -1e30f;
 enum { ST_LOAD = 1 << 20, ST_MMA = 1 << 21, ST_SOFTMAX = 1 << 22, ST_GUARD = 1 << 23, ST_EPI = 1 << 24 };
 
 struct PromptProblem {
@@ -92,23 +92,42 @@ __device__ __forceinline__ bool block_of(const uint4 *answer, int &x, int &y)
   return got != 0;
 }
 
-// D(tmem) (+)= A(smem) * B(smem)^T and A(tmem) * B(smem), 16-bit operands, 32-bit sums
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
+// D(tmem) (+)= A(smem) * B(smem)^T and A(tmem) * B(smem), 16-bit operands, 32-bit sums. A whole warp comes here, and the lane
+// with `leader` issues: a predicate instead of a branch lets the operands be computed in uniform registers, which is where the
+// instruction takes them from. (A test of its own in front of each instruction undoes that, at 100 cycles an instruction: products
+// of fewer channels or keys than a tile has run over the zeros there.)
+__device__ __forceinline__ void umma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
 {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add ? 1 : 0) : "memory");
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add ? 1 : 0), "r"(leader) : "memory");
 }
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add)
+__device__ __forceinline__ void umma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add)
 {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add ? 1 : 0) : "memory");
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add ? 1 : 0), "r"(leader) : "memory");
 }
-// V as it lies, keys x channels: the product's N (channels) is contiguous. Blocks of 64 channels are a box apart
-// (leading offset), groups of 8 keys 1024 bytes (stride offset).
-__device__ __forceinline__ uint64_t desc_v(uint32_t saddr)
+__device__ __forceinline__ void umma_commit_by(uint32_t leader, uint64_t *bar)
 {
-  return (uint64_t)((saddr & 0x3ffffu) >> 4) | (uint64_t)((128 * 128) >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
-         (uint64_t)2 << 61;
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+               "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(leader) : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one()
+{
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
+// Shared-memory descriptors, whose low word holds the address in 16-byte units: the rest is the same for every tile.
+// Q and K: rows of 128 bytes, swizzled, groups of 8 rows 1024 bytes apart. V as it lies, keys x channels: the product's N
+// (channels) is contiguous, blocks of 64 channels are a box apart (leading offset), groups of 8 keys 1024 bytes (stride offset).
+constexpr uint32_t DESC_HIGH = (1024u >> 4) | 1u << 14 | 2u << 29, DESC_K_LOW = 1u << 16, DESC_V_LOW = (128u * 128u >> 4) << 16;
+__device__ __forceinline__ uint64_t desc_of(uint32_t low)
+{
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(low), "r"(DESC_HIGH));
+  return d;
 }
 // D = f32 (1 at bit 4), types of A and B (0 = f16, 1 = bf16) at bits 7 and 10, bit 16: B's N contiguous, N / 8, M / 16
 __device__ __forceinline__ uint32_t idesc16(bool bf16, bool b_n_major, int n)
@@ -304,6 +323,116 @@ __device__ __forceinline__ void guard_warp(Control &ct, char *smem, const Prompt
   }
 }
 
+__device__ __noinline__ bool wait_long(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *status, int code)
+{
+  return mbar_wait(bar, parity, abort_flag, status, code);
+}
+
+// Warp 9: issues the MMAs. The whole warp walks through the tiles, so that what the instructions take from uniform
+// registers is computed there; one lane issues and commits.
+template <typename T, int DP>
+__device__ __forceinline__ void mma_warp(Control &ct, uint32_t base, uint32_t tmem_, const PromptProblem &p)
+{
+  using SH = Shape<DP>;
+  constexpr int ST = SH::STAGES;
+  volatile int *abort_flag = &ct.abort_flag;
+  const uint32_t leader = elect_one();
+  // a wait that fails is looked at once a tile only: until then products of stale tiles do no harm, their results are void
+  bool ok = true;
+  auto wait = [&](uint64_t *bar, uint32_t parity) {
+    if (!mbar_try_wait(bar, parity)) ok = wait_long(bar, parity, abort_flag, p.status, ST_MMA) && ok;
+  };
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_, 0);
+  const uint32_t q_low = __shfl_sync(0xffffffffu, ((base & 0x3ffffu) >> 4) | DESC_K_LOW, 0);
+  const uint32_t k_low = __shfl_sync(0xffffffffu, (((base + 2 * SH::TILE) & 0x3ffffu) >> 4) | DESC_K_LOW, 0);
+  const uint32_t v_low = __shfl_sync(0xffffffffu, (((base + 2 * SH::TILE) & 0x3ffffu) >> 4) | DESC_V_LOW, 0);
+  const uint32_t id_s = idesc16(Kind<T>::BF16, false, BK), id_o = idesc16(Kind<T>::BF16, true, (p.dim + 15) / 16 * 16);
+  int i = -1, np[2] = {0, 0}, nq[2] = {0, 0}, e = 0;        // e: the ring's number of the current key tile
+  struct Range { int lo, hi, ulo[2], uhi[2]; } cur, nxt;      // key tiles of an item and of its units
+  // the next item that has key tiles; those without need nothing here. False: there is none, or an error (ok)
+  auto next_item = [&](Range &r) {
+    while (true) {
+      i++;
+      wait(&ct.item_full[i % ITEMS], (i / ITEMS) & 1);
+      if (__any_sync(0xffffffffu, !ok) || __any_sync(0xffffffffu, ct.item[i % ITEMS].end)) return false;
+      const Work w = work_of(ct.item[i % ITEMS], p);
+      r.lo = __shfl_sync(0xffffffffu, w.lo, 0); r.hi = __shfl_sync(0xffffffffu, w.hi, 0);
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
+        r.ulo[x] = __shfl_sync(0xffffffffu, w.u[x].lo, 0); r.uhi[x] = __shfl_sync(0xffffffffu, w.u[x].hi, 0);
+      }
+      if (leader) mbar_arrive(&ct.item_empty[i % ITEMS]);
+      if (r.lo < r.hi) return true;
+    }
+  };
+  auto wait_kv = [&](int k) { wait(&ct.kv_full[k % ST], (k / ST) & 1); };
+  // S of unit x with tile j, K being number k of the ring, which has landed
+  auto issue_s = [&](int x, int lo, int hi, int j, int k) {
+    if (j == lo) {
+      wait(&ct.q_full[x], nq[x] & 1);
+      nq[x]++;
+      tc_fence_after();
+    }
+    const uint32_t a = q_low + x * (SH::TILE >> 4), b = k_low + (k % ST) * (SH::TILE >> 4);
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ks++) {
+      const uint32_t off = ((ks >> 2) * SH::BOX + (ks & 3) * 32) >> 4;
+      umma_ss(leader, tmem + x * 128, desc_of(a + off), desc_of(b + off), id_s, ks > 0);
+    }
+    umma_commit_by(leader, &ct.s_full[x]);
+    if (j == hi - 1) umma_commit_by(leader, &ct.q_empty[x]);
+  };
+  bool more = next_item(cur);
+  int j = 0;
+  if (more) {
+    j = cur.lo;
+    wait_kv(0);
+    tc_fence_after();
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+      if (j >= cur.ulo[x] && j < cur.uhi[x]) issue_s(x, cur.ulo[x], cur.uhi[x], j, 0);
+    umma_commit_by(leader, &ct.kv_empty[0]);
+  }
+  while (more) {
+    // the tile after this one, of this item or the next
+    const bool same = j + 1 < cur.hi;
+    int jn = j + 1;
+    if (!same) {
+      more = next_item(nxt);
+      jn = nxt.lo;
+    }
+    wait_kv(e + 1);
+    wait(&ct.clean[((e + 1) % ST) >> 1], ((e + 1) / ST) & 1);
+    if (more) wait_kv(e + 2);
+    if (__any_sync(0xffffffffu, !ok)) break;
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      if (j >= cur.ulo[x] && j < cur.uhi[x]) {
+        wait(&ct.p_full[x], np[x] & 1);
+        np[x]++;
+        tc_fence_after();
+        const uint32_t b = v_low + ((e + 1) % ST) * (SH::TILE >> 4);
+        const bool begun = j > cur.ulo[x], last = j == cur.uhi[x] - 1;
+#pragma unroll
+        for (int kk = 0; kk < BK / 16; kk++)
+          umma_ts(leader, tmem + 256 + x * DP, tmem + x * 128 + kk * 8, desc_of(b + kk * (2048 >> 4)), id_o, begun || kk > 0);
+        if (last) umma_commit_by(leader, &ct.o_full[x]);
+      }
+      const int lo_n = same ? cur.ulo[x] : nxt.ulo[x], hi_n = same ? cur.uhi[x] : nxt.uhi[x];
+      if (more && jn >= lo_n && jn < hi_n) issue_s(x, lo_n, hi_n, jn, e + 2);
+    }
+    umma_commit_by(leader, &ct.kv_empty[(e + 1) % ST]);
+    if (more) umma_commit_by(leader, &ct.kv_empty[(e + 2) % ST]);
+    e += 2;
+    j = jn;
+    if (!same) cur = nxt;
+  }
+  // the MMAs issued so far end before TMEM is given back
+  volatile int never = 0;
+  umma_commit_by(leader, &ct.drain);
+  mbar_wait(&ct.drain, 0, &never, p.status, ST_MMA);
+}
+
 // two values in a register pair, one instruction for both
 __device__ __forceinline__ uint64_t pair2(float a, float b)
 {
@@ -332,10 +461,9 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
 __device__ __forceinline__ float max3(float a, float b, float c)
 {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-
 // Warps 0 to 7: the softmax of a unit, a row a thread.
 template <typename T, int DP>
 __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t tmem, const PromptProblem &p)
@@ -361,6 +489,8 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t tmem, const 
     }
     const int pos = w.pos + r;
     const int last = p.causal ? min(lk - 1, pos) : lk - 1, first = p.window > 0 ? pos - p.window + 1 : 0;
+    // every row sees every key of the tiles whole_lo .. whole_hi - 1
+    const int whole_hi = (p.causal ? min(lk, max(w.pos + 1, 0)) : lk) / BK, whole_lo = p.window > 0 ? (max(w.pos + w.rows - p.window, 0) + BK - 1) / BK : 0;
     float m = NOTHING, l = 0.f;
     for (int j = w.lo; j < w.hi; j++) {
       if (!(ok = mbar_wait(&ct.s_full[x], s_phase, abort_flag, p.status, ST_SOFTMAX))) break;
@@ -370,7 +500,7 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t tmem, const 
 #pragma unroll
       for (int k = 0; k < 4; k++) tmem_ld_32(t_s + k * 32, s[k]);
       tmem_wait_ld();
-      if (masked(w, j, lk, p)) {
+      if (j >= whole_hi || j < whole_lo) {
         const int a = first - j * BK, b = last - j * BK;
 #pragma unroll
         for (int k = 0; k < 4; k++)
@@ -378,42 +508,51 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t tmem, const 
           for (int c = 0; c < 32; c++)
             if (k * 32 + c < a || k * 32 + c > b) s[k][c] = 0xff800000u;
       }
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      // With the reference as it is; with a new one where there is none yet, or where the weights' sum shows that one of them is
+      // beyond 2^15 (or no number). In between, the scores' maximum is not looked for: that took a fifth of the time.
+      bool raise = j == w.lo;
+      float2 total;
+      while (true) {
+        if (raise) {
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 32; c += 2)
+          for (int c = 0; c < 32; c += 2)
 #pragma unroll
-        for (int k = 0; k < 4; k++) top[k] = max3(top[k], __uint_as_float(s[k][c]), __uint_as_float(s[k][c + 1]));
-      const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
-      if (__any_sync(0xffffffffu, most > m + LAG)) {
-        const float to = fmaxf(m, most), f = ex2(m - to);
-        m = to;
-        l *= f;
-        if (j > w.lo) {
-          for (int c = 0; c < cols; c++) {
-            uint32_t o[16];
-            tmem_ld_16(t_o + c * 16, o);
-            tmem_wait_ld();
+            for (int k = 0; k < 4; k++) top[k] = max3(top[k], __uint_as_float(s[k][c]), __uint_as_float(s[k][c + 1]));
+          const float most = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * p.scale_log2;
+          if (!(most <= 3e38f)) l = __int_as_float(0x7fffffff);        // a NaN or an infinity among the scores
+          const float to = fmaxf(m, most), f = ex2(m - to);
+          m = to;
+          l *= f;
+          if (j > w.lo) {
+            for (int c = 0; c < cols; c++) {
+              uint32_t o[16];
+              tmem_ld_16(t_o + c * 16, o);
+              tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-            tmem_st_16(t_o + c * 16, o);
+              for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st_16(t_o + c * 16, o);
+            }
           }
         }
-      }
-      const uint64_t off2 = pair2(-m, -m);
-      uint64_t sum[4] = {0, 0, 0, 0};
+        const uint64_t off2 = pair2(-m, -m);
+        uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        uint32_t w16[16];
+        for (int k = 0; k < 4; k++) {
+          uint32_t w16[16];
 #pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          const float2 a = both(fma2(pair2(__uint_as_float(s[k][c]), __uint_as_float(s[k][c + 1])), scale2, off2));
-          const float e0 = ex2(a.x), e1 = ex2(a.y);
-          sum[k] = add2(sum[k], pair2(e0, e1));
-          w16[c / 2] = pack2<T>(e0, e1);       // off by 2^-8 (bf16) or 2^-11 (fp16) of each weight at most; their sum is taken unrounded
+          for (int c = 0; c < 32; c += 2) {
+            const uint64_t a = fma2(pair2(__uint_as_float(s[k][c]), __uint_as_float(s[k][c + 1])), scale2, off2);
+            const float2 e = make_float2(ex2(both(a).x), ex2(both(a).y));
+            sum[k] = add2(sum[k], pair2(e.x, e.y));
+            w16[c / 2] = pack2<T>(e.x, e.y);       // off by 2^-8 (bf16) or 2^-11 (fp16) of each weight at most; their sum is taken unrounded
+          }
+          tmem_st_16(t_s + k * 16, w16);
         }
-        tmem_st_16(t_s + k * 16, w16);
+        total = both(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+        if (raise || !__any_sync(0xffffffffu, !(total.x + total.y < 32768.f))) break;
+        raise = true;
       }
-      const float2 total = both(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
       l += total.x + total.y;
       tmem_wait_st();
       tc_fence_before();
@@ -486,7 +625,6 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   extern __shared__ char raw[];
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   char *smem = raw + (base - smem_u32(raw));
-  const uint32_t s_q = base, s_kv = base + 2 * SH::TILE;
   Control &ct = *reinterpret_cast<Control *>(smem + (2 + ST) * SH::TILE);
   static_assert(sizeof(Control) <= 1024, "control block");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -510,7 +648,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   const uint32_t tmem = ct.tmem;
   pdl_wait();
 
-  // item number i, false where an error ends the kernel; lanes that do not wait must not read
+  // item number i; false where an error ends the kernel
   auto wait_item = [&](int i, int code) { return mbar_wait(&ct.item_full[i % ITEMS], (i / ITEMS) & 1, abort_flag, p.status, code); };
 
   if (warp >= WARP_LOAD) {
@@ -550,94 +688,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         }
       }
     } else if (warp == WARP_MMA) {
-      if (lane == 0) {
-        const int ksteps = (p.dim + 15) / 16;
-        const uint32_t id_s = idesc16(Kind<T>::BF16, false, BK), id_o = idesc16(Kind<T>::BF16, true, ksteps * 16);
-        int i = -1, np[2] = {0, 0}, nq[2] = {0, 0}, e = 0;        // e: the ring's number of the current key tile
-        bool ok = true;
-        Work cur, nxt;
-        // the next item that has key tiles; those without need nothing here. False: there is none, or an error (ok)
-        auto next_item = [&](Work &w) {
-          while (true) {
-            i++;
-            if (!(ok = wait_item(i, ST_MMA)) || ct.item[i % ITEMS].end) return false;
-            w = work_of(ct.item[i % ITEMS], p);
-            mbar_arrive(&ct.item_empty[i % ITEMS]);
-            if (w.lo < w.hi) return true;
-          }
-        };
-        auto wait_kv = [&](int k) { return mbar_wait(&ct.kv_full[k % ST], (k / ST) & 1, abort_flag, p.status, ST_MMA); };
-        auto issue_s = [&](int x, const Unit &u, int j, int k) {      // K, number k of the ring, has landed
-          if (j == u.lo) {
-            if (!(ok = mbar_wait(&ct.q_full[x], nq[x] & 1, abort_flag, p.status, ST_MMA))) return;
-            nq[x]++;
-          }
-          const uint32_t a = s_q + x * SH::TILE, b = s_kv + (k % ST) * SH::TILE;
-          tc_fence_after();
-          for (int ks = 0; ks < ksteps; ks++) {
-            const uint32_t off = (ks >> 2) * SH::BOX + (ks & 3) * 32;
-            umma_ss(tmem + x * 128, umma_smem_desc<128>(a + off), umma_smem_desc<128>(b + off), id_s, ks > 0);
-          }
-          umma_commit(&ct.s_full[x]);
-          if (j == u.hi - 1) umma_commit(&ct.q_empty[x]);
-        };
-        bool more = next_item(cur);
-        int j = 0;
-        if (more) {
-          j = cur.lo;
-          ok = wait_kv(0);
-#pragma unroll
-          for (int x = 0; x < 2; x++)
-            if (ok && sees(cur.u[x], j)) issue_s(x, cur.u[x], j, 0);
-          if (ok) umma_commit(&ct.kv_empty[0]);
-        }
-        while (more && ok) {
-          // the tile after this one, of this item or the next
-          const bool same = j + 1 < cur.hi;
-          int jn = j + 1;
-          if (same) {
-            nxt = cur;
-          } else {
-            more = next_item(nxt);
-            if (!ok) break;
-            jn = nxt.lo;
-          }
-          bool have_v = false, have_k = false;
-#pragma unroll
-          for (int x = 0; x < 2; x++) {
-            const Unit &u = cur.u[x];
-            if (ok && sees(u, j)) {
-              if (!have_v) {
-                have_v = true;
-                ok = wait_kv(e + 1) && mbar_wait(&ct.clean[((e + 1) % ST) >> 1], ((e + 1) / ST) & 1, abort_flag, p.status, ST_MMA);
-                if (!ok) break;
-              }
-              if (!(ok = mbar_wait(&ct.p_full[x], np[x] & 1, abort_flag, p.status, ST_MMA))) break;
-              np[x]++;
-              tc_fence_after();
-              const uint32_t b = s_kv + ((e + 1) % ST) * SH::TILE;
-              const int parts = min(BK / 16, (u.keys - j * BK + 15) / 16);      // keys that none of its rows sees are left out
-              for (int kk = 0; kk < parts; kk++)
-                umma_ts(tmem + 256 + x * DP, tmem + x * 128 + kk * 8, desc_v(b + kk * 2048), id_o, j > u.lo || kk > 0);
-              if (j == u.hi - 1) umma_commit(&ct.o_full[x]);
-            }
-            if (ok && more && sees(nxt.u[x], jn)) {
-              if (!have_k) { have_k = true; if (!(ok = wait_kv(e + 2))) break; }
-              issue_s(x, nxt.u[x], jn, e + 2);
-            }
-          }
-          if (!ok) break;
-          umma_commit(&ct.kv_empty[(e + 1) % ST]);
-          if (more) umma_commit(&ct.kv_empty[(e + 2) % ST]);
-          e += 2;
-          j = jn;
-          if (!same) cur = nxt;
-        }
-        // the MMAs issued so far end before TMEM is given back
-        volatile int never = 0;
-        umma_commit(&ct.drain);
-        mbar_wait(&ct.drain, 0, &never, p.status, ST_MMA);
-      }
+      mma_warp<T, DP>(ct, base, tmem, p);
     } else {
       guard_warp<T, DP>(ct, smem, p, warp == WARP_GUARD, threadIdx.x - WARP_GUARD * 32);
     }
