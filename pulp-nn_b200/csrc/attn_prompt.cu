@@ -12,7 +12,7 @@
 // sequence's last rows, which see the most keys, come first.
 //
 //   warps 0-3, 4-7  softmax of unit 0 and 1: a thread is a row. S comes from TMEM, the weights go back there as the 16-bit
-//                   operand of the second product, in the columns S had. At an item's end they also write its rows.
+//                   operand of the second product. At an item's end they also write its rows.
 //   warp 8          loads Q, then K and V tiles in turn, by TMA into a ring of stages
 //   warp 9          issues the MMAs: S = Q K^T (both from shared memory), O += P V (P from TMEM). While one unit's weights
 //                   are computed, the other unit's products run; an item's first S follow the last O of the one before.
@@ -21,11 +21,15 @@
 //                   sequence's) become 0, and so do infinities and NaN among the rest, which the epilogue then adds to
 //                   the rows that do see them. Warp 10 also fetches the items, one ahead.
 //
-// TMEM: S of unit 0 and 1 (128 columns each), O of unit 0 and 1 (64 or 128 each).
+// What bounds it: 128 keys of two units take the tensor cores 2048 (1024) cycles at 128 (64) channels, and the special
+// function units, 16 exponentials a cycle, 2048 cycles at any number of channels. What decides is therefore how much of a
+// unit's cycle S -> weights -> P V -> S is in the way of its own next step:
+//   64 channels: TMEM (512 columns) holds S, P and O of both units side by side. S of the next tile is computed as soon as
+//     the softmax warps have S in registers, and they never wait for it.
+//   128 channels: P has to lie in columns that S had, and the next S comes behind P V. The weights are handed over in two
+//     halves, so that the first half's product runs under the second half's exponentials.
 // The running maximum is a reference that has to be near the true one only: it is taken from an item's first tile, and raised
 // (O being rescaled in TMEM by the softmax warps themselves) when a weight comes out above 2^15, which is rare.
-// Between the commit that announces S(j) and its own arrival with P(j), a softmax group has O to itself: the
-// commit comes behind the MMAs of tile j - 1.
 #include "attention.cuh"
 #include "sm100_primitives.cuh"
 
@@ -55,15 +59,22 @@ template <int DP> struct Shape {
   static constexpr int BOXES = DP / 64;                        // of 64 channels: rows of 128 bytes, swizzled
   static constexpr int BOX = 128 * 128;                        // bytes
   static constexpr int TILE = BOXES * BOX;
+  // TMEM: S of unit 0 and 1, O of unit 0 and 1, and P of both where there is room
+  static constexpr bool APART = DP == 64;
+  static constexpr int O_AT = 256, P_AT = APART ? 256 + 2 * DP : 0, P_STEP = APART ? 64 : 128;
   static constexpr int STAGES = DP == 128 ? 4 : 8;             // even: keys in the even stages, values in the odd ones
   static constexpr int SMEM = (2 + STAGES) * TILE + 1024 /* barriers */ + 1024 /* alignment */;
 };
 
-struct Item { int end, q0, k0, lq, lk, pair, kvh, dirty; };
+// A tile of queries: rows row0 .. row0 + rows - 1 of head `head`, the first at position pos; it sees the key tiles lo .. hi - 1.
+struct Unit { int row0, rows, head, pos, lo, hi; };
+// An item's units and the key tiles lo .. hi - 1 that either sees.
+struct Work { Unit u[2]; int q0, k0, lk, kvh, lo, hi; };
+struct Item { Work w; int end, dirty; };
 constexpr int ITEMS = 3;
 
 struct Control {
-  uint64_t q_full[2], q_empty[2], kv_full[8], kv_empty[8], clean[4], s_full[2], p_full[2], o_full[2], item_full[ITEMS], item_empty[ITEMS], next, drain;
+  uint64_t q_full[2], q_empty[2], kv_full[8], kv_empty[8], clean[4], s_full[2], s_free[2], p_half[2], p_full[2], pv_done[2], o_full[2], item_full[ITEMS], item_empty[ITEMS], next, drain;
   uint4 answer;                    // to the request for another block's work
   Item item[ITEMS];
   uint32_t tmem;
@@ -157,31 +168,24 @@ template <typename T> struct Kind;
 template <> struct Kind<__half> { static constexpr bool BF16 = false; static constexpr unsigned EXP = 0x7c00u; };
 template <> struct Kind<__nv_bfloat16> { static constexpr bool BF16 = true; static constexpr unsigned EXP = 0x7f80u; };
 
-// A tile of queries: rows row0 .. row0 + rows - 1 of head `head`, the first at position pos; it sees the key tiles lo .. hi - 1.
-struct Unit { int row0, rows, head, pos, lo, hi, keys; };
-// An item's units and the key tiles lo .. hi - 1 that either sees.
-struct Work { Unit u[2]; int q0, k0, lk, kvh, lo, hi; };
-
-__device__ __forceinline__ Work work_of(const Item &it, const PromptProblem &p)
+__device__ __forceinline__ void make_work(Work &w, int q0, int lq, int k0, int lk, int pair, int kvh, const PromptProblem &p)
 {
-  Work w;
-  w.q0 = it.q0; w.k0 = it.k0; w.lk = it.lk; w.kvh = it.kvh;
-#pragma unroll
+  w.q0 = q0; w.k0 = k0; w.lk = lk; w.kvh = kvh;
+  w.lo = 0x7fffffff; w.hi = 0;
   for (int x = 0; x < 2; x++) {
-    const int n = 2 * it.pair + x, rt = n / p.group;
-    Unit &u = w.u[x];
-    u.row0 = rt * BQ; u.head = it.kvh * p.group + n - rt * p.group;
-    u.rows = min(max(it.lq - u.row0, 0), BQ);
-    u.pos = u.row0 + it.lk - it.lq;
-    u.keys = u.rows == 0 ? 0 : (p.causal ? min(it.lk, max(u.pos + u.rows, 0)) : it.lk);       // it sees none from here on
+    const int n = 2 * pair + x, rt = n / p.group;
+    Unit u;
+    u.row0 = rt * BQ; u.head = kvh * p.group + n - rt * p.group;
+    u.rows = min(max(lq - u.row0, 0), BQ);
+    u.pos = u.row0 + lk - lq;
+    const int keys = u.rows == 0 ? 0 : (p.causal ? min(lk, max(u.pos + u.rows, 0)) : lk);       // it sees none from here on
     const int from = p.window > 0 ? max(0, u.pos - p.window + 1) : 0;
-    u.lo = from / BK; u.hi = (u.keys + BK - 1) / BK;
-    if (from >= u.keys) u.lo = u.hi = 0;
+    u.lo = from / BK; u.hi = (keys + BK - 1) / BK;
+    if (from >= keys) u.lo = u.hi = 0;
+    else { w.lo = min(w.lo, u.lo); w.hi = max(w.hi, u.hi); }
+    w.u[x] = u;
   }
-  const bool any0 = w.u[0].hi > w.u[0].lo, any1 = w.u[1].hi > w.u[1].lo;
-  w.lo = !any0 ? w.u[1].lo : (!any1 ? w.u[0].lo : min(w.u[0].lo, w.u[1].lo));
-  w.hi = max(w.u[0].hi, w.u[1].hi);
-  return w;
+  w.lo = min(w.lo, w.hi);
 }
 __device__ __forceinline__ bool sees(const Unit &u, int j) { return j >= u.lo && j < u.hi; }
 // whether some row of the unit does not see some key of tile j
@@ -197,7 +201,7 @@ __device__ __forceinline__ bool guarded(const Work &w, int j, const PromptProble
 
 // Finds pair number x of the units of all sequences. The search goes on where the last one stopped: `before` pairs lie
 // ahead of sequence s0. A whole warp; false where there are not so many pairs.
-__device__ __forceinline__ bool find_item(const PromptProblem &p, int x, int lane, int &s0, int &before, Item &it)
+__device__ __forceinline__ bool find_item(const PromptProblem &p, int x, int y, int lane, int &s0, int &before, Item &it)
 {
   for (; s0 < p.seqs; s0 += 256) {              // eight sequences a lane
     int at[9], count[8], sum = 0;
@@ -230,9 +234,9 @@ __device__ __forceinline__ bool find_item(const PromptProblem &p, int x, int lan
     if (hit) {
       const int src = __ffs(hit) - 1;
       which = __shfl_sync(0xffffffffu, which, src);
-      it.q0 = __shfl_sync(0xffffffffu, q0, src); it.lq = __shfl_sync(0xffffffffu, lq, src); it.pair = __shfl_sync(0xffffffffu, pair, src);
-      it.k0 = min(max(__ldg(p.cu_k + which), 0), p.nk);
-      it.lk = min(max(__ldg(p.cu_k + which + 1), it.k0), p.nk) - it.k0;
+      q0 = __shfl_sync(0xffffffffu, q0, src); lq = __shfl_sync(0xffffffffu, lq, src); pair = __shfl_sync(0xffffffffu, pair, src);
+      const int k0 = min(max(__ldg(p.cu_k + which), 0), p.nk), lk = min(max(__ldg(p.cu_k + which + 1), k0), p.nk) - k0;
+      if (lane == 0) make_work(it.w, q0, lq, k0, lk, pair, y, p);
       return true;
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
@@ -254,8 +258,8 @@ __device__ __forceinline__ void guard_warp(Control &ct, char *smem, const Prompt
   // publishes item number i
   auto publish = [&](int i) {
     ok = __all_sync(0xffffffffu, mbar_wait(&ct.item_empty[i % ITEMS], ((i / ITEMS) & 1) ^ 1, abort_flag, p.status, ST_GUARD));
-    Item it = {1, 0, 0, 0, 0, 0, 0, 0};
-    bool own = i == 0;
+    Item &it = ct.item[i % ITEMS];
+    bool own = i == 0, found = false;
     while (ok) {
       int x = blockIdx.x, y = blockIdx.y;
       bool got = true;
@@ -272,12 +276,11 @@ __device__ __forceinline__ void guard_warp(Control &ct, char *smem, const Prompt
       if (lane == 0) ask_for_block(&ct.answer, &ct.next);
       asked++; pending = true;
       if (y != row || x < before) { row = y; s0 = 0; before = 0; }
-      it.kvh = y;
-      if (find_item(p, x, lane, s0, before, it)) { it.end = 0; break; }
+      if ((found = find_item(p, x, y, lane, s0, before, it))) break;
       // a block beyond the last pair: the grid is made for the most there can be
     }
     if (lane == 0) {
-      ct.item[i % ITEMS] = it;
+      it.end = !found; it.dirty = 0;
       mbar_arrive(&ct.item_full[i % ITEMS]);
     }
     __syncwarp();
@@ -287,9 +290,10 @@ __device__ __forceinline__ void guard_warp(Control &ct, char *smem, const Prompt
   for (int i = 0; ok; i++) {
     ok = __all_sync(0xffffffffu, mbar_wait(&ct.item_full[i % ITEMS], (i / ITEMS) & 1, abort_flag, p.status, ST_GUARD));
     if (!ok || ct.item[i % ITEMS].end) break;
-    const Work w = work_of(ct.item[i % ITEMS], p);
+    const Work &w = ct.item[i % ITEMS].w;
     if (fetches) publish(i + 1);
-    for (int j = w.lo; j < w.hi && ok; j++, e += 2) {
+    const int lo = w.lo, hi = w.hi;
+    for (int j = lo; j < hi && ok; j++, e += 2) {
       const int st = e % ST;
       ok = __all_sync(0xffffffffu, mbar_wait(&ct.kv_full[st], (e / ST) & 1, abort_flag, p.status, ST_GUARD));
       if (!ok) break;
@@ -328,7 +332,7 @@ __device__ __noinline__ bool wait_long(uint64_t *bar, uint32_t parity, volatile 
   return mbar_wait(bar, parity, abort_flag, status, code);
 }
 
-// Warp 9: issues the MMAs. The whole warp walks through the tiles, so that what the instructions take from uniform
+// Warp 17: issues the MMAs. The whole warp walks through the tiles, so that what the instructions take from uniform
 // registers is computed there; one lane issues and commits.
 template <typename T, int DP>
 __device__ __forceinline__ void mma_warp(Control &ct, uint32_t base, uint32_t tmem_, const PromptProblem &p)
@@ -347,7 +351,7 @@ __device__ __forceinline__ void mma_warp(Control &ct, uint32_t base, uint32_t tm
   const uint32_t k_low = __shfl_sync(0xffffffffu, (((base + 2 * SH::TILE) & 0x3ffffu) >> 4) | DESC_K_LOW, 0);
   const uint32_t v_low = __shfl_sync(0xffffffffu, (((base + 2 * SH::TILE) & 0x3ffffu) >> 4) | DESC_V_LOW, 0);
   const uint32_t id_s = idesc16(Kind<T>::BF16, false, BK), id_o = idesc16(Kind<T>::BF16, true, (p.dim + 15) / 16 * 16);
-  int i = -1, np[2] = {0, 0}, nq[2] = {0, 0}, e = 0;        // e: the ring's number of the current key tile
+  int i = -1, np[2] = {0, 0}, nq[2] = {0, 0}, ns[2] = {0, 0}, e = 0;        // e: the ring's number of the current key tile
   struct Range { int lo, hi, ulo[2], uhi[2]; } cur, nxt;      // key tiles of an item and of its units
   // the next item that has key tiles; those without need nothing here. False: there is none, or an error (ok)
   auto next_item = [&](Range &r) {
@@ -355,12 +359,13 @@ __device__ __forceinline__ void mma_warp(Control &ct, uint32_t base, uint32_t tm
       i++;
       wait(&ct.item_full[i % ITEMS], (i / ITEMS) & 1);
       if (__any_sync(0xffffffffu, !ok) || __any_sync(0xffffffffu, ct.item[i % ITEMS].end)) return false;
-      const Work w = work_of(ct.item[i % ITEMS], p);
+      const Work &w = ct.item[i % ITEMS].w;
       r.lo = __shfl_sync(0xffffffffu, w.lo, 0); r.hi = __shfl_sync(0xffffffffu, w.hi, 0);
 #pragma unroll
       for (int x = 0; x < 2; x++) {
         r.ulo[x] = __shfl_sync(0xffffffffu, w.u[x].lo, 0); r.uhi[x] = __shfl_sync(0xffffffffu, w.u[x].hi, 0);
       }
+      __syncwarp();
       if (leader) mbar_arrive(&ct.item_empty[i % ITEMS]);
       if (r.lo < r.hi) return true;
     }
@@ -373,6 +378,11 @@ __device__ __forceinline__ void mma_warp(Control &ct, uint32_t base, uint32_t tm
       nq[x]++;
       tc_fence_after();
     }
+    if (SH::APART && ns[x] > 0) {              // the softmax has the last S in registers
+      wait(&ct.s_free[x], (ns[x] - 1) & 1);
+      tc_fence_after();
+    }
+    ns[x]++;
     const uint32_t a = q_low + x * (SH::TILE >> 4), b = k_low + (k % ST) * (SH::TILE >> 4);
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ks++) {
@@ -405,21 +415,36 @@ __device__ __forceinline__ void mma_warp(Control &ct, uint32_t base, uint32_t tm
     wait(&ct.clean[((e + 1) % ST) >> 1], ((e + 1) / ST) & 1);
     if (more) wait_kv(e + 2);
     if (__any_sync(0xffffffffu, !ok)) break;
+    const uint32_t b = v_low + ((e + 1) % ST) * (SH::TILE >> 4);
+    auto next_s = [&](int x) {
+      const int lo_n = same ? cur.ulo[x] : nxt.ulo[x], hi_n = same ? cur.uhi[x] : nxt.uhi[x];
+      if (more && jn >= lo_n && jn < hi_n) issue_s(x, lo_n, hi_n, jn, e + 2);
+    };
+    if (SH::APART) {
+#pragma unroll
+      for (int x = 0; x < 2; x++) next_s(x);
+    }
 #pragma unroll
     for (int x = 0; x < 2; x++) {
       if (j >= cur.ulo[x] && j < cur.uhi[x]) {
+        const bool begun = j > cur.ulo[x], last = j == cur.uhi[x] - 1;
+        const uint32_t o = tmem + SH::O_AT + x * DP, w = tmem + SH::P_AT + x * SH::P_STEP;
+        if (!SH::APART) {
+          wait(&ct.p_half[x], np[x] & 1);
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 4; kk++) umma_ts(leader, o, w + kk * 8, desc_of(b + kk * (2048 >> 4)), id_o, begun || kk > 0);
+          umma_commit_by(leader, &ct.pv_done[x]);         // of the first half
+        }
         wait(&ct.p_full[x], np[x] & 1);
         np[x]++;
         tc_fence_after();
-        const uint32_t b = v_low + ((e + 1) % ST) * (SH::TILE >> 4);
-        const bool begun = j > cur.ulo[x], last = j == cur.uhi[x] - 1;
 #pragma unroll
-        for (int kk = 0; kk < BK / 16; kk++)
-          umma_ts(leader, tmem + 256 + x * DP, tmem + x * 128 + kk * 8, desc_of(b + kk * (2048 >> 4)), id_o, begun || kk > 0);
+        for (int kk = SH::APART ? 0 : 4; kk < 8; kk++) umma_ts(leader, o, w + kk * 8, desc_of(b + kk * (2048 >> 4)), id_o, begun || kk > 0);
+        if (SH::APART) umma_commit_by(leader, &ct.pv_done[x]);
         if (last) umma_commit_by(leader, &ct.o_full[x]);
       }
-      const int lo_n = same ? cur.ulo[x] : nxt.ulo[x], hi_n = same ? cur.uhi[x] : nxt.uhi[x];
-      if (more && jn >= lo_n && jn < hi_n) issue_s(x, lo_n, hi_n, jn, e + 2);
+      if (!SH::APART) next_s(x);
     }
     umma_commit_by(leader, &ct.kv_empty[(e + 1) % ST]);
     if (more) umma_commit_by(leader, &ct.kv_empty[(e + 2) % ST]);
@@ -468,38 +493,38 @@ __device__ __forceinline__ float max3(float a, float b, float c)
 template <typename T, int DP>
 __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t tmem, const PromptProblem &p)
 {
+  using SH = Shape<DP>;
   volatile int *abort_flag = &ct.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, x = warp >> 2, r = threadIdx.x & 127;
   const uint32_t rowbase = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-  const uint32_t t_s = rowbase + x * 128, t_o = rowbase + 256 + x * DP;
-  const int cols = (p.dim + 15) / 16;
+  const uint32_t t_s = rowbase + x * 128, t_o = rowbase + SH::O_AT + x * DP, t_p = rowbase + SH::P_AT + x * SH::P_STEP;
+  const int groups = (p.dim + 15) / 16;
   const uint64_t scale2 = pair2(p.scale_log2, p.scale_log2);
-  uint32_t s_phase = 0, o_phase = 0;
+  uint32_t done = 0, o_phase = 0;              // tiles of this unit; item ends
   bool ok = true;
   for (int i = 0; ok; i++) {
     if (!(ok = mbar_wait(&ct.item_full[i % ITEMS], (i / ITEMS) & 1, abort_flag, p.status, ST_SOFTMAX))) break;
     const Item &it = ct.item[i % ITEMS];
     if (it.end) break;
-    Unit w;
-    int q0, k0, lk, kvh;
-    {
-      const Work all = work_of(it, p);
-      w = x == 0 ? all.u[0] : all.u[1];
-      q0 = all.q0; k0 = all.k0; lk = all.lk; kvh = all.kvh;
-    }
+    const Unit w = it.w.u[x];
+    const int lk = it.w.lk;
     const int pos = w.pos + r;
     const int last = p.causal ? min(lk - 1, pos) : lk - 1, first = p.window > 0 ? pos - p.window + 1 : 0;
     // every row sees every key of the tiles whole_lo .. whole_hi - 1
     const int whole_hi = (p.causal ? min(lk, max(w.pos + 1, 0)) : lk) / BK, whole_lo = p.window > 0 ? (max(w.pos + w.rows - p.window, 0) + BK - 1) / BK : 0;
     float m = NOTHING, l = 0.f;
-    for (int j = w.lo; j < w.hi; j++) {
-      if (!(ok = mbar_wait(&ct.s_full[x], s_phase, abort_flag, p.status, ST_SOFTMAX))) break;
-      s_phase ^= 1;
+    for (int j = w.lo; j < w.hi; j++, done++) {
+      if (!(ok = mbar_wait(&ct.s_full[x], done & 1, abort_flag, p.status, ST_SOFTMAX))) break;
       tc_fence_after();
       uint32_t s[4][32];
 #pragma unroll
       for (int k = 0; k < 4; k++) tmem_ld_32(t_s + k * 32, s[k]);
       tmem_wait_ld();
+      if (SH::APART) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ct.s_free[x]);
+      }
       if (j >= whole_hi || j < whole_lo) {
         const int a = first - j * BK, b = last - j * BK;
 #pragma unroll
@@ -508,56 +533,88 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t tmem, const 
           for (int c = 0; c < 32; c++)
             if (k * 32 + c < a || k * 32 + c > b) s[k][c] = 0xff800000u;
       }
+      // A new reference: the maximum so far. O is rescaled where it holds something (`has`); its products have ended.
+      auto raise = [&](bool has) {
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 32; c += 2)
+#pragma unroll
+          for (int k = 0; k < 4; k++) top[k] = max3(top[k], __uint_as_float(s[k][c]), __uint_as_float(s[k][c + 1]));
+        const float most = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * p.scale_log2;
+        if (!(most <= 3e38f)) l = __int_as_float(0x7fffffff);        // a NaN or an infinity among the scores
+        const float to = fmaxf(m, most), f = ex2(m - to);
+        m = to;
+        l *= f;
+        if (has) {
+          for (int c = 0; c < groups; c++) {
+            uint32_t o[16];
+            tmem_ld_16(t_o + c * 16, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+            tmem_st_16(t_o + c * 16, o);
+          }
+        }
+      };
+      // the weights of 32 keys, as the second product wants them, and their sum
+      auto weights = [&](int k, uint64_t off2) {
+        uint64_t sum = 0;
+        uint32_t w16[16];
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          const uint64_t a = fma2(pair2(__uint_as_float(s[k][c]), __uint_as_float(s[k][c + 1])), scale2, off2);
+          const float2 e = make_float2(ex2(both(a).x), ex2(both(a).y));
+          sum = add2(sum, pair2(e.x, e.y));
+          w16[c / 2] = pack2<T>(e.x, e.y);       // off by 2^-8 (bf16) or 2^-11 (fp16) of each weight at most; their sum is taken unrounded
+        }
+        tmem_st_16(t_p + k * 16, w16);
+        return sum;
+      };
+      auto hand_over = [&](uint64_t *bar) {
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+      };
       // With the reference as it is; with a new one where there is none yet, or where the weights' sum shows that one of them is
       // beyond 2^15 (or no number). In between, the scores' maximum is not looked for: that took a fifth of the time.
-      bool raise = j == w.lo;
-      float2 total;
-      while (true) {
-        if (raise) {
-          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      bool raised = j == w.lo;
+      if (raised) raise(false);
+      if (SH::APART) {
+        if (done > 0 && !(ok = mbar_wait(&ct.pv_done[x], (done - 1) & 1, abort_flag, p.status, ST_SOFTMAX))) break;
+        tc_fence_after();
+        while (true) {
+          const uint64_t off2 = pair2(-m, -m);
+          uint64_t sum[4];
 #pragma unroll
-          for (int c = 0; c < 32; c += 2)
+          for (int k = 0; k < 4; k++) sum[k] = weights(k, off2);
+          const float2 v = both(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+          if (raised || !__any_sync(0xffffffffu, !(v.x + v.y < 32768.f))) { l += v.x + v.y; break; }
+          raised = true;
+          raise(true);
+        }
+        hand_over(&ct.p_full[x]);
+      } else {
 #pragma unroll
-            for (int k = 0; k < 4; k++) top[k] = max3(top[k], __uint_as_float(s[k][c]), __uint_as_float(s[k][c + 1]));
-          const float most = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * p.scale_log2;
-          if (!(most <= 3e38f)) l = __int_as_float(0x7fffffff);        // a NaN or an infinity among the scores
-          const float to = fmaxf(m, most), f = ex2(m - to);
-          m = to;
-          l *= f;
-          if (j > w.lo) {
-            for (int c = 0; c < cols; c++) {
-              uint32_t o[16];
-              tmem_ld_16(t_o + c * 16, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-              tmem_st_16(t_o + c * 16, o);
+        for (int h = 0; h < 2; h++) {
+          while (true) {
+            const uint64_t off2 = pair2(-m, -m);
+            const uint64_t a = weights(2 * h, off2), b = weights(2 * h + 1, off2);
+            const float2 v = both(add2(a, b));
+            if (raised || !__any_sync(0xffffffffu, !(v.x + v.y < 32768.f))) { l += v.x + v.y; break; }
+            raised = true;
+            // the second half: the first half's product must have ended before O is rescaled
+            if (h == 1) {
+              if (!(ok = mbar_wait(&ct.pv_done[x], done & 1, abort_flag, p.status, ST_SOFTMAX))) break;
+              tc_fence_after();
             }
+            raise(h == 1 || j > w.lo);
           }
+          if (!ok) break;
+          hand_over(h == 0 ? &ct.p_half[x] : &ct.p_full[x]);
         }
-        const uint64_t off2 = pair2(-m, -m);
-        uint64_t sum[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          uint32_t w16[16];
-#pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            const uint64_t a = fma2(pair2(__uint_as_float(s[k][c]), __uint_as_float(s[k][c + 1])), scale2, off2);
-            const float2 e = make_float2(ex2(both(a).x), ex2(both(a).y));
-            sum[k] = add2(sum[k], pair2(e.x, e.y));
-            w16[c / 2] = pack2<T>(e.x, e.y);       // off by 2^-8 (bf16) or 2^-11 (fp16) of each weight at most; their sum is taken unrounded
-          }
-          tmem_st_16(t_s + k * 16, w16);
-        }
-        total = both(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
-        if (raise || !__any_sync(0xffffffffu, !(total.x + total.y < 32768.f))) break;
-        raise = true;
+        if (!ok) break;
       }
-      l += total.x + total.y;
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ct.p_full[x]);
     }
     if (!ok) break;
     // ---- the rows ----
@@ -568,11 +625,11 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t tmem, const 
       tc_fence_after();
     }
     const bool live = r < w.rows;
-    const int64_t row = q0 + w.row0 + r;
+    const int64_t row = it.w.q0 + w.row0 + r;
     const float inv = l == 0.f ? 0.f : 1.f / l;         // a row that sees nothing is zero
     char *dst = p.out + row * p.out_row + (int64_t)w.head * p.out_head;
     const bool dirty = any && *reinterpret_cast<const volatile int *>(&it.dirty);
-    for (int c = 0; c < cols; c++) {
+    for (int c = 0; c < groups; c++) {
       float y[16];
       if (any) {
         uint32_t o[16];
@@ -585,11 +642,11 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t tmem, const 
         for (int k = 0; k < 16; k++) y[k] = 0.f;
       }
       if (dirty && live) {      // the infinities and NaN that the guards took out of the tiles, where this row sees them
-        const Work all = work_of(it, p);
+        const Work &all = it.w;
         for (int j = w.lo; j < w.hi; j++) {
           if (!guarded(all, j, p)) continue;
           for (int k = max(first, j * BK); k <= min(last, j * BK + BK - 1); k++) {
-            const T *v = reinterpret_cast<const T *>(p.v + (int64_t)(k0 + k) * p.v_row + (int64_t)kvh * p.v_head) + c * 16;
+            const T *v = reinterpret_cast<const T *>(p.v + (int64_t)(all.k0 + k) * p.v_row + (int64_t)all.kvh * p.v_head) + c * 16;
 #pragma unroll
             for (int n = 0; n < 16; n++)
               if (c * 16 + n < p.dim) {
@@ -633,7 +690,8 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   if (threadIdx.x == 0) {
     ct.abort_flag = 0;
     for (int x = 0; x < 2; x++) {
-      mbar_init(&ct.q_full[x], 1); mbar_init(&ct.q_empty[x], 1); mbar_init(&ct.s_full[x], 1); mbar_init(&ct.p_full[x], 4); mbar_init(&ct.o_full[x], 1);
+      mbar_init(&ct.q_full[x], 1); mbar_init(&ct.q_empty[x], 1); mbar_init(&ct.s_full[x], 1); mbar_init(&ct.o_full[x], 1);
+      mbar_init(&ct.s_free[x], 4); mbar_init(&ct.p_half[x], 4); mbar_init(&ct.p_full[x], 4); mbar_init(&ct.pv_done[x], 1);
     }
     for (int s = 0; s < ST; s++) { mbar_init(&ct.kv_full[s], 1); mbar_init(&ct.kv_empty[s], 1); }
     for (int s = 0; s < ST / 2; s++) mbar_init(&ct.clean[s], 2);
@@ -659,7 +717,8 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         bool ok = true;
         for (int i = 0; ok; i++) {
           if (!(ok = wait_item(i, ST_LOAD)) || ct.item[i % ITEMS].end) break;
-          const Work w = work_of(ct.item[i % ITEMS], p);
+          const Work &w = ct.item[i % ITEMS].w;
+          const int hi = w.hi, kvh = w.kvh, k0 = w.k0;
 #pragma unroll
           for (int x = 0; x < 2; x++) {
             if (!ok || w.u[x].hi <= w.u[x].lo) continue;
@@ -669,12 +728,12 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
               tma_load_3d(smem + x * SH::TILE + b * SH::BOX, &map_q, &ct.q_full[x], b * 64, w.u[x].head, w.q0 + w.u[x].row0);
             nq[x]++;
           }
-          for (int j2 = 2 * w.lo; j2 < 2 * w.hi && ok; j2++) {
+          for (int j2 = 2 * w.lo; j2 < 2 * hi && ok; j2++) {
             const int st = e % ST;
             if (!(ok = mbar_wait(&ct.kv_empty[st], ((e / ST) & 1) ^ 1, abort_flag, p.status, ST_LOAD))) break;
             mbar_arrive_expect_tx(&ct.kv_full[st], SH::TILE);
             for (int b = 0; b < SH::BOXES; b++)
-              tma_load_3d(smem + (2 + st) * SH::TILE + b * SH::BOX, e & 1 ? &map_v : &map_k, &ct.kv_full[st], b * 64, w.kvh, w.k0 + (j2 >> 1) * BK);
+              tma_load_3d(smem + (2 + st) * SH::TILE + b * SH::BOX, e & 1 ? &map_v : &map_k, &ct.kv_full[st], b * 64, kvh, k0 + (j2 >> 1) * BK);
             e++;
           }
           mbar_arrive(&ct.item_empty[i % ITEMS]);
