@@ -10,10 +10,11 @@
 // would want 128 rows, M = tokens, for 16 bytes of results each: it reads its operands from shared memory just the
 // same, and its accumulators would have to come back through TMEM for the running maximum.
 //
-// A warp works alone: tiles of 16 (8-bit: 32) tokens, fetched by itself with 16-byte cp.async into STAGES buffers of its own;
-// there is no barrier between warps until the end. Each lane looks up the page of one token, one tile ahead of
-// its fetch, so pages of any size may end anywhere in a tile, and tokens behind the end are filled with zeros
-// without being read. WARPS warps are a CTA, CTAs of a cluster share a sequence, and the partial results are joined
+// A warp works alone: tiles of 16 (8-bit or up to 64 channels: 32) tokens, fetched by itself into STAGES buffers of its own;
+// there is no barrier between warps until the end. Each lane looks up the page of one token, one tile ahead of its
+// fetch. Where pages are a multiple of 16 slots, every 16 tokens lie in one page and come by one TMA copy for each 128 bytes of
+// their rows: copies of 16 bytes with a page each cost as many instructions as all the arithmetic. Pages of any
+// other size are fetched with these (16-byte cp.async), tokens behind the end without being read. WARPS warps are a CTA, CTAs of a cluster share a sequence, and the partial results are joined
 // through (distributed) shared memory in a fixed order: no workspace, no atomics, the same result every time.
 //
 // Running maximum: the reference m only has to be near the true maximum, not equal to it. It is raised (and the sums
@@ -35,7 +36,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int WARPS = 4, STAGES = 3;
+#ifndef DEC_STAGES
+#define DEC_STAGES 3
+#endif
+constexpr int WARPS = 4, STAGES = DEC_STAGES;
 constexpr float LAG = 8.f, NOTHING = -1e30f;
 
 struct DecodeProblem {
@@ -49,6 +53,8 @@ struct DecodeProblem {
   int hq, group, head_tiles, dim, max_pages, window, q_type, out_type;
   float scale_log2, out_inv_step;
   int out_zero, splits;
+  int box;                                       // tokens of a TMA copy: 16 or a whole tile
+  int *status;
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool live)
@@ -103,13 +109,22 @@ __device__ __forceinline__ float load_q(const char *p, int type)
   return type == PULPNN_TYPE_F16 ? __half2float(*reinterpret_cast<const __half *>(p)) : __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(p));
 }
 
+// Rows of 128 bytes (a box of 64 16-bit channels or of up to 128 8-bit ones), whose 16-byte chunks are swizzled by their row the way
+// TMA does it: eight rows of one chunk lie in different banks.
 template <int DP, bool EIGHT> struct Tile {
   static constexpr int SIZE = EIGHT ? 1 : 2;
-  static constexpr int TOKENS = EIGHT ? 32 : 16;
-  static constexpr int ROW = DP * SIZE + 16;                 // padded: 8 rows of one 16-byte column lie in different banks
+  static constexpr int TOKENS = EIGHT || DP <= 64 ? 32 : 16;
+  static constexpr int BOXES = EIGHT || DP <= 64 ? 1 : 2;
+  static constexpr int BOX = TOKENS * 128;                   // bytes
   static constexpr int CHUNKS = DP * SIZE / 16;              // of a row
-  static constexpr int STAGE = 2 * TOKENS * ROW + (EIGHT ? 2 * TOKENS * 4 : 0);
+  static constexpr int STAGE = 2 * BOXES * BOX;              // keys, values
   static constexpr int PIPE = WARPS * STAGES * STAGE;
+  static constexpr int SCALES = EIGHT ? WARPS * STAGES * 2 * TOKENS * 4 : 0;
+  // address of a 16-byte chunk of a token's row, from the tile's first byte
+  static __device__ __forceinline__ uint32_t at(int token, int chunk)
+  {
+    return (BOXES > 1 ? (chunk >> 3) * BOX : 0) + token * 128 + (((chunk & 7) ^ (token & 7)) << 4);
+  }
 };
 // what the join needs, in the pipeline's place: per warp [heads][DP] sums, then the CTA's
 template <int DP, int NT> struct Join {
@@ -118,18 +133,23 @@ template <int DP, int NT> struct Join {
   static constexpr int STATS = 3 * HEADS;                    // m, l, reference of the sums
   static constexpr int BYTES = (WARPS * (WARP + STATS) + WARP + STATS) * 4;
 };
-template <int DP, int NT, bool EIGHT> constexpr int decode_smem()
-{
-  return Tile<DP, EIGHT>::PIPE > Join<DP, NT>::BYTES ? Tile<DP, EIGHT>::PIPE : Join<DP, NT>::BYTES;
-}
+// dynamic shared memory: the pipeline, or the join in its place; the scales; room to align the whole
+template <int DP, int NT, bool EIGHT> struct Smem {
+  static constexpr int PIPE = Tile<DP, EIGHT>::PIPE > Join<DP, NT>::BYTES ? Tile<DP, EIGHT>::PIPE : Join<DP, NT>::BYTES;
+  static constexpr int BYTES = PIPE + Tile<DP, EIGHT>::SCALES + 1024;
+};
 
-template <typename T, int DP, int NT, bool EIGHT>
-__global__ void __launch_bounds__(WARPS * 32) attn_decode_kernel(const DecodeProblem p)
+template <typename T, int DP, int NT, bool EIGHT, bool TMA>
+__global__ void __launch_bounds__(WARPS * 32)
+attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const DecodeProblem p)
 {
   using TL = Tile<DP, EIGHT>;
   using JN = Join<DP, NT>;
-  constexpr int KS = DP / 16, MT = TL::TOKENS / 16, COPIES = TL::TOKENS * TL::CHUNKS / 32;
-  extern __shared__ __align__(128) char smem[];
+  constexpr int KS = DP / 16, MT = TL::TOKENS / 16;
+  extern __shared__ char raw[];
+  __shared__ uint64_t full[WARPS][STAGES];
+  __shared__ int abort_flag;
+  char *smem = raw + (((sm100::smem_u32(raw) + 1023u) & ~1023u) - sm100::smem_u32(raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = blockIdx.x % p.splits;
@@ -138,53 +158,81 @@ __global__ void __launch_bounds__(WARPS * 32) attn_decode_kernel(const DecodePro
   const int kvh = rest % p.cache.n_heads, seq = rest / p.cache.n_heads;
   const int h0 = kvh * p.group + ht * NT * 8, heads = min(NT * 8, p.group - ht * NT * 8);
 
-  if (p.dim < DP) {       // channels behind the head's own stay zero: a NaN there would spoil the product with q's zeros
+  if (TMA) {
+    if (threadIdx.x == 0) {
+      abort_flag = 0;
+      for (int i = 0; i < WARPS * STAGES; i++) sm100::mbar_init(&full[0][0] + i, 1);
+      sm100::mbar_fence_init();
+    }
+    __syncthreads();
+  } else if (p.dim < DP) {       // channels behind the head's own stay zero: a NaN there would spoil the product with q's zeros
     for (int i = threadIdx.x; i < TL::PIPE / 16; i += WARPS * 32) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
   }
   pdl_wait();
   const int n = min(max(__ldg(p.lens + seq), 0), p.max_pages * p.cache.page_size);
-  const int first = p.window > 0 ? max(0, n - p.window) : 0;
-  const int tiles = (n - first + TL::TOKENS - 1) / TL::TOKENS;
+  const int first = p.window > 0 ? max(0, n - p.window) : 0, origin = TMA ? first & ~15 : first;      // of the tiles
+  const int tiles = (n - origin + TL::TOKENS - 1) / TL::TOKENS;
   const int lo = (int)((int64_t)tiles * rank / p.splits), hi = (int)((int64_t)tiles * (rank + 1) / p.splits);
   const int mine = hi - lo > warp ? (hi - lo - warp + WARPS - 1) / WARPS : 0;       // tiles lo + warp + i * WARPS
 
-  const uint32_t pipe = sm100::smem_u32(smem) + warp * STAGES * TL::STAGE;
+  char *pipe_at = smem + warp * STAGES * TL::STAGE;
+  const uint32_t pipe = sm100::smem_u32(pipe_at);
+  const uint32_t scales = sm100::smem_u32(smem) + Smem<DP, NT, EIGHT>::PIPE + warp * STAGES * 2 * TL::TOKENS * 4;
   const int *table = p.table + seq * p.table_stride;
   // the page of this lane's token of tile i; -1 where there is none
   auto page_of = [&](int i, int &at) -> int {
-    const int token = first + (lo + warp + i * WARPS) * TL::TOKENS + (lane & (TL::TOKENS - 1));
+    const int token = origin + (lo + warp + i * WARPS) * TL::TOKENS + (lane & (TL::TOKENS - 1));
     at = 0;
     if (i >= mine || token >= n) return -1;
     const int in_row = p.cache.by_page.div(token), page = __ldg(table + in_row);
     at = token - in_row * p.cache.page_size;
     return page >= 0 && page < p.cache.n_pages ? page : -1;
   };
-  unsigned live_ring = 0;      // STAGES words of bits would be as good: bit (stage) of lane's token
+  unsigned live_ring = 0;      // bit `stage`: whether this lane's token of that stage counts
   auto fetch = [&](int i, int page, int at) {
     const int stage = i % STAGES;
     const uint32_t base = pipe + stage * TL::STAGE;
-    const bool live = page >= 0;
-    const int64_t off = live ? row_of(p.cache, page, at, kvh) * TL::SIZE : 0;
+    const bool live = page >= 0 && (!TMA || origin + (lo + warp + i * WARPS) * TL::TOKENS + (lane & (TL::TOKENS - 1)) >= first);
     live_ring = (live_ring & ~(1u << stage)) | (live ? 1u << stage : 0u);
     if (i < mine) {
+      if (TMA) {
+        // a page that is none lies outside the map, and its rows become zero
+        const int page16 = TL::TOKENS > 16 ? __shfl_sync(0xffffffffu, page, 16) : 0, at16 = TL::TOKENS > 16 ? __shfl_sync(0xffffffffu, at, 16) : 0;
+        if (lane == 0) {
+          uint64_t *bar = &full[warp][stage];
+          char *dst = pipe_at + stage * TL::STAGE;
+          sm100::mbar_arrive_expect_tx(bar, TL::STAGE);
 #pragma unroll
-      for (int j = 0; j < COPIES; j++) {
-        const int item = lane + 32 * j, row = item / TL::CHUNKS, chunk = item % TL::CHUNKS;
-        const int64_t o = __shfl_sync(0xffffffffu, off, row);
-        const bool ok = __shfl_sync(0xffffffffu, live, row);
-        if (chunk * 16 < p.dim * TL::SIZE) {
-          cp_async16(base + row * TL::ROW + chunk * 16, p.cache.k + (ok ? o + chunk * 16 : 0), ok);
-          cp_async16(base + (TL::TOKENS + row) * TL::ROW + chunk * 16, p.cache.v + (ok ? o + chunk * 16 : 0), ok);
+          for (int b = 0; b < TL::BOXES; b++) {
+            sm100::tma_load_4d(dst + b * TL::BOX, &map_k, bar, b * 64, at, kvh, page);
+            sm100::tma_load_4d(dst + (TL::BOXES + b) * TL::BOX, &map_v, bar, b * 64, at, kvh, page);
+            if (TL::TOKENS > 16 && p.box == 16) {
+              sm100::tma_load_4d(dst + b * TL::BOX + 2048, &map_k, bar, b * 64, at16, kvh, page16);
+              sm100::tma_load_4d(dst + (TL::BOXES + b) * TL::BOX + 2048, &map_v, bar, b * 64, at16, kvh, page16);
+            }
+          }
+        }
+      } else {
+        const int64_t off = live ? row_of(p.cache, page, at, kvh) * TL::SIZE : 0;
+#pragma unroll
+        for (int j = 0; j < TL::TOKENS * TL::CHUNKS / 32; j++) {
+          const int item = lane + 32 * j, row = item / TL::CHUNKS, chunk = item % TL::CHUNKS;
+          const int64_t o = __shfl_sync(0xffffffffu, off, row);
+          const bool ok = __shfl_sync(0xffffffffu, live, row);
+          if (chunk * 16 < p.dim * TL::SIZE) {
+            cp_async16(base + TL::at(row, chunk), p.cache.k + (ok ? o + chunk * 16 : 0), ok);
+            cp_async16(base + TL::BOXES * TL::BOX + TL::at(row, chunk), p.cache.v + (ok ? o + chunk * 16 : 0), ok);
+          }
         }
       }
       if (EIGHT) {
         const int64_t s = live ? scale_of(p.cache, page, at, kvh) : 0;
-        cp_async4(base + 2 * TL::TOKENS * TL::ROW + lane * 4, p.cache.k_scale + s, live);
-        cp_async4(base + 2 * TL::TOKENS * TL::ROW + (32 + lane) * 4, p.cache.v_scale + s, live);
+        cp_async4(scales + (stage * 2 * TL::TOKENS + lane) * 4, p.cache.k_scale + s, live);
+        cp_async4(scales + ((stage * 2 + 1) * TL::TOKENS + lane) * 4, p.cache.v_scale + s, live);
       }
     }
-    cp_commit();
+    if (EIGHT || !TMA) cp_commit();
   };
   int page_next, at_next;
   {
@@ -247,13 +295,27 @@ __global__ void __launch_bounds__(WARPS * 32) attn_decode_kernel(const DecodePro
     l[nt][0] = l[nt][1] = 0.f;
   }
 
+  bool landed = true;
   for (int i = 0; i < mine; i++) {
+    const int stage = i % STAGES;
     fetch(i + STAGES - 1, page_next, at_next);
     page_next = page_of(i + STAGES, at_next);
-    cp_wait<STAGES - 1>();
+    if (EIGHT || !TMA) cp_wait<STAGES - 1>();
+    if (TMA) landed = sm100::mbar_wait(&full[warp][stage], (i / STAGES) & 1, &abort_flag, p.status, 1 << 25) && landed;
     __syncwarp();
-    const uint32_t base = pipe + (i % STAGES) * TL::STAGE, vbase = base + TL::TOKENS * TL::ROW, sbase = base + 2 * TL::TOKENS * TL::ROW;
-    const unsigned live = __ballot_sync(0xffffffffu, (live_ring >> (i % STAGES)) & 1u);
+    const uint32_t base = pipe + stage * TL::STAGE, vbase = base + TL::BOXES * TL::BOX, sbase = scales + stage * 2 * TL::TOKENS * 4;
+    const unsigned live = __ballot_sync(0xffffffffu, (live_ring >> stage) & 1u);
+    if (TMA && !EIGHT && live != 0xffffffffu) {
+      // a page's rows that are not this sequence's tokens: a weight of 0 does not keep an infinity or a NaN out of the sum
+      if (!((live >> lane) & 1u) && lane < TL::TOKENS) {
+#pragma unroll
+        for (int b = 0; b < TL::BOXES; b++)
+#pragma unroll
+          for (int c = 0; c < 8; c++) sm100::sts128(vbase + b * TL::BOX + lane * 128 + c * 16, 0, 0, 0, 0);
+      }
+      sm100::fence_proxy_async();
+      __syncwarp();
+    }
 
     // S^T: tokens 16 mt + {g, g + 8} x heads 8 nt + {2t, 2t + 1}
     float s[MT][NT][4];
@@ -267,11 +329,11 @@ __global__ void __launch_bounds__(WARPS * 32) attn_decode_kernel(const DecodePro
       for (int ks = 0; ks < KS; ks++) {
         unsigned a[4];
         if (EIGHT) {
-          const unsigned w0 = lds32(base + (mt * 16 + g) * TL::ROW + ks * 16 + 4 * t) ^ 0x80808080u;
-          const unsigned w1 = lds32(base + (mt * 16 + 8 + g) * TL::ROW + ks * 16 + 4 * t) ^ 0x80808080u;
+          const unsigned w0 = lds32(base + TL::at(mt * 16 + g, ks) + 4 * t) ^ 0x80808080u;
+          const unsigned w1 = lds32(base + TL::at(mt * 16 + 8 + g, ks) + 4 * t) ^ 0x80808080u;
           a[0] = widen(w0, 0x4140); a[1] = widen(w1, 0x4140); a[2] = widen(w0, 0x4342); a[3] = widen(w1, 0x4342);
         } else {
-          ldmatrix4(base + (mt * 16 + (lane & 15)) * TL::ROW + ks * 32 + (lane >> 4) * 16, a);
+          ldmatrix4(base + TL::at(mt * 16 + (lane & 15), ks * 2 + (lane >> 4)), a);
         }
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) mma<T>(s[mt][nt], a, qf[nt][ks][0], qf[nt][ks][1]);
@@ -288,7 +350,7 @@ __global__ void __launch_bounds__(WARPS * 32) attn_decode_kernel(const DecodePro
         float ks_ = 1.f;
         if (EIGHT) {
           ks_ = __uint_as_float(lds32(sbase + token * 4));
-          vs[mt][r] = __uint_as_float(lds32(sbase + (32 + token) * 4));
+          vs[mt][r] = __uint_as_float(lds32(sbase + (TL::TOKENS + token) * 4));
           lvs[mt][r] = __log2f(fabsf(vs[mt][r]));
         }
 #pragma unroll
@@ -341,8 +403,7 @@ __global__ void __launch_bounds__(WARPS * 32) attn_decode_kernel(const DecodePro
             const float x = s[mt][nt][2 * r + c], e = ex2(x - m[nt][c]);
             l[nt][c] += e;
             // rounded to 16 bits for the product with V: off by 2^-8 (bf16) or 2^-11 (fp16) at most; the sum l takes it unrounded
-            w[c] = EIGHT ? (vs[mt][r] == vs[mt][r] ? ex2(x + lvs[mt][r] - ref[nt][c]) : vs[mt][r]) : e;
-            if (EIGHT && vs[mt][r] < 0.f) w[c] = -w[c];
+            w[c] = EIGHT ? __uint_as_float(__float_as_uint(ex2(x + lvs[mt][r] - ref[nt][c])) ^ (__float_as_uint(vs[mt][r]) & 0x80000000u)) : e;
           }
           b[nt][r] = transpose8(pack2<T>(w[0], w[1]));
         }
@@ -350,9 +411,10 @@ __global__ void __launch_bounds__(WARPS * 32) attn_decode_kernel(const DecodePro
       if (EIGHT) {
 #pragma unroll
         for (int blk = 0; blk < DP / 32; blk++) {
-          const uint32_t v = vbase + (mt * 16 + 2 * t) * TL::ROW + blk * 32 + 4 * g;
-          const unsigned w0 = lds32(v) ^ 0x80808080u, w1 = lds32(v + TL::ROW) ^ 0x80808080u;
-          const unsigned w2 = lds32(v + 8 * TL::ROW) ^ 0x80808080u, w3 = lds32(v + 9 * TL::ROW) ^ 0x80808080u;
+          const uint32_t v = vbase + TL::at(mt * 16 + 2 * t, blk * 2 + (g >> 2)) + 4 * (g & 3);
+          const uint32_t u = vbase + TL::at(mt * 16 + 2 * t + 1, blk * 2 + (g >> 2)) + 4 * (g & 3);
+          const unsigned w0 = lds32(v) ^ 0x80808080u, w1 = lds32(u) ^ 0x80808080u;
+          const unsigned w2 = lds32(v + 8 * 128) ^ 0x80808080u, w3 = lds32(u + 8 * 128) ^ 0x80808080u;
           const unsigned x0 = __byte_perm(w0, w1, 0x5140), x1 = __byte_perm(w0, w1, 0x7362);
           const unsigned y0 = __byte_perm(w2, w3, 0x5140), y1 = __byte_perm(w2, w3, 0x7362);
           const unsigned a0[4] = {widen(x0, 0x4140), widen(x0, 0x4342), widen(y0, 0x4140), widen(y0, 0x4342)};
@@ -368,7 +430,7 @@ __global__ void __launch_bounds__(WARPS * 32) attn_decode_kernel(const DecodePro
         for (int ks = 0; ks < KS; ks++) {
           unsigned a[4];
           // matrices: (tokens 0-7, channels 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15), each transposed
-          ldmatrix4_trans(vbase + (mt * 16 + (lane & 7) + (lane >> 4) * 8) * TL::ROW + ks * 32 + ((lane >> 3) & 1) * 16, a);
+          ldmatrix4_trans(vbase + TL::at(mt * 16 + (lane & 7) + (lane >> 4) * 8, ks * 2 + ((lane >> 3) & 1)), a);
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) mma<T>(o[nt][ks], a, b[nt][0], b[nt][1]);
         }
@@ -377,6 +439,10 @@ __global__ void __launch_bounds__(WARPS * 32) attn_decode_kernel(const DecodePro
     __syncwarp();          // the buffer is free for the fetch of the next turn
   }
   cp_wait<0>();
+  if (TMA && !landed) {      // given up: what is in flight must land before its memory is used for something else
+    volatile int never = 0;
+    for (int i = max(0, mine - STAGES); i < mine; i++) sm100::mbar_wait(&full[warp][i % STAGES], (i / STAGES) & 1, &never, nullptr, 0);
+  }
 
   // ---- join: warps, then CTAs of the cluster -----------------------------------------------------
   __syncthreads();         // the pipeline's memory is free
@@ -451,34 +517,59 @@ __global__ void __launch_bounds__(WARPS * 32) attn_decode_kernel(const DecodePro
   cluster.sync();          // no CTA leaves while another reads its sums
 }
 
-template <typename T, int DP, int NT, bool EIGHT>
-bool decode_go(Context &c, const DecodeProblem &p, int64_t pairs)
+// [n_pages][n_heads][page_size][dim] at the cache's strides, boxes of 128 bytes of `box` slots of one head, 128-byte swizzle
+bool make_cache_map(CUtensorMap *map, const pulpnn_kv_cache_t &c, const void *base, int box)
 {
-  constexpr int smem = decode_smem<DP, NT, EIGHT>();
-  auto k = attn_decode_kernel<T, DP, NT, EIGHT>;
+  sm100::EncodeTiledFn enc = sm100::encode_tiled_fn();
+  if (!enc) { set_error(PULPNN_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver"); return false; }
+  const bool eight = c.type == PULPNN_TYPE_S8;
+  const int size = eight ? 1 : 2;
+  const cuuint64_t any = (cuuint64_t)c.head_dim * size;       // the stride of an axis of one element does not matter
+  const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.page_size, (cuuint64_t)c.n_heads, (cuuint64_t)c.n_pages};
+  const cuuint64_t strides[3] = {c.page_size > 1 ? (cuuint64_t)c.slot_stride * size : any, c.n_heads > 1 ? (cuuint64_t)c.head_stride * size : any,
+                                 c.n_pages > 1 ? (cuuint64_t)c.page_stride * size : any};
+  const cuuint32_t boxes[4] = {(cuuint32_t)(eight ? 128 : 64), (cuuint32_t)box, 1, 1}, step[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, eight ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, strides,
+                         boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { set_error(PULPNN_ERR_CUDA, "cuTensorMapEncodeTiled (cache) failed with code %d", (int)r); return false; }
+  return true;
+}
+
+struct DecodeLaunch { const DecodeProblem &p; const CUtensorMap &k, &v; int64_t pairs; bool tma; };
+
+template <typename T, int DP, int NT, bool EIGHT, bool TMA>
+bool decode_go(Context &c, const DecodeLaunch &d)
+{
+  constexpr int smem = Smem<DP, NT, EIGHT>::BYTES;
+  auto k = attn_decode_kernel<T, DP, NT, EIGHT, TMA>;
   static PerDeviceInt ready;
   if (!ready.get(c.device)) {
     if (!cuda_ok(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute(attn_decode)")) return false;
     ready.set(c.device, 1);
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(pairs * p.splits)); cfg.blockDim = dim3(WARPS * 32); cfg.dynamicSmemBytes = smem; cfg.stream = c.stream;
+  cfg.gridDim = dim3((unsigned)(d.pairs * d.p.splits)); cfg.blockDim = dim3(WARPS * 32); cfg.dynamicSmemBytes = smem; cfg.stream = c.stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)p.splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  attr[1].val.clusterDim.x = (unsigned)d.p.splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr; cfg.numAttrs = 2;
-  if (!cuda_ok(cudaLaunchKernelEx(&cfg, k, p), "pulpnn_attn_decode")) return false;
+  if (!cuda_ok(cudaLaunchKernelEx(&cfg, k, d.k, d.v, d.p), "pulpnn_attn_decode")) return false;
   count_launch("attn_decode_kernel");
   return true;
 }
-template <typename T, bool EIGHT>
-bool decode_dim(Context &c, const DecodeProblem &p, int64_t pairs, bool two)
+template <typename T, int DP, bool EIGHT>
+bool decode_tiles(Context &c, const DecodeLaunch &d)
 {
-  if (p.dim <= 64) return two ? decode_go<T, 64, 2, EIGHT>(c, p, pairs) : decode_go<T, 64, 1, EIGHT>(c, p, pairs);
-  if (p.dim <= 96) return two ? decode_go<T, 96, 2, EIGHT>(c, p, pairs) : decode_go<T, 96, 1, EIGHT>(c, p, pairs);
-  return two ? decode_go<T, 128, 2, EIGHT>(c, p, pairs) : decode_go<T, 128, 1, EIGHT>(c, p, pairs);
+  if (d.p.group > 8) return d.tma ? decode_go<T, DP, 2, EIGHT, true>(c, d) : decode_go<T, DP, 2, EIGHT, false>(c, d);
+  return d.tma ? decode_go<T, DP, 1, EIGHT, true>(c, d) : decode_go<T, DP, 1, EIGHT, false>(c, d);
+}
+template <typename T, bool EIGHT>
+bool decode_dim(Context &c, const DecodeLaunch &d)
+{
+  return d.p.dim <= 64 ? decode_tiles<T, 64, EIGHT>(c, d) : (d.p.dim <= 96 ? decode_tiles<T, 96, EIGHT>(c, d) : decode_tiles<T, 128, EIGHT>(c, d));
 }
 
 }  // namespace
@@ -523,18 +614,31 @@ extern "C" int pulpnn_attn_decode(const pulpnn_kv_cache_t *cache, const pulpnn_a
   p.q_type = a->q_type; p.out_type = a->out_type;
   p.scale_log2 = a->scale * 1.4426950408889634074f;
   p.out_inv_step = a->out_type == PULPNN_TYPE_U8 ? 1.f / a->out_step : 1.f; p.out_zero = a->out_zero;
-  const bool two = p.group > 8;
+  const bool two = p.group > 8, eight = cache->type == PULPNN_TYPE_S8;
   p.head_tiles = (p.group + (two ? 15 : 7)) / (two ? 16 : 8);
   const int64_t pairs = (int64_t)a->n_seqs * cache->n_heads * p.head_tiles;
   ATTN_REQUIRE(pairs <= 0x0fffffff, PULPNN_ERR_UNSUPPORTED, "%s: %d sequences of %d heads", who, a->n_seqs, a->n_heads);
-  // CTAs of a sequence: no more than leave each warp two tiles of the longest one
+  // CTAs of a sequence: as long as there are fewer than four for each that fits the GPU at a time, but no more than leave each
+  // warp two tiles of the longest sequence
   int64_t most = (int64_t)a->max_pages * cache->page_size;
   if (a->window > 0 && a->window < most) most = a->window;
-  const int tile = cache->type == PULPNN_TYPE_S8 ? 32 : 16;
+  const int tile = eight || p.dim <= 64 ? 32 : 16;
   p.splits = 1;
-  while (p.splits < 8 && most > (int64_t)p.splits * WARPS * tile * 2 && pairs * p.splits < 8 * 2 * c.sm_count) p.splits *= 2;
+  while (p.splits < 8 && most > (int64_t)p.splits * WARPS * tile * 2 && pairs * p.splits < 4 * 2 * c.sm_count) p.splits *= 2;
   if (c.opt_split_k > 0) p.splits = c.opt_split_k >= 8 ? 8 : (c.opt_split_k >= 4 ? 4 : (c.opt_split_k >= 2 ? 2 : 1));
-  const bool ok = cache->type == PULPNN_TYPE_S8 ? decode_dim<__half, true>(c, p, pairs, two)
-                  : (a->q_type == PULPNN_TYPE_F16 ? decode_dim<__half, false>(c, p, pairs, two) : decode_dim<__nv_bfloat16, false>(c, p, pairs, two));
+  // pages that hold whole runs of 16 tokens come by TMA, whose maps want positive strides below 2^40 bytes
+  auto fits = [&](int n, int64_t s) { return n == 1 || (s > 0 && s < (int64_t)1 << 38); };
+  const bool tma = cache->page_size % 16 == 0 && fits(cache->page_size, cache->slot_stride) && fits(cache->n_heads, cache->head_stride) &&
+                   fits(cache->n_pages, cache->page_stride);
+  p.box = tile == 32 && cache->page_size % 32 == 0 && p.window == 0 ? 32 : 16;
+  CUtensorMap mk, mv;
+  p.status = nullptr;
+  if (tma) {
+    if (!ctx_status_word_unless_capturing(c, &p.status)) return c.err;
+    if (!make_cache_map(&mk, *cache, cache->k, p.box) || !make_cache_map(&mv, *cache, cache->v, p.box)) return c.err;
+  }
+  const DecodeLaunch d = {p, mk, mv, pairs, tma};
+  const bool ok = eight ? decode_dim<__half, true>(c, d)
+                        : (a->q_type == PULPNN_TYPE_F16 ? decode_dim<__half, false>(c, d) : decode_dim<__nv_bfloat16, false>(c, d));
   return ok ? PULPNN_OK : c.err;
 }
