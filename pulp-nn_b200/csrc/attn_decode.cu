@@ -14,8 +14,11 @@
 // there is no barrier between warps until the end. Each lane looks up the page of one token, one tile ahead of its
 // fetch. Where pages are a multiple of 16 slots, every 16 tokens lie in one page and come by one TMA copy for each 128 bytes of
 // their rows: copies of 16 bytes with a page each cost as many instructions as all the arithmetic. Pages of any
-// other size are fetched with these (16-byte cp.async), tokens behind the end without being read. WARPS warps are a CTA, CTAs of a cluster share a sequence, and the partial results are joined
-// through (distributed) shared memory in a fixed order: no workspace, no atomics, the same result every time.
+// other size are fetched with these (16-byte cp.async), tokens behind the end without being read. WARPS warps are a CTA, up to eight CTAs of a cluster share a sequence, and the partial results are joined through
+// (distributed) shared memory. Where clusters of eight are too few to fill the GPU, several share a sequence and leave
+// their sums in memory for attn_join_kernel: memory from a pool, allocated and freed in the stream's order, so that calls
+// on other streams and replays of other graphs have their own. Every join goes in a fixed order, without atomics: the
+// same result every time.
 //
 // Running maximum: the reference m only has to be near the true maximum, not equal to it. It is raised (and the sums
 // rescaled) when some score is more than 2^LAG above it, which one vote per tile finds out; the weights stay
@@ -36,10 +39,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-#ifndef DEC_STAGES
-#define DEC_STAGES 3
-#endif
-constexpr int WARPS = 4, STAGES = DEC_STAGES;
+// Two stages of 8 KB a warp and three CTAs an SM: twelve warps keep 96 KB under way and two thirds of the issue slots busy where
+// the cache holds 8 bits. Three stages and two CTAs: 171 instead of 165 us for 64 ragged sequences of up to 8192 tokens in
+// 16 bits, 189 instead of 151 for 200 of 80 channels.
+constexpr int WARPS = 4, STAGES = 2, MOST_SPLITS = 8;
 constexpr float LAG = 8.f, NOTHING = -1e30f;
 
 struct DecodeProblem {
@@ -52,7 +55,8 @@ struct DecodeProblem {
   CacheView cache;
   int hq, group, head_tiles, dim, max_pages, window, q_type, out_type;
   float scale_log2, out_inv_step;
-  int out_zero, splits;
+  int out_zero, splits, parts;                   // CTAs of a cluster, clusters of a sequence
+  float *sums;                                   // parts > 1: [pair][part][Partial]
   int box;                                       // tokens of a TMA copy: 16 or a whole tile
   int *status;
 };
@@ -139,6 +143,40 @@ template <int DP, int NT, bool EIGHT> struct Smem {
   static constexpr int BYTES = PIPE + Tile<DP, EIGHT>::SCALES + 1024;
 };
 
+// what a cluster leaves behind: sums [8 NT heads][MAX_HEAD_DIM], and m, l and the sums' reference of each head
+__host__ __device__ constexpr int partial_floats(int nt) { return nt * 8 * (MAX_HEAD_DIM + 4); }
+
+// A block for each head and sequence: joins the parts, a channel a thread.
+template <int NT>
+__global__ void __launch_bounds__(MAX_HEAD_DIM) attn_join_kernel(const DecodeProblem p)
+{
+  pdl_wait();
+  const int pair = blockIdx.x, head = blockIdx.y, ch = threadIdx.x;
+  const int ht = pair % p.head_tiles, kvh = pair / p.head_tiles % p.cache.n_heads, seq = pair / p.head_tiles / p.cache.n_heads;
+  if (head >= min(NT * 8, p.group - ht * NT * 8)) return;
+  const float *sums = p.sums + (int64_t)pair * p.parts * partial_floats(NT);
+  float M = NOTHING, R = NOTHING, L = 0.f, acc = 0.f;
+  for (int i = 0; i < p.parts; i++) {
+    const float *st = sums + i * partial_floats(NT) + NT * 8 * MAX_HEAD_DIM;
+    M = fmaxf(M, st[head]);
+    R = fmaxf(R, st[2 * NT * 8 + head]);
+  }
+  for (int i = 0; i < p.parts; i++) {
+    const float *st = sums + i * partial_floats(NT) + NT * 8 * MAX_HEAD_DIM;
+    L += st[NT * 8 + head] * ex2(st[head] - M);
+    if (ch < p.dim) acc += sums[i * partial_floats(NT) + head * MAX_HEAD_DIM + ch] * ex2(st[2 * NT * 8 + head] - R);
+  }
+  const float y = L == 0.f ? 0.f : acc * (ex2(R - M) / L);
+  const int h = kvh * p.group + ht * NT * 8 + head;
+  char *dst = p.out + seq * p.out_seq + (int64_t)h * p.out_head;
+  if (ch < p.dim) {
+    if (p.out_type == PULPNN_TYPE_U8) dst[ch] = (char)to_u8(y, p.out_inv_step, p.out_zero);
+    else if (p.out_type == PULPNN_TYPE_F16) reinterpret_cast<__half *>(dst)[ch] = __float2half_rn(y);
+    else reinterpret_cast<__nv_bfloat16 *>(dst)[ch] = __float2bfloat16_rn(y);
+  }
+  if (p.lse && ch == 0) p.lse[(int64_t)seq * p.hq + h] = (M + log2f(L)) * 0.69314718055994530942f;
+}
+
 template <typename T, int DP, int NT, bool EIGHT, bool TMA>
 __global__ void __launch_bounds__(WARPS * 32)
 attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const DecodeProblem p)
@@ -154,6 +192,8 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = blockIdx.x % p.splits;
   int rest = blockIdx.x / p.splits;
+  const int cluster_id = rest, part = rest % p.parts;
+  rest /= p.parts;
   const int ht = rest % p.head_tiles; rest /= p.head_tiles;
   const int kvh = rest % p.cache.n_heads, seq = rest / p.cache.n_heads;
   const int h0 = kvh * p.group + ht * NT * 8, heads = min(NT * 8, p.group - ht * NT * 8);
@@ -173,7 +213,8 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   const int n = min(max(__ldg(p.lens + seq), 0), p.max_pages * p.cache.page_size);
   const int first = p.window > 0 ? max(0, n - p.window) : 0, origin = TMA ? first & ~15 : first;      // of the tiles
   const int tiles = (n - origin + TL::TOKENS - 1) / TL::TOKENS;
-  const int lo = (int)((int64_t)tiles * rank / p.splits), hi = (int)((int64_t)tiles * (rank + 1) / p.splits);
+  const int share = part * p.splits + rank, shares = p.parts * p.splits;
+  const int lo = (int)((int64_t)tiles * share / shares), hi = (int)((int64_t)tiles * (share + 1) / shares);
   const int mine = hi - lo > warp ? (hi - lo - warp + WARPS - 1) / WARPS : 0;       // tiles lo + warp + i * WARPS
 
   char *pipe_at = smem + warp * STAGES * TL::STAGE;
@@ -508,6 +549,13 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       const float4 x = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(cta_sums, r) + head * JN::PITCH + ch);
       acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
     }
+    if (p.parts > 1) {
+      float *dst = p.sums + (int64_t)cluster_id * partial_floats(NT);
+      *reinterpret_cast<float4 *>(dst + head * MAX_HEAD_DIM + ch) = acc;
+      dst += NT * 8 * MAX_HEAD_DIM;
+      if (ch == 0) { dst[head] = M; dst[NT * 8 + head] = L; dst[2 * NT * 8 + head] = R; }
+      continue;
+    }
     const float f = L == 0.f ? 0.f : (EIGHT ? ex2(R - M) : 1.f) / L;      // a row that sees nothing is zero
     const float y[4] = {acc.x * f, acc.y * f, acc.z * f, acc.w * f};
     char *dst = p.out + seq * p.out_seq + (int64_t)(h0 + head) * p.out_head;
@@ -536,29 +584,63 @@ bool make_cache_map(CUtensorMap *map, const pulpnn_kv_cache_t &c, const void *ba
   return true;
 }
 
-struct DecodeLaunch { const DecodeProblem &p; const CUtensorMap &k, &v; int64_t pairs; bool tma; };
+struct DecodeLaunch { DecodeProblem &p; const CUtensorMap &k, &v; int64_t pairs, longest; int tile; bool tma; };
+
+// CTAs of a cluster and clusters of a sequence. `slots` CTAs run at a time; `tiles` are a warp's of the longest sequence with one
+// CTA. A sequence's time falls with its CTAs and a round of CTAs costs some tiles' time of its own (its first loads and the join:
+// 4 us, where a tile of 8 KB takes a slot 0.5 us, memory being shared by all): the number with the least rounds x (share of
+// the sequence + 8 tiles), as if all sequences were as long as the longest.
+void choose_splits(const Context &c, DecodeProblem &p, int64_t pairs, int slots, int64_t longest, int tile)
+{
+  const int64_t tiles = (longest + WARPS * tile - 1) / (WARPS * tile);
+  auto cost = [&](int64_t shares) { return ((pairs * shares + slots - 1) / slots) * ((tiles + shares - 1) / shares + 8); };
+  p.splits = 1; p.parts = 1;
+  for (int s = 2; s <= MOST_SPLITS; s++)
+    if (cost(s) < cost(p.splits)) p.splits = s;
+  // more than a cluster: only where these are too few to fill the GPU, and each warp still has 8 tiles (a second kernel costs 3 us)
+  if (p.splits == MOST_SPLITS)
+    while (pairs * MOST_SPLITS * (p.parts + 1) <= slots && tiles >= (int64_t)MOST_SPLITS * (p.parts + 1) * 8) p.parts++;
+  if (c.opt_split_k > 0) {
+    p.splits = c.opt_split_k < MOST_SPLITS ? c.opt_split_k : MOST_SPLITS;
+    p.parts = c.opt_split_k < 2 * MOST_SPLITS ? 1 : (c.opt_split_k < 512 ? c.opt_split_k / MOST_SPLITS : 64);
+  }
+}
 
 template <typename T, int DP, int NT, bool EIGHT, bool TMA>
 bool decode_go(Context &c, const DecodeLaunch &d)
 {
   constexpr int smem = Smem<DP, NT, EIGHT>::BYTES;
   auto k = attn_decode_kernel<T, DP, NT, EIGHT, TMA>;
-  static PerDeviceInt ready;
-  if (!ready.get(c.device)) {
+  static PerDeviceInt resident;
+  if (!resident.get(c.device)) {
     if (!cuda_ok(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute(attn_decode)")) return false;
-    ready.set(c.device, 1);
+    int n = 0;
+    if (!cuda_ok(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, WARPS * 32, smem), "occupancy(attn_decode)")) return false;
+    resident.set(c.device, n < 1 ? 1 : n);
+  }
+  choose_splits(c, d.p, d.pairs, resident.get(c.device) * c.sm_count, d.longest, d.tile);
+  if (d.p.parts > 1) {
+    d.p.sums = static_cast<float *>(ctx_stream_alloc(c, (size_t)(d.pairs * d.p.parts) * partial_floats(NT) * 4));
+    if (!d.p.sums) d.p.parts = 1;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(d.pairs * d.p.splits)); cfg.blockDim = dim3(WARPS * 32); cfg.dynamicSmemBytes = smem; cfg.stream = c.stream;
+  cfg.gridDim = dim3((unsigned)(d.pairs * d.p.parts * d.p.splits)); cfg.blockDim = dim3(WARPS * 32); cfg.dynamicSmemBytes = smem; cfg.stream = c.stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = (unsigned)d.p.splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr; cfg.numAttrs = 2;
-  if (!cuda_ok(cudaLaunchKernelEx(&cfg, k, d.k, d.v, d.p), "pulpnn_attn_decode")) return false;
-  count_launch("attn_decode_kernel");
-  return true;
+  bool ok = cuda_ok(cudaLaunchKernelEx(&cfg, k, d.k, d.v, d.p), "pulpnn_attn_decode");
+  if (ok) count_launch("attn_decode_kernel");
+  if (d.p.parts > 1) {
+    if (ok) {
+      ok = cuda_ok(launch_pdl(attn_join_kernel<NT>, dim3((unsigned)d.pairs, NT * 8), dim3(MAX_HEAD_DIM), 0, c.stream, d.p), "pulpnn_attn_decode (join)");
+      if (ok) count_launch("attn_join_kernel");
+    }
+    ctx_stream_free(c, d.p.sums);
+  }
+  return ok;
 }
 template <typename T, int DP, bool EIGHT>
 bool decode_tiles(Context &c, const DecodeLaunch &d)
@@ -618,26 +700,21 @@ extern "C" int pulpnn_attn_decode(const pulpnn_kv_cache_t *cache, const pulpnn_a
   p.head_tiles = (p.group + (two ? 15 : 7)) / (two ? 16 : 8);
   const int64_t pairs = (int64_t)a->n_seqs * cache->n_heads * p.head_tiles;
   ATTN_REQUIRE(pairs <= 0x0fffffff, PULPNN_ERR_UNSUPPORTED, "%s: %d sequences of %d heads", who, a->n_seqs, a->n_heads);
-  // CTAs of a sequence: as long as there are fewer than four for each that fits the GPU at a time, but no more than leave each
-  // warp two tiles of the longest sequence
-  int64_t most = (int64_t)a->max_pages * cache->page_size;
-  if (a->window > 0 && a->window < most) most = a->window;
+  int64_t longest = (int64_t)a->max_pages * cache->page_size;
+  if (a->window > 0 && a->window < longest) longest = a->window;
   const int tile = eight || p.dim <= 64 ? 32 : 16;
-  p.splits = 1;
-  while (p.splits < 8 && most > (int64_t)p.splits * WARPS * tile * 2 && pairs * p.splits < 4 * 2 * c.sm_count) p.splits *= 2;
-  if (c.opt_split_k > 0) p.splits = c.opt_split_k >= 8 ? 8 : (c.opt_split_k >= 4 ? 4 : (c.opt_split_k >= 2 ? 2 : 1));
   // pages that hold whole runs of 16 tokens come by TMA, whose maps want positive strides below 2^40 bytes
   auto fits = [&](int n, int64_t s) { return n == 1 || (s > 0 && s < (int64_t)1 << 38); };
   const bool tma = cache->page_size % 16 == 0 && fits(cache->page_size, cache->slot_stride) && fits(cache->n_heads, cache->head_stride) &&
                    fits(cache->n_pages, cache->page_stride);
   p.box = tile == 32 && cache->page_size % 32 == 0 && p.window == 0 ? 32 : 16;
   CUtensorMap mk, mv;
-  p.status = nullptr;
+  p.status = nullptr; p.sums = nullptr;
   if (tma) {
     if (!ctx_status_word_unless_capturing(c, &p.status)) return c.err;
     if (!make_cache_map(&mk, *cache, cache->k, p.box) || !make_cache_map(&mv, *cache, cache->v, p.box)) return c.err;
   }
-  const DecodeLaunch d = {p, mk, mv, pairs, tma};
+  const DecodeLaunch d = {p, mk, mv, pairs, longest, tile, tma};
   const bool ok = eight ? decode_dim<__half, true>(c, d)
                         : (a->q_type == PULPNN_TYPE_F16 ? decode_dim<__half, false>(c, d) : decode_dim<__nv_bfloat16, false>(c, d));
   return ok ? PULPNN_OK : c.err;

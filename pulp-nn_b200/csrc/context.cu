@@ -3,6 +3,7 @@
 #include <cstdio>
 #include <cstring>
 #include <atomic>
+#include <mutex>
 #include <new>
 
 #include "internal.cuh"
@@ -148,6 +149,40 @@ bool ctx_partials_done(Context &c)
 {
   return cuda_ok(cudaEventRecord(c.partials.done, c.stream), "cudaEventRecord(partial sums)");
 }
+
+// A pool of the library's own for each device, which keeps what it has (the default pool gives memory back whenever the
+// host waits). It lives as long as the process.
+static cudaMemPool_t stream_pool(int device)
+{
+  static std::mutex lock;
+  static cudaMemPool_t pools[MAX_DEVICES] = {};
+  if (device < 0 || device >= MAX_DEVICES) return nullptr;
+  std::lock_guard<std::mutex> guard(lock);
+  if (!pools[device]) {
+    RelaxedCapture relaxed;
+    cudaMemPoolProps props = {};
+    props.allocType = cudaMemAllocationTypePinned;
+    props.location.type = cudaMemLocationTypeDevice;
+    props.location.id = device;
+    cudaMemPool_t pool;
+    if (cudaMemPoolCreate(&pool, &props) != cudaSuccess) { cudaGetLastError(); return nullptr; }
+    uint64_t keep = ~0ull;
+    if (cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep) != cudaSuccess) cudaGetLastError();
+    pools[device] = pool;
+  }
+  return pools[device];
+}
+
+void *ctx_stream_alloc(Context &c, size_t bytes)
+{
+  cudaMemPool_t pool = stream_pool(c.device);
+  void *p = nullptr;
+  if (!pool) return nullptr;
+  if (cudaMallocFromPoolAsync(&p, bytes, pool, c.stream) != cudaSuccess) { cudaGetLastError(); return nullptr; }
+  return p;
+}
+
+void ctx_stream_free(Context &c, void *p) { cuda_ok(cudaFreeAsync(p, c.stream), "cudaFreeAsync"); }
 
 // device word that kernels with bounded waits report into (read by pulpnn_device_status)
 int *ctx_status_word(Context &c)

@@ -245,6 +245,10 @@ void *ctx_scratch(Context &c, size_t bytes);    // grow-only device scratch, nul
 // no error, under a stream capture and where there is none to be had. ctx_partials_done() after the last kernel that reads them.
 void *ctx_partials(Context &c, size_t bytes);
 bool ctx_partials_done(Context &c);
+// Memory that belongs to the work enqueued on the context's stream between the two calls (in a capture: to the graph); nullptr, and
+// no error, where there is none to be had.
+void *ctx_stream_alloc(Context &c, size_t bytes);
+void ctx_stream_free(Context &c, void *p);
 
 // A per-kernel setting that belongs to a device (cudaFuncSetAttribute, an occupancy figure) is
 // cached per device, not per process or per thread: one process may drive several GPUs, from one
