@@ -50,6 +50,7 @@ struct PromptProblem {
   float *lse;
   const int *cu_q, *cu_k;
   int64_t v_row, v_head, out_row, out_head;       // bytes
+  FastDiv by_group;
   int nq, nk, seqs, hq, group, dim, causal, window, out_type, out_zero;
   float scale_log2, out_inv_step;
   int *status;
@@ -63,7 +64,8 @@ template <int DP> struct Shape {
   static constexpr bool APART = DP == 64;
   static constexpr int O_AT = 256, P_AT = APART ? 256 + 2 * DP : 0, P_STEP = APART ? 64 : 128;
   static constexpr int STAGES = DP == 128 ? 4 : 8;             // even: keys in the even stages, values in the odd ones
-  static constexpr int SMEM = (2 + STAGES) * TILE + 1024 /* barriers */ + 1024 /* alignment */;
+  static constexpr int STAGING = 32 * 128;                     // of a softmax warp: 32 rows of 64 channels on their way out
+  static constexpr int SMEM = (2 + STAGES) * TILE + 1024 /* barriers */ + 8 * STAGING + 1024 /* alignment */;
 };
 
 // A tile of queries: rows row0 .. row0 + rows - 1 of head `head`, the first at position pos; it sees the key tiles lo .. hi - 1.
@@ -173,7 +175,7 @@ __device__ __forceinline__ void make_work(Work &w, int q0, int lq, int k0, int l
   w.q0 = q0; w.k0 = k0; w.lk = lk; w.kvh = kvh;
   w.lo = 0x7fffffff; w.hi = 0;
   for (int x = 0; x < 2; x++) {
-    const int n = 2 * pair + x, rt = n / p.group;
+    const int n = 2 * pair + x, rt = p.by_group.div(n);
     Unit u;
     u.row0 = rt * BQ; u.head = kvh * p.group + n - rt * p.group;
     u.rows = min(max(lq - u.row0, 0), BQ);
@@ -204,10 +206,13 @@ __device__ __forceinline__ bool guarded(const Work &w, int j, const PromptProble
 __device__ __forceinline__ bool find_item(const PromptProblem &p, int x, int y, int lane, int &s0, int &before, Item &it)
 {
   for (; s0 < p.seqs; s0 += 256) {              // eight sequences a lane
-    int at[9], count[8], sum = 0;
+    int at[9], at_k[9], count[8], sum = 0;
     const int b0 = s0 + lane * 8;
 #pragma unroll
-    for (int k = 0; k < 9; k++) at[k] = b0 + k <= p.seqs ? min(max(__ldg(p.cu_q + b0 + k), 0), p.nq) : 0;
+    for (int k = 0; k < 9; k++) {
+      at[k] = b0 + k <= p.seqs ? min(max(__ldg(p.cu_q + b0 + k), 0), p.nq) : 0;
+      at_k[k] = b0 + k <= p.seqs ? min(max(__ldg(p.cu_k + b0 + k), 0), p.nk) : 0;
+    }
 #pragma unroll
     for (int k = 0; k < 8; k++) {
       const int tiles = b0 + k < p.seqs ? (max(at[k + 1] - at[k], 0) + BQ - 1) / BQ : 0;
@@ -220,23 +225,19 @@ __device__ __forceinline__ bool find_item(const PromptProblem &p, int x, int y, 
       const int v = __shfl_up_sync(0xffffffffu, incl, d);
       if (lane >= d) incl += v;
     }
-    int off = before + incl - sum, which = -1, q0 = 0, lq = 0, pair = 0;
+    int off = before + incl - sum, q0 = 0, lq = 0, k0 = 0, lk = 0, pair = -1;
 #pragma unroll
     for (int k = 0; k < 8; k++) {
       if (x >= off && x < off + count[k]) {
-        which = b0 + k;
         // the last rows of a causal sequence see the most keys: they begin first
-        q0 = at[k]; lq = at[k + 1] - at[k]; pair = count[k] - 1 - (x - off);
+        q0 = at[k]; lq = at[k + 1] - at[k]; k0 = at_k[k]; lk = max(at_k[k + 1] - at_k[k], 0); pair = count[k] - 1 - (x - off);
       }
       off += count[k];
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, which >= 0);
+    const unsigned hit = __ballot_sync(0xffffffffu, pair >= 0);
     if (hit) {
-      const int src = __ffs(hit) - 1;
-      which = __shfl_sync(0xffffffffu, which, src);
-      q0 = __shfl_sync(0xffffffffu, q0, src); lq = __shfl_sync(0xffffffffu, lq, src); pair = __shfl_sync(0xffffffffu, pair, src);
-      const int k0 = min(max(__ldg(p.cu_k + which), 0), p.nk), lk = min(max(__ldg(p.cu_k + which + 1), k0), p.nk) - k0;
-      if (lane == 0) make_work(it.w, q0, lq, k0, lk, pair, y, p);
+      if (lane == __ffs(hit) - 1) make_work(it.w, q0, lq, k0, lk, pair, y, p);
+      __syncwarp();
       return true;
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
@@ -491,7 +492,7 @@ __device__ __forceinline__ float max3(float a, float b, float c)
 }
 // Warps 0 to 7: the softmax of a unit, a row a thread.
 template <typename T, int DP>
-__device__ __forceinline__ void softmax_warps(Control &ct, uint32_t tmem, const PromptProblem &p)
+__device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uint32_t tmem, const PromptProblem &p)
 {
   using SH = Shape<DP>;
   volatile int *abort_flag = &ct.abort_flag;
@@ -629,6 +630,9 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t tmem, const 
     const float inv = l == 0.f ? 0.f : 1.f / l;         // a row that sees nothing is zero
     char *dst = p.out + row * p.out_row + (int64_t)w.head * p.out_head;
     const bool dirty = any && *reinterpret_cast<const volatile int *>(&it.dirty);
+    // 16-bit rows go through shared memory, 64 channels at a time, and leave as whole rows: stored by their own threads, each
+    // instruction would touch 32 rows (300 tokens of 32 heads: 4900 of 24000 cycles)
+    const uint32_t stage = staging + warp * SH::STAGING;
     for (int c = 0; c < groups; c++) {
       float y[16];
       if (any) {
@@ -656,13 +660,33 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t tmem, const 
           }
         }
       }
-      if (live) {
+      if (p.out_type == PULPNN_TYPE_U8) {
+        if (live) {
 #pragma unroll
-        for (int k = 0; k < 16; k += 4)
-          if (c * 16 + k < p.dim) {
-            const float z[4] = {y[k], y[k + 1], y[k + 2], y[k + 3]};
-            store4(dst, c * 16 + k, p.out_type, z, p.out_inv_step, p.out_zero);
-          }
+          for (int k = 0; k < 16; k += 4)
+            if (c * 16 + k < p.dim) {
+              const float z[4] = {y[k], y[k + 1], y[k + 2], y[k + 3]};
+              store4(dst, c * 16 + k, p.out_type, z, p.out_inv_step, p.out_zero);
+            }
+        }
+        continue;
+      }
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+        sts128(stage + lane * 128 + ((((c & 3) * 2 + k) ^ (lane & 7)) << 4), pack2<T>(y[8 * k], y[8 * k + 1]), pack2<T>(y[8 * k + 2], y[8 * k + 3]),
+               pack2<T>(y[8 * k + 4], y[8 * k + 5]), pack2<T>(y[8 * k + 6], y[8 * k + 7]));
+      if ((c & 3) == 3 || c == groups - 1) {
+        __syncwarp();
+        const int chunk = lane & 7, channel = (c & ~3) * 16 + chunk * 8;
+        char *to = p.out + ((int64_t)it.w.q0 + w.row0 + (warp & 3) * 32) * p.out_row + (int64_t)w.head * p.out_head + channel * 2;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          const int n = k * 4 + (lane >> 3);
+          uint4 v;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(stage + n * 128 + ((chunk ^ (n & 7)) << 4)) : "memory");
+          if ((warp & 3) * 32 + n < w.rows && channel < p.dim) *reinterpret_cast<uint4 *>(to + n * p.out_row) = v;
+        }
+        __syncwarp();
       }
     }
     if (live && p.lse) p.lse[row * p.hq + w.head] = (m + log2f(l)) * 0.69314718055994530942f;
@@ -753,7 +777,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    softmax_warps<T, DP>(ct, tmem, p);
+    softmax_warps<T, DP>(ct, base + (2 + ST) * SH::TILE + 1024, tmem, p);
   }
 
   __syncwarp();
@@ -838,7 +862,7 @@ extern "C" int pulpnn_attn_prompt(const pulpnn_attn_prompt_t *a)
   const int os = type_size(a->out_type);
   p.v = static_cast<const char *>(a->v); p.out = static_cast<char *>(a->out); p.lse = a->lse; p.cu_q = a->cu_q; p.cu_k = a->cu_k;
   p.v_row = a->v_stride[0] * 2; p.v_head = a->v_stride[1] * 2; p.out_row = a->out_stride[0] * os; p.out_head = a->out_stride[1] * os;
-  p.nq = a->n_q_rows; p.nk = a->n_k_rows; p.seqs = a->n_seqs; p.hq = a->n_heads; p.group = a->n_heads / a->n_kv_heads; p.dim = a->head_dim;
+  p.nq = a->n_q_rows; p.nk = a->n_k_rows; p.seqs = a->n_seqs; p.hq = a->n_heads; p.group = a->n_heads / a->n_kv_heads; p.by_group.set((unsigned)p.group); p.dim = a->head_dim;
   p.causal = a->causal != 0; p.out_type = a->out_type; p.out_zero = a->out_zero;
   p.window = a->window < 0x3fffffff ? a->window : 0x3fffffff;      // positions are below 2^30
   p.scale_log2 = a->scale * 1.4426950408889634074f;

@@ -32,7 +32,7 @@ int check_cache(const char *who, const pulpnn_kv_cache_t *c)
 namespace {
 
 constexpr int THREADS = 256;               // of a gather's block
-constexpr int WARPS = 4;                   // of an append's
+constexpr int WARPS = 4, MOST_TOKENS = 8;  // of an append's
 
 struct AppendProblem {
   const char *in[3];          // q, k, v
@@ -43,155 +43,194 @@ struct AppendProblem {
   const int *positions;
   const double *inv_freq;
   CacheView cache;
-  int first, heads[3], dim, half, chunks, per_warp;      // chunks of 8 channels in a row; rows of a warp
+  int n, heads[3], tokens[3], blocks[3];                 // of q, k, v: heads; tokens of a block; blocks
+  FastDiv by_heads[3];
+  int dim, half, interleaved, chunks, per_warp;                       // chunks of 8 channels in a row; rows of a warp
 };
 
 struct S32 {};
 struct F32 {};
 
-// eight channels as they come
-template <typename IN> struct Raw { uint4 a; };
-template <> struct Raw<S32> { uint4 a, b; };
-template <> struct Raw<F32> { uint4 a, b; };
-template <typename IN> struct Width { static constexpr int v = sizeof(Raw<IN>) / 8; };
+// four channels as they come
+template <typename IN> struct Raw { uint2 v; };
+template <> struct Raw<S32> { uint4 v; };
+template <> struct Raw<F32> { uint4 v; };
+template <typename IN> struct Width { static constexpr int v = sizeof(Raw<IN>) / 4; };
 
-template <typename IN> __device__ __forceinline__ Raw<IN> load8(const char *p) { return *reinterpret_cast<const Raw<IN> *>(p); }
-template <typename IN> __device__ __forceinline__ void values(const Raw<IN> &w, float (&x)[8])
+template <typename IN> __device__ __forceinline__ Raw<IN> load4(const char *p) { return *reinterpret_cast<const Raw<IN> *>(p); }
+template <typename IN> __device__ __forceinline__ void values(const Raw<IN> &w, float *x)
 {
-  const float2 a = unpack2<IN>(w.a.x), b = unpack2<IN>(w.a.y), c = unpack2<IN>(w.a.z), d = unpack2<IN>(w.a.w);
-  x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y; x[4] = c.x; x[5] = c.y; x[6] = d.x; x[7] = d.y;
+  const float2 a = unpack2<IN>(w.v.x), b = unpack2<IN>(w.v.y);
+  x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
 }
-template <> __device__ __forceinline__ void values<S32>(const Raw<S32> &w, float (&x)[8])
+template <> __device__ __forceinline__ void values<S32>(const Raw<S32> &w, float *x)
 {
-  x[0] = (float)(int)w.a.x; x[1] = (float)(int)w.a.y; x[2] = (float)(int)w.a.z; x[3] = (float)(int)w.a.w;
-  x[4] = (float)(int)w.b.x; x[5] = (float)(int)w.b.y; x[6] = (float)(int)w.b.z; x[7] = (float)(int)w.b.w;
+  x[0] = (float)(int)w.v.x; x[1] = (float)(int)w.v.y; x[2] = (float)(int)w.v.z; x[3] = (float)(int)w.v.w;
 }
-template <> __device__ __forceinline__ void values<F32>(const Raw<F32> &w, float (&x)[8])
+template <> __device__ __forceinline__ void values<F32>(const Raw<F32> &w, float *x)
 {
-  x[0] = __uint_as_float(w.a.x); x[1] = __uint_as_float(w.a.y); x[2] = __uint_as_float(w.a.z); x[3] = __uint_as_float(w.a.w);
-  x[4] = __uint_as_float(w.b.x); x[5] = __uint_as_float(w.b.y); x[6] = __uint_as_float(w.b.z); x[7] = __uint_as_float(w.b.w);
+  x[0] = __uint_as_float(w.v.x); x[1] = __uint_as_float(w.v.y); x[2] = __uint_as_float(w.v.z); x[3] = __uint_as_float(w.v.w);
 }
 template <typename IN> __device__ __forceinline__ float load1(const char *p) { return (float)*reinterpret_cast<const IN *>(p); }
 template <> __device__ __forceinline__ float load1<S32>(const char *p) { return (float)*reinterpret_cast<const int *>(p); }
 template <> __device__ __forceinline__ float load1<F32>(const char *p) { return *reinterpret_cast<const float *>(p); }
 // times the real value of a step, channel by channel
-__device__ __forceinline__ void times8(const float *step, float (&x)[8])
+__device__ __forceinline__ void times4(const float *step, float *x)
 {
-  float s[8];
   if ((reinterpret_cast<uintptr_t>(step) & 15) == 0) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(step)), b = __ldg(reinterpret_cast<const float4 *>(step) + 1);
-    s[0] = a.x; s[1] = a.y; s[2] = a.z; s[3] = a.w; s[4] = b.x; s[5] = b.y; s[6] = b.z; s[7] = b.w;
+    const float4 s = __ldg(reinterpret_cast<const float4 *>(step));
+    x[0] *= s.x; x[1] *= s.y; x[2] *= s.z; x[3] *= s.w;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; i++) s[i] = __ldg(step + i);
+    for (int i = 0; i < 4; i++) x[i] *= __ldg(step + i);
   }
-#pragma unroll
-  for (int i = 0; i < 8; i++) x[i] *= s[i];
 }
 // x * inv to the nearest integer, ties to even, in the low byte: 1.5 * 2^23 leaves the sum no bits below one
 __device__ __forceinline__ unsigned code(float x, float inv) { return __float_as_uint(fmaf(x, inv, 12582912.f)); }
 
-// One block: the queries, the keys or the values (blockIdx.y) of one token, so that everything but the head is the same for
-// the whole block. A warp holds per_warp whole rows; BATCH loads of a thread are under way together, the first of them
-// while the token's angles are computed.
-template <typename IN, typename WIDE, bool EIGHT, bool INTERLEAVED>
+// One block: the queries, the keys or the values of a few tokens, as many as give each thread about BATCH rows, so that
+// strides and addresses are the whole block's, and the tokens' angles and slots are looked up once. A warp holds per_warp whole
+// rows; BATCH loads of a thread are under way together, the first of them while the angles are computed.
+// HALVES (all channels rotate, or none): a lane's eight channels are four of each half of the row, so that it has both of every
+// pair, whichever way they are paired, and 32-bit rows are read without gaps between the lanes. Otherwise eight side by side, whose
+// mates come from another lane, or one by one where they are not eight side by side either.
+template <typename IN, typename WIDE, bool EIGHT, bool HALVES>
 __global__ void __launch_bounds__(WARPS * 32, Width<IN>::v == 2 ? 8 : 6) kv_append_kernel(const AppendProblem p)
 {
-  constexpr int SIZE = Width<IN>::v, BATCH = SIZE == 2 ? 4 : 2;
-  __shared__ __align__(16) float2 turn[MAX_HEAD_DIM / 2];
-  const int token = blockIdx.x, which = blockIdx.y + p.first, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int sub = lane / p.chunks, c0 = (lane - sub * p.chunks) * 8, first_lane = sub * p.chunks;
-  const int heads = p.heads[which], half = which < 2 ? p.half : 0;
-  const bool side_by_side = !INTERLEAVED && (half & 7) == 0, low = c0 < half, turns = c0 < 2 * half;
-  const int mate = (lane + (low ? half >> 3 : -(half >> 3))) & 31;      // holds the other channels of this lane's eight pairs
-  const int64_t in_head = p.in_head[which], out_head = p.out_head[which];
-  const char *in = p.in[which] + token * p.in_token[which] + c0 * SIZE;
-  char *out = p.out[which] ? p.out[which] + token * p.out_token[which] + c0 * 2 : nullptr;
+  constexpr int SIZE = Width<IN>::v, BATCH = SIZE == 2 ? 4 : 3;
+  __shared__ __align__(16) float2 turns[MOST_TOKENS][MAX_HEAD_DIM / 2];
+  __shared__ int2 where[MOST_TOKENS];           // page and place in it; page -1: the token is not stored
+  const int which = blockIdx.x < p.blocks[0] ? 0 : (blockIdx.x < p.blocks[0] + p.blocks[1] ? 1 : 2);
+  const int block = blockIdx.x - (which > 0 ? p.blocks[0] : 0) - (which > 1 ? p.blocks[1] : 0);
+  const int token0 = block * p.tokens[which], tokens = min(p.tokens[which], p.n - token0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sub = lane / p.chunks, chunk = lane - sub * p.chunks, first_lane = sub * p.chunks;
+  const int c0 = HALVES ? chunk * 4 : chunk * 8, c1 = HALVES ? p.dim / 2 + chunk * 4 : chunk * 8 + 4;      // two times four channels
+  const int heads = p.heads[which], rows = tokens * heads, half = which < 2 ? p.half : 0;
+  const FastDiv by_heads = p.by_heads[which];
+  const int64_t in_head = p.in_head[which], out_head = p.out_head[which], in_token = p.in_token[which], out_token = p.out_token[which];
+  const char *in = p.in[which] + token0 * in_token;
+  char *out = p.out[which] ? p.out[which] + token0 * out_token : nullptr;
   const float *steps = sizeof(IN) == 1 ? p.step[which] : nullptr;       // of S32 only
+  char *held = which == 1 ? p.cache.k : p.cache.v;
+  const int stride = WARPS * p.per_warp;
   pdl_wait();
-  const long long slot = which ? __ldg(p.slots + token) : -1;
-  const bool stored = slot >= 0 && slot < p.cache.n_slots;
-  const int page = stored ? p.cache.by_page.div((int)slot) : 0, at = stored ? (int)slot - page * p.cache.page_size : 0;
-  char *held = (which == 1 ? p.cache.k : p.cache.v) + (row_of(p.cache, page, at, 0) + c0) * (EIGHT ? 1 : 2);
-  const int64_t held_head = p.cache.head_stride * (EIGHT ? 1 : 2);
-  for (int head0 = warp * p.per_warp + sub, done = 0; done < heads; done += BATCH * WARPS * p.per_warp, head0 += BATCH * WARPS * p.per_warp) {
-    Raw<IN> own[BATCH];
+  for (int base = 0; base < rows; base += BATCH * stride) {
+    Raw<IN> lo[BATCH], hi[BATCH];
+    int head[BATCH], token[BATCH];
     bool live[BATCH];
 #pragma unroll
     for (int b = 0; b < BATCH; b++) {
-      const int head = head0 + b * WARPS * p.per_warp;
-      live[b] = sub < p.per_warp && head < heads;
-      if (live[b]) own[b] = load8<IN>(in + head * in_head);
+      const int row = base + b * stride + warp * p.per_warp + sub;
+      live[b] = sub < p.per_warp && row < rows;
+      token[b] = by_heads.div(row); head[b] = row - token[b] * heads;
+      if (live[b]) {
+        const char *src = in + token[b] * in_token + head[b] * in_head;
+        if (!HALVES && SIZE == 2) {
+          const uint4 both = *reinterpret_cast<const uint4 *>(src + c0 * SIZE);
+          reinterpret_cast<uint2 &>(lo[b]) = make_uint2(both.x, both.y); reinterpret_cast<uint2 &>(hi[b]) = make_uint2(both.z, both.w);
+        } else {
+          lo[b] = load4<IN>(src + c0 * SIZE); hi[b] = load4<IN>(src + c1 * SIZE);
+        }
+      }
     }
-    if (done == 0 && half) {
-      if (threadIdx.x < half) {
+    if (base == 0) {
+      for (int i = threadIdx.x; i < tokens * half; i += WARPS * 32) {
         // The angle in turns, in 64 bits: a position of 10^5 times a frequency near 1 leaves 32 bits with errors of 10^-2.
         // Its fraction of a turn keeps 24 bits, and sincospif takes multiples of pi.
-        const double t = (double)__ldg(p.positions + token) * __ldg(p.inv_freq + threadIdx.x) * 0.15915494309189533577;
+        const int k = i / half, f = i - k * half;
+        const double t = (double)__ldg(p.positions + token0 + k) * __ldg(p.inv_freq + f) * 0.15915494309189533577;
         float s, c;
         sincospif(2.f * (float)(t - rint(t)), &s, &c);
-        turn[threadIdx.x] = make_float2(c, s);
+        turns[k][f] = make_float2(c, s);
+      }
+      if (which && threadIdx.x < tokens) {
+        const long long slot = __ldg(p.slots + token0 + threadIdx.x);
+        const bool stored = slot >= 0 && slot < p.cache.n_slots;
+        const int page = stored ? p.cache.by_page.div((int)slot) : -1;
+        where[threadIdx.x] = make_int2(page, stored ? (int)slot - page * p.cache.page_size : 0);
       }
       __syncthreads();
     }
 #pragma unroll
     for (int b = 0; b < BATCH; b++) {
-      const int head = head0 + b * WARPS * p.per_warp;
       if (!__any_sync(0xffffffffu, live[b])) break;
-      float x[8], y[8], z[8];
-      if (!live[b]) own[b] = Raw<IN>{};
-      values<IN>(own[b], x);
-      if (sizeof(IN) == 1 && steps && live[b]) times8(steps + head * p.dim + c0, x);
-      if (side_by_side && half) {
-        if (SIZE == 2) {
-          Raw<IN> w;
-          w.a.x = __shfl_sync(0xffffffffu, own[b].a.x, mate); w.a.y = __shfl_sync(0xffffffffu, own[b].a.y, mate);
-          w.a.z = __shfl_sync(0xffffffffu, own[b].a.z, mate); w.a.w = __shfl_sync(0xffffffffu, own[b].a.w, mate);
-          values<IN>(w, z);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; i++) z[i] = __shfl_sync(0xffffffffu, x[i], mate);
-        }
+      float x[8], y[8];
+      if (!live[b]) lo[b] = hi[b] = Raw<IN>{};
+      values<IN>(lo[b], x);
+      values<IN>(hi[b], x + 4);
+      const int k = live[b] ? token[b] : 0;
+      const float2 *turn = turns[k];
+      if (sizeof(IN) == 1 && steps && live[b]) {
+        times4(steps + head[b] * p.dim + c0, x);
+        times4(steps + head[b] * p.dim + c1, x + 4);
       }
-      if (!turns) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) y[i] = x[i];
-      } else if (INTERLEAVED) {
+      for (int i = 0; i < 8; i++) y[i] = x[i];
+      if (HALVES && half && !p.interleaved) {
+        const float4 u = *reinterpret_cast<const float4 *>(turn + c0), v = *reinterpret_cast<const float4 *>(turn + c0 + 2);
+        const float cs[4] = {u.x, u.z, v.x, v.z}, sn[4] = {u.y, u.w, v.y, v.w};
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          const bool in_rot = c0 + i < 2 * half;
-          const float2 t = in_rot ? turn[(c0 + i) >> 1] : make_float2(1.f, 0.f);
-          y[i] = in_rot ? x[i] * t.x - x[i + 1] * t.y : x[i];
-          y[i + 1] = in_rot ? x[i + 1] * t.x + x[i] * t.y : x[i + 1];
+        for (int i = 0; i < 4; i++) {
+          y[i] = x[i] * cs[i] - x[i + 4] * sn[i];
+          y[i + 4] = x[i + 4] * cs[i] + x[i] * sn[i];
         }
-      } else if (side_by_side) {
-        const float sign = low ? -1.f : 1.f;
-        const float4 *t = reinterpret_cast<const float4 *>(turn + (low ? c0 : c0 - half));
+      } else if (half && p.interleaved) {
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          const float4 u = t[i / 2];
-          y[i] = x[i] * u.x + z[i] * (sign * u.y);
-          y[i + 1] = x[i + 1] * u.z + z[i + 1] * (sign * u.w);
+        for (int i = 0; i < 8; i += 4) {
+          const int c = i == 0 ? c0 : c1;
+          if (c < 2 * half) {
+            float4 u = *reinterpret_cast<const float4 *>(turn + (c >> 1));
+            if (c + 2 >= 2 * half) { u.z = 1.f; u.w = 0.f; }
+            y[i] = x[i] * u.x - x[i + 1] * u.y; y[i + 1] = x[i + 1] * u.x + x[i] * u.y;
+            y[i + 2] = x[i + 2] * u.z - x[i + 3] * u.w; y[i + 3] = x[i + 3] * u.z + x[i + 2] * u.w;
+          }
         }
-      } else {
+      } else if (!HALVES && half && (half & 7) == 0) {
+        const bool low = c0 < half;
+        const int mate = (lane + (low ? half >> 3 : -(half >> 3))) & 31;
+        float z[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) z[i] = __shfl_sync(0xffffffffu, x[i], mate);
+        if (c0 < 2 * half) {
+          const float sign = low ? -1.f : 1.f;
+          const float4 *t = reinterpret_cast<const float4 *>(turn + (low ? c0 : c0 - half));
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) {
+            const float4 u = t[i / 2];
+            y[i] = x[i] * u.x + z[i] * (sign * u.y);
+            y[i + 1] = x[i + 1] * u.z + z[i + 1] * (sign * u.w);
+          }
+        }
+      } else if (!HALVES && half) {
+        const char *src = in + token[b] * in_token + head[b] * in_head;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
           const int c = c0 + i;
-          y[i] = x[i];
           if (c < 2 * half && live[b]) {
             const bool lower = c < half;
-            const int to = lower ? half : -half;
-            float other = load1<IN>(in + head * in_head + (i + to) * SIZE);
-            if (sizeof(IN) == 1 && steps) other *= __ldg(steps + head * p.dim + c + to);
-            const float2 t = turn[lower ? c : c - half];
-            y[i] = x[i] * t.x + (lower ? -other : other) * t.y;
+            const int other = lower ? c + half : c - half;
+            float z = load1<IN>(src + other * SIZE);
+            if (sizeof(IN) == 1 && steps) z *= __ldg(steps + head[b] * p.dim + other);
+            const float2 t = turn[lower ? c : other];
+            y[i] = x[i] * t.x + (lower ? -z : z) * t.y;
           }
         }
+        __syncwarp();          // in place: every lane of the row has read what another lane now writes over
       }
-      if (!INTERLEAVED && !side_by_side) __syncwarp();        // in place: every lane of the row has read what another lane now writes over
-      const uint4 wide = make_uint4(pack2<WIDE>(y[0], y[1]), pack2<WIDE>(y[2], y[3]), pack2<WIDE>(y[4], y[5]), pack2<WIDE>(y[6], y[7]));
-      if (live[b] && out) *reinterpret_cast<uint4 *>(out + head * out_head) = wide;
+      const uint2 wide0 = make_uint2(pack2<WIDE>(y[0], y[1]), pack2<WIDE>(y[2], y[3])), wide1 = make_uint2(pack2<WIDE>(y[4], y[5]), pack2<WIDE>(y[6], y[7]));
+      auto put = [&](char *row) {
+        if (HALVES) {
+          *reinterpret_cast<uint2 *>(row + c0 * 2) = wide0;
+          *reinterpret_cast<uint2 *>(row + c1 * 2) = wide1;
+        } else {
+          *reinterpret_cast<uint4 *>(row + c0 * 2) = make_uint4(wide0.x, wide0.y, wide1.x, wide1.y);
+        }
+      };
+      if (live[b] && out) put(out + token[b] * out_token + head[b] * out_head);
       if (which == 0) continue;
+      const int2 at = where[k];
+      const bool stored = live[b] && at.x >= 0;
       if (EIGHT) {
         float most = 0.f;
         bool odd = false;
@@ -208,41 +247,53 @@ __global__ void __launch_bounds__(WARPS * 32, Width<IN>::v == 2 ? 8 : 6) kv_appe
           if (from >= p.chunks) from %= p.chunks;
           most = fmaxf(most, __shfl_sync(0xffffffffu, most, (first_lane + from) & 31));
         }
-        if (live[b] && stored) {
+        if (stored) {
           const bool fine = most <= 3.402823466e38f, any = most >= 7.888609e-31f && fine;     // 2^-100
           const float inv = any ? 127.f / most : 0.f;
-          uint2 w = make_uint2(0, 0);
+          unsigned w0 = 0, w1 = 0;
           if (any) {
-            w.x = __byte_perm(__byte_perm(code(y[0], inv), code(y[1], inv), 0x0040), __byte_perm(code(y[2], inv), code(y[3], inv), 0x0040), 0x5410);
-            w.y = __byte_perm(__byte_perm(code(y[4], inv), code(y[5], inv), 0x0040), __byte_perm(code(y[6], inv), code(y[7], inv), 0x0040), 0x5410);
+            w0 = __byte_perm(__byte_perm(code(y[0], inv), code(y[1], inv), 0x0040), __byte_perm(code(y[2], inv), code(y[3], inv), 0x0040), 0x5410);
+            w1 = __byte_perm(__byte_perm(code(y[4], inv), code(y[5], inv), 0x0040), __byte_perm(code(y[6], inv), code(y[7], inv), 0x0040), 0x5410);
           }
-          *reinterpret_cast<uint2 *>(held + head * held_head) = w;
-          if (c0 == 0)
-            (which == 1 ? p.cache.k_scale : p.cache.v_scale)[scale_of(p.cache, page, at, head)] =
+          char *row = held + row_of(p.cache, at.x, at.y, head[b]);
+          *reinterpret_cast<unsigned *>(row + c0) = w0;
+          *reinterpret_cast<unsigned *>(row + c1) = w1;
+          if (chunk == 0)
+            (which == 1 ? p.cache.k_scale : p.cache.v_scale)[scale_of(p.cache, at.x, at.y, head[b])] =
                 any ? most / 127.f : (fine ? 0.f : __int_as_float(0x7fffffff));
         }
-      } else if (live[b] && stored) {
-        *reinterpret_cast<uint4 *>(held + head * held_head) = wide;
+      } else if (stored) {
+        put(held + row_of(p.cache, at.x, at.y, head[b]) * 2);
       }
     }
   }
 }
 
 template <typename IN, typename WIDE, bool EIGHT>
-cudaError_t append_go(const AppendProblem &p, int n, bool interleaved, cudaStream_t s)
+cudaError_t append_go(AppendProblem &p, int sms, cudaStream_t s)
 {
-  const dim3 grid((unsigned)n, (unsigned)(3 - p.first));
-  return interleaved ? launch_pdl(kv_append_kernel<IN, WIDE, EIGHT, true>, grid, dim3(WARPS * 32), 0, s, p)
-                     : launch_pdl(kv_append_kernel<IN, WIDE, EIGHT, false>, grid, dim3(WARPS * 32), 0, s, p);
+  // tokens of a block: for BATCH rows a thread where there are blocks enough, else one
+  const int rows = WARPS * p.per_warp * (Width<IN>::v == 2 ? 4 : 3);
+  unsigned blocks = 0;
+  for (int i = 0; i < 3; i++) {
+    p.tokens[i] = 1; p.blocks[i] = 0;
+    if (p.heads[i] == 0) continue;
+    while (p.tokens[i] < MOST_TOKENS && p.tokens[i] * p.heads[i] < rows && p.n >= 8 * sms * (p.tokens[i] + 1)) p.tokens[i]++;
+    p.by_heads[i].set((unsigned)p.heads[i]);
+    p.blocks[i] = (p.n + p.tokens[i] - 1) / p.tokens[i];
+    blocks += (unsigned)p.blocks[i];
+  }
+  return p.half == 0 || 2 * p.half == p.dim ? launch_pdl(kv_append_kernel<IN, WIDE, EIGHT, true>, dim3(blocks), dim3(WARPS * 32), 0, s, p)
+                                            : launch_pdl(kv_append_kernel<IN, WIDE, EIGHT, false>, dim3(blocks), dim3(WARPS * 32), 0, s, p);
 }
 template <typename WIDE, bool EIGHT>
-cudaError_t append_in(int in_type, const AppendProblem &p, int n, bool interleaved, cudaStream_t s)
+cudaError_t append_in(int in_type, AppendProblem &p, int sms, cudaStream_t s)
 {
   switch (in_type) {
-    case PULPNN_TYPE_F16: return append_go<__half, WIDE, EIGHT>(p, n, interleaved, s);
-    case PULPNN_TYPE_BF16: return append_go<__nv_bfloat16, WIDE, EIGHT>(p, n, interleaved, s);
-    case PULPNN_TYPE_F32: return append_go<F32, WIDE, EIGHT>(p, n, interleaved, s);
-    default: return append_go<S32, WIDE, EIGHT>(p, n, interleaved, s);
+    case PULPNN_TYPE_F16: return append_go<__half, WIDE, EIGHT>(p, sms, s);
+    case PULPNN_TYPE_BF16: return append_go<__nv_bfloat16, WIDE, EIGHT>(p, sms, s);
+    case PULPNN_TYPE_F32: return append_go<F32, WIDE, EIGHT>(p, sms, s);
+    default: return append_go<S32, WIDE, EIGHT>(p, sms, s);
   }
 }
 
@@ -343,6 +394,7 @@ extern "C" int pulpnn_kv_append(const pulpnn_kv_cache_t *cache, const pulpnn_kv_
                "%s: a 16-bit cache of another type than out_type", who);
   ATTN_REQUIRE((a->q != nullptr) == (a->q_out != nullptr), PULPNN_ERR_INVALID_ARG, "%s: q without q_out, or q_out without q", who);
   ATTN_REQUIRE(!a->q || (a->n_q_heads > 0 && a->n_q_heads <= 65535), PULPNN_ERR_INVALID_ARG, "%s: %d query heads", who, a->n_q_heads);
+  ATTN_REQUIRE(a->n_tokens <= 0x2fffffff, PULPNN_ERR_UNSUPPORTED, "%s: %d tokens", who, a->n_tokens);
   ATTN_REQUIRE(a->rotary_dim >= 0 && a->rotary_dim <= cache->head_dim && a->rotary_dim % 2 == 0, PULPNN_ERR_INVALID_ARG,
                "%s: rotary_dim %d of %d channels", who, a->rotary_dim, cache->head_dim);
   ATTN_REQUIRE(a->rotary_dim == 0 || (a->positions && a->inv_freq), PULPNN_ERR_INVALID_ARG, "%s: a rotation without positions or frequencies", who);
@@ -373,13 +425,13 @@ extern "C" int pulpnn_kv_append(const pulpnn_kv_cache_t *cache, const pulpnn_kv_
   }
   p.slots = reinterpret_cast<const long long *>(a->slots); p.positions = a->positions; p.inv_freq = a->inv_freq;
   p.cache = view_of(*cache);
-  p.first = a->q ? 0 : 1; p.heads[0] = a->q ? a->n_q_heads : 0; p.heads[1] = p.heads[2] = cache->n_heads; p.dim = cache->head_dim;
-  p.half = a->rotary_dim / 2;
+  p.n = a->n_tokens; p.heads[0] = a->q ? a->n_q_heads : 0; p.heads[1] = p.heads[2] = cache->n_heads; p.dim = cache->head_dim;
+  p.half = a->rotary_dim / 2; p.interleaved = a->interleaved != 0;
   p.chunks = p.dim / 8; p.per_warp = 32 / p.chunks;
-  const bool il = a->interleaved != 0, f16 = a->out_type == PULPNN_TYPE_F16;
+  const bool f16 = a->out_type == PULPNN_TYPE_F16;
   const cudaError_t e = cache->type == PULPNN_TYPE_S8
-      ? (f16 ? append_in<__half, true>(a->in_type, p, a->n_tokens, il, c.stream) : append_in<__nv_bfloat16, true>(a->in_type, p, a->n_tokens, il, c.stream))
-      : (f16 ? append_in<__half, false>(a->in_type, p, a->n_tokens, il, c.stream) : append_in<__nv_bfloat16, false>(a->in_type, p, a->n_tokens, il, c.stream));
+      ? (f16 ? append_in<__half, true>(a->in_type, p, c.sm_count, c.stream) : append_in<__nv_bfloat16, true>(a->in_type, p, c.sm_count, c.stream))
+      : (f16 ? append_in<__half, false>(a->in_type, p, c.sm_count, c.stream) : append_in<__nv_bfloat16, false>(a->in_type, p, c.sm_count, c.stream));
   if (!cuda_ok(e, who)) return c.err;
   count_launch("kv_append_kernel");
   return PULPNN_OK;
