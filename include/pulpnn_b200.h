@@ -376,6 +376,8 @@ int pulpnn_kv_gather(const pulpnn_kv_cache_t *cache, const pulpnn_kv_gather_t *a
  *
  *  - q_type: F16 or BF16, the cache's where that is 16 bits wide. out_type: q_type, or U8: rint(out / out_step) + out_zero,
  *    cut to 0 .. 255.
+ *  - out overlaps no input. A long sequence of a call with few of them is read by several groups of CTAs, whose sums are
+ *    joined by a second kernel through memory allocated in the stream's order (in a capture: owned by the graph).
  *  - Lengths are cut to 0 .. max_pages * page_size. A token whose page lies outside the cache is left out, as if masked.
  *  - Scores, sums and the softmax are held in 32 bits; a token's weight is rounded to 16 bits for its product with v.
  */
@@ -400,7 +402,9 @@ int pulpnn_attn_decode(const pulpnn_kv_cache_t *cache, const pulpnn_attn_decode_
  *
  *  - type: F16 or BF16, of q, k and v. out_type: type, or U8 as above. scale > 0.
  *  - What a query does not see does not reach its result, infinities and NaN there included.
- *  - Offsets are cut to the rows there are; rows of out and lse that no sequence holds are left as they were.
+ *  - out overlaps no input; strides are positive and below 2^38. Offsets ascend; what lies beyond the rows there are is cut
+ *    off, and a sequence that ends before it begins is empty. Rows of out and lse that no sequence holds are left as
+ *    they were.
  *  - Scores, sums and the softmax are held in 32 bits; weights are rounded to 16 bits for their product with v.
  */
 typedef struct {

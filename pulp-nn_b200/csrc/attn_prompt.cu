@@ -880,7 +880,7 @@ extern "C" int pulpnn_attn_prompt(const pulpnn_attn_prompt_t *a)
   }
   // at most this many pairs of units: a sequence's rows fill all its tiles but one, and a pair may be half empty
   const int64_t pairs = (((int64_t)a->n_q_rows / BQ + a->n_seqs) * p.group + a->n_seqs + 1) / 2;
-  ATTN_REQUIRE(pairs <= 0x7fffffff, PULPNN_ERR_UNSUPPORTED, "%s: %d rows in %d sequences", who, a->n_q_rows, a->n_seqs);
+  ATTN_REQUIRE(pairs <= 0x3fffffff, PULPNN_ERR_UNSUPPORTED, "%s: %d rows in %d sequences", who, a->n_q_rows, a->n_seqs);
   const dim3 grid((unsigned)pairs, (unsigned)a->n_kv_heads);
   const bool f16 = a->type == PULPNN_TYPE_F16, narrow = a->head_dim <= 64;
   const bool ok = f16 ? (narrow ? prompt_go<__half, 64>(c, mq, mk, mv, p, grid) : prompt_go<__half, 128>(c, mq, mk, mv, p, grid))

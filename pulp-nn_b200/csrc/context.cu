@@ -3,7 +3,6 @@
 #include <cstdio>
 #include <cstring>
 #include <atomic>
-#include <mutex>
 #include <new>
 
 #include "internal.cuh"
@@ -154,23 +153,24 @@ bool ctx_partials_done(Context &c)
 // host waits). It lives as long as the process.
 static cudaMemPool_t stream_pool(int device)
 {
-  static std::mutex lock;
-  static cudaMemPool_t pools[MAX_DEVICES] = {};
+  static std::atomic<cudaMemPool_t> pools[MAX_DEVICES];
   if (device < 0 || device >= MAX_DEVICES) return nullptr;
-  std::lock_guard<std::mutex> guard(lock);
-  if (!pools[device]) {
-    RelaxedCapture relaxed;
-    cudaMemPoolProps props = {};
-    props.allocType = cudaMemAllocationTypePinned;
-    props.location.type = cudaMemLocationTypeDevice;
-    props.location.id = device;
-    cudaMemPool_t pool;
-    if (cudaMemPoolCreate(&pool, &props) != cudaSuccess) { cudaGetLastError(); return nullptr; }
-    uint64_t keep = ~0ull;
-    if (cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep) != cudaSuccess) cudaGetLastError();
-    pools[device] = pool;
+  cudaMemPool_t have = pools[device].load(std::memory_order_acquire);
+  if (have) return have;
+  RelaxedCapture relaxed;
+  cudaMemPoolProps props = {};
+  props.allocType = cudaMemAllocationTypePinned;
+  props.location.type = cudaMemLocationTypeDevice;
+  props.location.id = device;
+  cudaMemPool_t pool;
+  if (cudaMemPoolCreate(&pool, &props) != cudaSuccess) { cudaGetLastError(); return nullptr; }
+  uint64_t keep = ~0ull;
+  if (cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep) != cudaSuccess) cudaGetLastError();
+  if (!pools[device].compare_exchange_strong(have, pool, std::memory_order_acq_rel)) {
+    cudaMemPoolDestroy(pool);        // another thread was first
+    return have;
   }
-  return pools[device];
+  return pool;
 }
 
 void *ctx_stream_alloc(Context &c, size_t bytes)

@@ -38,6 +38,7 @@ struct AppendProblem {
   const char *in[3];          // q, k, v
   char *out[3];
   const float *step[3];
+  int step_vector[3];         // begins on a 16-byte boundary
   int64_t in_token[3], in_head[3], out_token[3], out_head[3];      // bytes
   const long long *slots;
   const int *positions;
@@ -45,7 +46,7 @@ struct AppendProblem {
   CacheView cache;
   int n, heads[3], tokens[3], blocks[3];                 // of q, k, v: heads; tokens of a block; blocks
   FastDiv by_heads[3];
-  int dim, half, interleaved, chunks, per_warp;                       // chunks of 8 channels in a row; rows of a warp
+  int dim, half, interleaved, chunks, pow2, per_warp;                       // chunks of 8 channels in a row; rows of a warp
 };
 
 struct S32 {};
@@ -75,15 +76,22 @@ template <typename IN> __device__ __forceinline__ float load1(const char *p) { r
 template <> __device__ __forceinline__ float load1<S32>(const char *p) { return (float)*reinterpret_cast<const int *>(p); }
 template <> __device__ __forceinline__ float load1<F32>(const char *p) { return *reinterpret_cast<const float *>(p); }
 // times the real value of a step, channel by channel
-__device__ __forceinline__ void times4(const float *step, float *x)
+__device__ __forceinline__ void times4(const float *step, bool vector, float *x)
 {
-  if ((reinterpret_cast<uintptr_t>(step) & 15) == 0) {
+  if (vector) {
     const float4 s = __ldg(reinterpret_cast<const float4 *>(step));
     x[0] *= s.x; x[1] *= s.y; x[2] *= s.z; x[3] *= s.w;
   } else {
 #pragma unroll
     for (int i = 0; i < 4; i++) x[i] *= __ldg(step + i);
   }
+}
+// the larger magnitude; NaN where one of them is
+__device__ __forceinline__ float larger(float a, float b)
+{
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
 }
 // x * inv to the nearest integer, ties to even, in the low byte: 1.5 * 2^23 leaves the sum no bits below one
 __device__ __forceinline__ unsigned code(float x, float inv) { return __float_as_uint(fmaf(x, inv, 12582912.f)); }
@@ -99,7 +107,7 @@ __global__ void __launch_bounds__(WARPS * 32, Width<IN>::v == 2 ? 8 : 6) kv_appe
 {
   constexpr int SIZE = Width<IN>::v, BATCH = SIZE == 2 ? 4 : 3;
   __shared__ __align__(16) float2 turns[MOST_TOKENS][MAX_HEAD_DIM / 2];
-  __shared__ int2 where[MOST_TOKENS];           // page and place in it; page -1: the token is not stored
+  __shared__ longlong2 where[MOST_TOKENS];      // of a token's head 0: its row's and its scale's place in the cache; -1: it is not stored
   const int which = blockIdx.x < p.blocks[0] ? 0 : (blockIdx.x < p.blocks[0] + p.blocks[1] ? 1 : 2);
   const int block = blockIdx.x - (which > 0 ? p.blocks[0] : 0) - (which > 1 ? p.blocks[1] : 0);
   const int token0 = block * p.tokens[which], tokens = min(p.tokens[which], p.n - token0);
@@ -147,8 +155,8 @@ __global__ void __launch_bounds__(WARPS * 32, Width<IN>::v == 2 ? 8 : 6) kv_appe
       if (which && threadIdx.x < tokens) {
         const long long slot = __ldg(p.slots + token0 + threadIdx.x);
         const bool stored = slot >= 0 && slot < p.cache.n_slots;
-        const int page = stored ? p.cache.by_page.div((int)slot) : -1;
-        where[threadIdx.x] = make_int2(page, stored ? (int)slot - page * p.cache.page_size : 0);
+        const int page = stored ? p.cache.by_page.div((int)slot) : 0, at = stored ? (int)slot - page * p.cache.page_size : 0;
+        where[threadIdx.x] = stored ? make_longlong2(row_of(p.cache, page, at, 0), scale_of(p.cache, page, at, 0)) : make_longlong2(-1, -1);
       }
       __syncthreads();
     }
@@ -162,8 +170,8 @@ __global__ void __launch_bounds__(WARPS * 32, Width<IN>::v == 2 ? 8 : 6) kv_appe
       const int k = live[b] ? token[b] : 0;
       const float2 *turn = turns[k];
       if (sizeof(IN) == 1 && steps && live[b]) {
-        times4(steps + head[b] * p.dim + c0, x);
-        times4(steps + head[b] * p.dim + c1, x + 4);
+        times4(steps + head[b] * p.dim + c0, p.step_vector[which], x);
+        times4(steps + head[b] * p.dim + c1, p.step_vector[which], x + 4);
       }
 #pragma unroll
       for (int i = 0; i < 8; i++) y[i] = x[i];
@@ -229,41 +237,43 @@ __global__ void __launch_bounds__(WARPS * 32, Width<IN>::v == 2 ? 8 : 6) kv_appe
       };
       if (live[b] && out) put(out + token[b] * out_token + head[b] * out_head);
       if (which == 0) continue;
-      const int2 at = where[k];
+      const longlong2 at = where[k];
       const bool stored = live[b] && at.x >= 0;
+      const int64_t place = at.x + head[b] * p.cache.head_stride;
       if (EIGHT) {
         float most = 0.f;
-        bool odd = false;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          most = fmaxf(most, fabsf(y[i]));
-          odd |= !(fabsf(y[i]) <= 3.402823466e38f);
-        }
-        if (odd) most = __int_as_float(0x7f800000);
-        // around the row's lanes: after steps of 1, 2, 4 and 8 each of up to 16 has met all others
+        for (int i = 0; i < 8; i++) most = larger(most, y[i]);
+        if (p.pow2) {
 #pragma unroll
-        for (int d = 1; d < 16; d *= 2) {
-          int from = lane - first_lane + d;
-          if (from >= p.chunks) from %= p.chunks;
-          most = fmaxf(most, __shfl_sync(0xffffffffu, most, (first_lane + from) & 31));
+          for (int d = 1; d < 16; d *= 2)
+            if (d < p.chunks) most = larger(most, __shfl_xor_sync(0xffffffffu, most, d));
+        } else {
+          // around the row's lanes: after steps of 1, 2, 4 and 8 each of up to 16 has met all others
+#pragma unroll
+          for (int d = 1; d < 16; d *= 2) {
+            int from = lane - first_lane + d;
+            while (from >= p.chunks) from -= p.chunks;
+            most = larger(most, __shfl_sync(0xffffffffu, most, (first_lane + from) & 31));
+          }
         }
         if (stored) {
           const bool fine = most <= 3.402823466e38f, any = most >= 7.888609e-31f && fine;     // 2^-100
-          const float inv = any ? 127.f / most : 0.f;
+          const float inv = __frcp_rn(most) * 127.f;
           unsigned w0 = 0, w1 = 0;
           if (any) {
             w0 = __byte_perm(__byte_perm(code(y[0], inv), code(y[1], inv), 0x0040), __byte_perm(code(y[2], inv), code(y[3], inv), 0x0040), 0x5410);
             w1 = __byte_perm(__byte_perm(code(y[4], inv), code(y[5], inv), 0x0040), __byte_perm(code(y[6], inv), code(y[7], inv), 0x0040), 0x5410);
           }
-          char *row = held + row_of(p.cache, at.x, at.y, head[b]);
+          char *row = held + place;
           *reinterpret_cast<unsigned *>(row + c0) = w0;
           *reinterpret_cast<unsigned *>(row + c1) = w1;
           if (chunk == 0)
-            (which == 1 ? p.cache.k_scale : p.cache.v_scale)[scale_of(p.cache, at.x, at.y, head[b])] =
-                any ? most / 127.f : (fine ? 0.f : __int_as_float(0x7fffffff));
+            (which == 1 ? p.cache.k_scale : p.cache.v_scale)[at.y + head[b] * p.cache.s_head_stride] =
+                any ? most * (1.f / 127.f) : (fine ? 0.f : __int_as_float(0x7fffffff));
         }
       } else if (stored) {
-        put(held + row_of(p.cache, at.x, at.y, head[b]) * 2);
+        put(held + place * 2);
       }
     }
   }
@@ -394,7 +404,7 @@ extern "C" int pulpnn_kv_append(const pulpnn_kv_cache_t *cache, const pulpnn_kv_
                "%s: a 16-bit cache of another type than out_type", who);
   ATTN_REQUIRE((a->q != nullptr) == (a->q_out != nullptr), PULPNN_ERR_INVALID_ARG, "%s: q without q_out, or q_out without q", who);
   ATTN_REQUIRE(!a->q || (a->n_q_heads > 0 && a->n_q_heads <= 65535), PULPNN_ERR_INVALID_ARG, "%s: %d query heads", who, a->n_q_heads);
-  ATTN_REQUIRE(a->n_tokens <= 0x2fffffff, PULPNN_ERR_UNSUPPORTED, "%s: %d tokens", who, a->n_tokens);
+  ATTN_REQUIRE(a->n_tokens <= 0x2aaaaaaa, PULPNN_ERR_UNSUPPORTED, "%s: %d tokens", who, a->n_tokens);
   ATTN_REQUIRE(a->rotary_dim >= 0 && a->rotary_dim <= cache->head_dim && a->rotary_dim % 2 == 0, PULPNN_ERR_INVALID_ARG,
                "%s: rotary_dim %d of %d channels", who, a->rotary_dim, cache->head_dim);
   ATTN_REQUIRE(a->rotary_dim == 0 || (a->positions && a->inv_freq), PULPNN_ERR_INVALID_ARG, "%s: a rotation without positions or frequencies", who);
@@ -419,7 +429,7 @@ extern "C" int pulpnn_kv_append(const pulpnn_kv_cache_t *cache, const pulpnn_kv_
   const float *step[3] = {a->q_step, a->k_step, a->v_step};
   const int64_t *is_[3] = {a->q_stride, a->k_stride, a->v_stride}, *os[3] = {a->q_out_stride, a->k_out_stride, a->v_out_stride};
   for (int i = 0; i < 3; i++) {
-    p.in[i] = static_cast<const char *>(in[i]); p.out[i] = static_cast<char *>(out[i]); p.step[i] = s32 ? step[i] : nullptr;
+    p.in[i] = static_cast<const char *>(in[i]); p.out[i] = static_cast<char *>(out[i]); p.step[i] = s32 ? step[i] : nullptr; p.step_vector[i] = aligned(step[i], 16);
     p.in_token[i] = is_[i][0] * is; p.in_head[i] = is_[i][1] * is;
     p.out_token[i] = os[i][0] * 2; p.out_head[i] = os[i][1] * 2;
   }
@@ -427,7 +437,7 @@ extern "C" int pulpnn_kv_append(const pulpnn_kv_cache_t *cache, const pulpnn_kv_
   p.cache = view_of(*cache);
   p.n = a->n_tokens; p.heads[0] = a->q ? a->n_q_heads : 0; p.heads[1] = p.heads[2] = cache->n_heads; p.dim = cache->head_dim;
   p.half = a->rotary_dim / 2; p.interleaved = a->interleaved != 0;
-  p.chunks = p.dim / 8; p.per_warp = 32 / p.chunks;
+  p.chunks = p.dim / 8; p.pow2 = (p.chunks & (p.chunks - 1)) == 0; p.per_warp = 32 / p.chunks;
   const bool f16 = a->out_type == PULPNN_TYPE_F16;
   const cudaError_t e = cache->type == PULPNN_TYPE_S8
       ? (f16 ? append_in<__half, true>(a->in_type, p, c.sm_count, c.stream) : append_in<__nv_bfloat16, true>(a->in_type, p, c.sm_count, c.stream))

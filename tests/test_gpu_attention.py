@@ -295,6 +295,121 @@ def test_decode_uint8_output(cache):
     decode_case(7, [1, 40, 300], 4, 2, 128, F16, cache, 16, False, u8=True)
 
 
+@pytest.fixture
+def forced_split():
+    yield lambda n: api.set_option(api.OPT_SPLIT_K, n)
+    api.set_option(api.OPT_SPLIT_K, 0)
+
+
+@pytest.mark.parametrize("cache,page,dim", [(BF16, 16, 128), (S8, 32, 64), (S8, 20, 128), (F16, 7, 80)])
+@pytest.mark.parametrize("split", [1, 2, 3, 7, 8, 16, 40, 600])
+def test_decode_splits(forced_split, split, cache, page, dim):
+    """However many CTAs and clusters share a sequence (600: more than there are tiles), empty sequences among them."""
+    forced_split(split)
+    decode_case(split, [0, 1, 130, 1000, 33], 12, 1, dim, F16 if cache == F16 else BF16, cache, page, False)
+    if split >= 16:
+        assert api.last_kernel() == "attn_join_kernel"
+
+
+def test_decode_splits_uint8_output(forced_split):
+    forced_split(24)
+    decode_case(7, [1, 40, 0, 700], 4, 2, 72, F16, F16, 16, False, u8=True)
+
+
+def test_decode_one_long_sequence_is_shared_by_clusters():
+    decode_case(13, [60000], 4, 1, 128, BF16, BF16, 16, False)
+    assert api.last_kernel() == "attn_join_kernel"
+
+
+def test_decode_captured_and_on_several_streams_at_once():
+    """Calls that need memory for their parts: captured into two graphs that are replayed side by side with a third, eager
+    stream, lengths changing between replays."""
+    g = gen(14)
+    dim, page, pages = 128, 16, 2048
+    c = Cache(g, BF16, 2 * pages, page, 1, dim, False)
+    tables = [torch.randperm(2 * pages, generator=g, device="cuda")[:pages].to(torch.int32)[None].contiguous() for _ in range(3)]
+    q = [normal(g, 1, 4, dim, dtype=BF16) for _ in range(3)]
+    lens = [torch.zeros(1, dtype=torch.int32, device="cuda") for _ in range(3)]
+    out, want = [torch.empty_like(x) for x in q], []
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    graphs = []
+    torch.cuda.synchronize()
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        api.set_stream(streams[i])
+        with torch.cuda.graph(graph, stream=streams[i]):
+            api.pulpnn_attn_decode(c.handle, q[i], tables[i], lens[i], out[i])
+        assert api.last_kernel() == "attn_join_kernel"
+        graphs.append(graph)
+    for turn, n in enumerate((30000, 17, 0, 32768)):
+        for i in range(3):
+            lens[i].fill_(max(0, n - 100 * i))
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for i in range(2):
+                with torch.cuda.stream(streams[i]):
+                    graphs[i].replay()
+            api.set_stream(streams[2])
+            api.pulpnn_attn_decode(c.handle, q[2], tables[2], lens[2], out[2])
+        api.set_stream(None)
+        torch.cuda.synchronize()
+        for i in range(3):
+            m = max(0, n - 100 * i)
+            t = torch.arange(m, device="cuda")
+            slots = tables[i][0].long()[t // page] * page + t % page
+            k, v = (c.rows(w, slots)[:, 0] for w in range(2))
+            want, _, sums, product = attend(q[i][0].double(), k, v, torch.ones(4, m, dtype=torch.bool, device="cuda"), dim ** -0.5)
+            if m == 0:
+                assert (out[i] == 0).all()
+            else:
+                assert ((out[i][0].double() - want).abs() <= tolerance(want, sums, product, m, dim, BF16, BF16)).all(), (turn, i)
+
+
+def test_calls_of_several_threads():
+    """Each host thread has a context, a stream and its own results."""
+    import threading
+    g = gen(15)
+    c = Cache(g, S8, 600, 16, 2, 64, False)
+    jobs, errors = [], []
+    for i in range(4):
+        n = 2000 * i + 150
+        q = normal(g, 1, 8, 64, dtype=BF16)
+        table = torch.randperm(600, generator=g, device="cuda")[:(n + 15) // 16].to(torch.int32)[None].contiguous()
+        lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+        want = torch.empty_like(q)
+        api.pulpnn_attn_decode(c.handle, q, table, lens, want)
+        p = normal(g, 200 + i, 4, 64, dtype=F16)
+        cu = torch.tensor([0, 200 + i], dtype=torch.int32, device="cuda")
+        pw = torch.empty_like(p)
+        api.pulpnn_attn_prompt(p, p[:, :2], p[:, 2:], cu, pw)
+        jobs.append((q, table, lens, want, p, cu, pw))
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            api.set_device(0)
+            stream = torch.cuda.Stream()
+            api.set_stream(stream)
+            q, table, lens, want, p, cu, pw = jobs[i]
+            for _ in range(20):
+                out, po = torch.empty_like(q), torch.empty_like(p)
+                stream.wait_stream(torch.cuda.current_stream())
+                api.pulpnn_attn_decode(c.handle, q, table, lens, out)
+                api.pulpnn_attn_prompt(p, p[:, :2], p[:, 2:], cu, po)
+                api.synchronize()
+                assert torch.equal(out, want) and torch.equal(po, pw)
+            assert api.device_status() == 0
+        except BaseException as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+
+
 @pytest.mark.parametrize("cache", [BF16, S8])
 def test_decode_pages_outside_the_cache_are_left_out(cache):
     decode_case(8, [40, 100, 700, 33], 4, 1, 64, BF16, cache, 16, False, bad=True, extra_pages=3)
