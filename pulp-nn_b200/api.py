@@ -469,28 +469,27 @@ class KVCache:
     _pack = struct.Struct("=4Q6q6i").pack
 
     def __init__(self, k, v, k_scale=None, v_scale=None, heads_first=False):
-        _need(k.dim() == 4 and k.shape == v.shape, "keys and values of shapes %s and %s" % (tuple(k.shape), tuple(v.shape)))
-        _need(k.dtype == v.dtype and k.stride() == v.stride(), "keys and values of different types or strides")
-        _need(k.stride(3) == 1, "the channels of a row do not lie side by side")
-        self.type, self.heads_first, self.tensors = _type(k), heads_first, (k, v, k_scale, v_scale)
-        pages, slots, heads, self.head_dim = k.shape
-        s, axes = k.stride(), (0, 1, 2)
-        if heads_first:
-            slots, heads, axes = heads, slots, (0, 2, 1)
-        self.n_pages, self.page_size, self.n_heads, t = pages, slots, heads, (0, 0, 0)
-        _need(all(n == 1 or st != 0 for n, st in zip(k.shape, s)), "rows of the cache share memory")
-        if self.type == TYPE_S8:
-            _need(k_scale is not None and v_scale is not None, "an int8 cache without scales")
-            _need(k_scale.shape == k.shape[:3] and v_scale.shape == k.shape[:3], "scales are shaped as the cache without its last axis")
+        shape, s, type_ = k.shape, k.stride(), _type(k)
+        _need(len(shape) == 4 and v.shape == shape, "keys and values are of one shape, with four axes")
+        _need(v.dtype == k.dtype and v.stride() == s, "keys and values are of one type, with the same strides")
+        _need(s[3] == 1, "the channels of a row lie side by side")
+        _need((s[0] or shape[0] == 1) and (s[1] or shape[1] == 1) and (s[2] or shape[2] == 1), "rows of the cache share memory")
+        t = (0, 0, 0)
+        if type_ == TYPE_S8:
+            _need(k_scale is not None and v_scale is not None, "an int8 cache has scales")
+            _need(k_scale.shape == shape[:3] and v_scale.shape == shape[:3], "scales are shaped as the cache without its last axis")
             _need(_type(k_scale) == TYPE_F32 and _type(v_scale) == TYPE_F32, "scales are float32")
-            _need(k_scale.stride() == v_scale.stride(), "scales with different strides")
             t = k_scale.stride()
-            _need(all(n == 1 or st != 0 for n, st in zip(k.shape, t)), "scales share memory")
+            _need(v_scale.stride() == t, "scales have the same strides")
+            _need((t[0] or shape[0] == 1) and (t[1] or shape[1] == 1) and (t[2] or shape[2] == 1), "scales share memory")
         else:
-            _need(k_scale is None and v_scale is None, "scales of a 16-bit cache")
-        s = [s[i] if k.shape[i] > 1 else 0 for i in axes]
-        self.block = self._pack(k.data_ptr(), v.data_ptr(), _addr_of(k_scale), _addr_of(v_scale), *s, *(t[i] for i in axes), self.type,
-                                pages, slots, heads, self.head_dim, 0)
+            _need(k_scale is None and v_scale is None, "a 16-bit cache has no scales")
+        self.type, self.heads_first, self.tensors = type_, heads_first, (k, v, k_scale, v_scale)
+        slot, head = (2, 1) if heads_first else (1, 2)          # the axes
+        self.n_pages, self.page_size, self.n_heads, self.head_dim = shape[0], shape[slot], shape[head], shape[3]
+        self.block = self._pack(k.data_ptr(), v.data_ptr(), _addr_of(k_scale), _addr_of(v_scale), s[0] if shape[0] > 1 else 0,
+                                s[slot] if shape[slot] > 1 else 0, s[head] if shape[head] > 1 else 0, t[0], t[slot], t[head], type_,
+                                self.n_pages, self.page_size, self.n_heads, self.head_dim, 0)
 
 
 def _addr_of(x):
