@@ -79,6 +79,11 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t a, unsigned (&r)[4])
 {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
+// two 16x16 blocks of bytes, transposed: a lane's word i of a block holds column g + 8 i of rows 4t .. 4t + 3
+__device__ __forceinline__ void ldmatrix2_trans8(uint32_t a, unsigned (&r)[4])
+{
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
 __device__ __forceinline__ unsigned transpose8(unsigned a)
 {
   unsigned d;
@@ -336,6 +341,12 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     l[nt][0] = l[nt][1] = 0.f;
   }
 
+  // Which of 16 tokens are rows g and g + 8 of the products' fragments. 8-bit: the transposed load gives a lane tokens 4t .. 4t + 3,
+  // of which two follow from rows 2t and 2t + 1 of the first eight and two from the second eight; t >= 2 has them the other
+  // way round, so that the first eight rows of a key load lie in different banks.
+  auto token_of = [&](int r) { return EIGHT ? 4 * (g >> 1) + ((g >> 2) ^ r) * 2 + (g & 1) : r * 8 + g; };
+  const int k_row = 4 * ((lane & 7) >> 1) + ((((lane & 7) >> 2) ^ ((lane >> 3) & 1)) * 2) + (lane & 1);
+  const unsigned first_two = t < 2 ? 0x4140 : 0x4342, last_two = t < 2 ? 0x4342 : 0x4140;
   bool landed = true;
   for (int i = 0; i < mine; i++) {
     const int stage = i % STAGES;
@@ -358,7 +369,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       __syncwarp();
     }
 
-    // S^T: tokens 16 mt + {g, g + 8} x heads 8 nt + {2t, 2t + 1}
+    // S^T: tokens 16 mt + {token_of(0), token_of(1)} x heads 8 nt + {2t, 2t + 1}
     float s[MT][NT][4];
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
@@ -367,17 +378,23 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 #pragma unroll
         for (int e = 0; e < 4; e++) s[mt][nt][e] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++) {
+      for (int ks = 0; ks < KS; ks += EIGHT ? 2 : 1) {
         unsigned a[4];
         if (EIGHT) {
-          const unsigned w0 = lds32(base + TL::at(mt * 16 + g, ks) + 4 * t) ^ 0x80808080u;
-          const unsigned w1 = lds32(base + TL::at(mt * 16 + 8 + g, ks) + 4 * t) ^ 0x80808080u;
-          a[0] = widen(w0, 0x4140); a[1] = widen(w1, 0x4140); a[2] = widen(w0, 0x4342); a[3] = widen(w1, 0x4342);
+          unsigned w[4];
+          ldmatrix4(base + TL::at(mt * 16 + k_row, ks + (lane >> 4)), w);
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const unsigned w0 = w[2 * e] ^ 0x80808080u, w1 = w[2 * e + 1] ^ 0x80808080u;
+            a[0] = widen(w0, 0x4140); a[1] = widen(w1, 0x4140); a[2] = widen(w0, 0x4342); a[3] = widen(w1, 0x4342);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) mma<T>(s[mt][nt], a, qf[nt][ks + e][0], qf[nt][ks + e][1]);
+          }
         } else {
           ldmatrix4(base + TL::at(mt * 16 + (lane & 15), ks * 2 + (lane >> 4)), a);
-        }
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) mma<T>(s[mt][nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+          for (int nt = 0; nt < NT; nt++) mma<T>(s[mt][nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+        }
       }
     }
     float vs[MT][2], lvs[MT][2];
@@ -386,7 +403,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     for (int mt = 0; mt < MT; mt++)
 #pragma unroll
       for (int r = 0; r < 2; r++) {
-        const int token = mt * 16 + r * 8 + g;
+        const int token = mt * 16 + token_of(r);
         const bool ok = (live >> token) & 1u;
         float ks_ = 1.f;
         if (EIGHT) {
@@ -452,14 +469,12 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       if (EIGHT) {
 #pragma unroll
         for (int blk = 0; blk < DP / 32; blk++) {
-          const uint32_t v = vbase + TL::at(mt * 16 + 2 * t, blk * 2 + (g >> 2)) + 4 * (g & 3);
-          const uint32_t u = vbase + TL::at(mt * 16 + 2 * t + 1, blk * 2 + (g >> 2)) + 4 * (g & 3);
-          const unsigned w0 = lds32(v) ^ 0x80808080u, w1 = lds32(u) ^ 0x80808080u;
-          const unsigned w2 = lds32(v + 8 * 128) ^ 0x80808080u, w3 = lds32(u + 8 * 128) ^ 0x80808080u;
-          const unsigned x0 = __byte_perm(w0, w1, 0x5140), x1 = __byte_perm(w0, w1, 0x7362);
-          const unsigned y0 = __byte_perm(w2, w3, 0x5140), y1 = __byte_perm(w2, w3, 0x7362);
-          const unsigned a0[4] = {widen(x0, 0x4140), widen(x0, 0x4342), widen(y0, 0x4140), widen(y0, 0x4342)};
-          const unsigned a1[4] = {widen(x1, 0x4140), widen(x1, 0x4342), widen(y1, 0x4140), widen(y1, 0x4342)};
+          unsigned w[4];
+          ldmatrix2_trans8(vbase + TL::at(mt * 16 + (lane & 15), blk * 2 + (lane >> 4)), w);
+#pragma unroll
+          for (int e = 0; e < 4; e++) w[e] ^= 0x80808080u;
+          const unsigned a0[4] = {widen(w[0], first_two), widen(w[1], first_two), widen(w[0], last_two), widen(w[1], last_two)};
+          const unsigned a1[4] = {widen(w[2], first_two), widen(w[3], first_two), widen(w[2], last_two), widen(w[3], last_two)};
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) {
             mma<T>(o[nt][2 * blk], a0, b[nt][0], b[nt][1]);
@@ -504,7 +519,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       for (int ks = 0; ks < KS; ks++)
 #pragma unroll
         for (int r = 0; r < 2; r++) {
-          const int ch = EIGHT ? (ks >> 1) * 32 + 4 * g + 2 * (ks & 1) + r : ks * 16 + r * 8 + g;
+          const int ch = ks * 16 + r * 8 + g;
           dst[ch] = o[nt][ks][2 * r + c];
         }
     }
