@@ -440,7 +440,7 @@ def _vector(x, name, n, type_):
     """Address of n contiguous values, 0 for None."""
     if x is None:
         return 0
-    if x.shape != (n,) or not x.is_contiguous() or _type(x) != type_:
+    if x.numel() != n or _type_of.get(x.dtype) != type_ or not x.is_contiguous():
         raise PulpNNError(ERR_INVALID_ARG, "%s: %s %s, where %d values in one piece are wanted" % (name, x.dtype, tuple(x.shape), n))
     return x.data_ptr()
 
@@ -454,10 +454,10 @@ class _StructCall:
     def __call__(self, *blocks):
         f = self.f
         if f is None:
-            f = getattr(_lib.load_library(), self.name)
-            f.restype, f.argtypes = C.c_int, [C.c_char_p] * self.n
-            self.f = f
-        if f(*blocks) != OK:
+            # the library's functions are shared objects of ctypes: a prototype of our own leaves theirs alone
+            proto = C.CFUNCTYPE(C.c_int, *[C.c_char_p] * self.n)
+            f = self.f = proto(C.cast(getattr(_lib.load_library(), self.name), C.c_void_p).value)
+        if f(*blocks):
             _check()
 
 
@@ -500,7 +500,6 @@ _append_pack = struct.Struct("=12Q12q6i").pack
 _append_call = _StructCall("pulpnn_kv_append", 2)
 _gather_pack = struct.Struct("=3Q4q2i").pack
 _gather_call = _StructCall("pulpnn_kv_gather", 2)
-_NO_ROWS = (0, 0, 0)
 
 
 def pulpnn_kv_append(cache, slots, k, v, positions=None, inv_freq=None, interleaved=False, q=None, q_out=None, k_out=None,
@@ -512,33 +511,40 @@ def pulpnn_kv_append(cache, slots, k, v, positions=None, inv_freq=None, interlea
     if n == 0:
         return
     in_type = _type(k)
-    out_type = cache.type if cache.type != TYPE_S8 else None
-    for o in (q_out, k_out, v_out):
-        if out_type is None and o is not None:
-            out_type = _type(o)
-    if out_type is None:
-        out_type = TYPE_BF16                                # nothing of that type is written
-    pk, pv = _rows(k, "k", n, heads, dim, in_type), _rows(v, "v", n, heads, dim, in_type)
-    _need((q is None) == (q_out is None), "q and q_out come together")
-    pq, oq, hq = _NO_ROWS, _NO_ROWS, 0
+    out_type = cache.type
+    if out_type == TYPE_S8:                     # the outputs' own; any, where nothing of that type is written
+        o = q_out if q_out is not None else k_out if k_out is not None else v_out
+        out_type = TYPE_BF16 if o is None else _type(o)
+    pk, pk0, pk1 = _rows(k, "k", n, heads, dim, in_type)
+    pv, pv0, pv1 = _rows(v, "v", n, heads, dim, in_type)
+    pq = pq0 = pq1 = oq = oq0 = oq1 = hq = ok = ok0 = ok1 = ov = ov0 = ov1 = sq = sk = sv = 0
     if q is not None:
         hq = q.shape[1]
-        pq, oq = _rows(q, "q", n, hq, dim, in_type), _rows(q_out, "q_out", n, hq, dim, out_type, True)
-    ok = _NO_ROWS if k_out is None else _rows(k_out, "k_out", n, heads, dim, out_type, True)
-    ov = _NO_ROWS if v_out is None else _rows(v_out, "v_out", n, heads, dim, out_type, True)
-    half = 0 if inv_freq is None else inv_freq.shape[0]
-    steps = (0, 0, 0)
+        pq, pq0, pq1 = _rows(q, "q", n, hq, dim, in_type)
+        _need(q_out is not None, "q and q_out come together")
+        oq, oq0, oq1 = _rows(q_out, "q_out", n, hq, dim, out_type, True)
+    elif q_out is not None:
+        _need(False, "q and q_out come together")
+    if k_out is not None:
+        ok, ok0, ok1 = _rows(k_out, "k_out", n, heads, dim, out_type, True)
+    if v_out is not None:
+        ov, ov0, ov1 = _rows(v_out, "v_out", n, heads, dim, out_type, True)
     if in_type == TYPE_S32:
-        _need(k_step is not None and v_step is not None and (q is None or q_step is not None), "int32 rows without steps")
-        steps = (_vector(q_step, "q_step", hq * dim, TYPE_F32), _vector(k_step, "k_step", heads * dim, TYPE_F32),
-                 _vector(v_step, "v_step", heads * dim, TYPE_F32))
-    else:
-        _need(q_step is None and k_step is None and v_step is None, "steps are for int32 rows")
-    _need(half == 0 or positions is not None, "a rotation without positions")
+        _need(k_step is not None and v_step is not None and (q is None or q_step is not None), "int32 rows have steps")
+        sq, sk, sv = (_vector(q_step, "q_step", hq * dim, TYPE_F32), _vector(k_step, "k_step", heads * dim, TYPE_F32),
+                      _vector(v_step, "v_step", heads * dim, TYPE_F32))
+    elif q_step is not None or k_step is not None or v_step is not None:
+        _need(False, "steps are for int32 rows")
+    at = angles = half = 0
+    if inv_freq is not None:
+        half = inv_freq.shape[0]
+        _need(positions is not None or half == 0, "a rotation has positions")
+        angles = _vector(inv_freq, "inv_freq", half, _TYPE_F64)
+    if positions is not None:
+        at = _vector(positions, "positions", n, TYPE_S32)
     _append_call(cache.block, _append_pack(
-        pq[0], pk[0], pv[0], oq[0], ok[0], ov[0], *steps, _vector(slots, "slots", n, _TYPE_S64),
-        _vector(positions, "positions", n, TYPE_S32), _vector(inv_freq, "inv_freq", half, _TYPE_F64), pq[1], pq[2], pk[1], pk[2],
-        pv[1], pv[2], oq[1], oq[2], ok[1], ok[2], ov[1], ov[2], n, hq, 2 * half, 1 if interleaved else 0, in_type, out_type))
+        pq, pk, pv, oq, ok, ov, sq, sk, sv, _vector(slots, "slots", n, _TYPE_S64), at, angles, pq0, pq1, pk0, pk1, pv0, pv1,
+        oq0, oq1, ok0, ok1, ov0, ov1, n, hq, 2 * half, 1 if interleaved else 0, in_type, out_type))
 
 
 def pulpnn_kv_gather(cache, slots, k_out, v_out=None):
@@ -549,10 +555,13 @@ def pulpnn_kv_gather(cache, slots, k_out, v_out=None):
         return
     first = k_out if k_out is not None else v_out
     _need(first is not None, "neither k_out nor v_out")
-    out_type = _type(first)
-    a, b = (_NO_ROWS if x is None else _rows(x, name, n, cache.n_heads, cache.head_dim, out_type, True)
-            for x, name in ((k_out, "k_out"), (v_out, "v_out")))
-    _gather_call(cache.block, _gather_pack(_vector(slots, "slots", n, _TYPE_S64), a[0], b[0], a[1], a[2], b[1], b[2], n, out_type))
+    out_type, heads, dim = _type(first), cache.n_heads, cache.head_dim
+    a = a0 = a1 = b = b0 = b1 = 0
+    if k_out is not None:
+        a, a0, a1 = _rows(k_out, "k_out", n, heads, dim, out_type, True)
+    if v_out is not None:
+        b, b0, b1 = _rows(v_out, "v_out", n, heads, dim, out_type, True)
+    _gather_call(cache.block, _gather_pack(_vector(slots, "slots", n, _TYPE_S64), a, b, a0, a1, b0, b1, n, out_type))
 
 
 _decode_pack = struct.Struct("=5Q5q2f8i").pack
@@ -562,8 +571,8 @@ _decode_call = _StructCall("pulpnn_attn_decode", 2)
 def _out_type(out, in_type, out_step):
     """The type of an attention's output: the queries', or uint8 with a step."""
     type_ = _type(out)
-    _need(type_ == in_type or type_ == TYPE_U8, "out is neither of q's type nor uint8")
-    _need((type_ == TYPE_U8) == (out_step is not None), "uint8 outputs, and only these, have an out_step")
+    if type_ != in_type and type_ != TYPE_U8 or (type_ == TYPE_U8) != (out_step is not None):
+        _need(False, "out is of q's type, or uint8; uint8 outputs, and only these, have an out_step")
     return type_
 
 
@@ -576,20 +585,21 @@ def pulpnn_attn_decode(cache, q, block_table, seq_lens, out, scale=None, window=
         return
     q_type = _type(q)
     out_type = _out_type(out, q_type, out_step)
-    _need(dim == cache.head_dim, "q and the cache have different numbers of channels")
-    a, b = _rows(q, "q", n, heads, dim, q_type), _rows(out, "out", n, heads, dim, out_type, True)
-    _need(block_table.dim() == 2 and block_table.shape[0] == n and _type(block_table) == TYPE_S32, "block_table is int32 [sequences][pages]")
-    pages = block_table.shape[1]
-    _need(pages <= 1 or block_table.stride(1) == 1, "the pages of a sequence do not lie side by side in block_table")
+    if dim != cache.head_dim:
+        _need(False, "q and the cache have different numbers of channels")
+    pq, q0, q1 = _rows(q, "q", n, heads, dim, q_type)
+    po, o0, o1 = _rows(out, "out", n, heads, dim, out_type, True)
+    shape, strides = block_table.shape, block_table.stride()
+    if len(shape) != 2 or shape[0] != n or _type(block_table) != TYPE_S32 or (strides[1] != 1 and shape[1] > 1):
+        _need(False, "block_table is int32 [sequences][pages], the pages of a sequence side by side")
+    pages, lengths = shape[1], _vector(seq_lens, "seq_lens", n, TYPE_S32)
     _decode_call(cache.block, _decode_pack(
-        a[0], b[0], _lse(lse, n, heads), block_table.data_ptr() if pages else seq_lens.data_ptr(), _vector(seq_lens, "seq_lens", n, TYPE_S32),
-        a[1], a[2], b[1], b[2], block_table.stride(0) if n > 1 else 0, dim ** -0.5 if scale is None else scale,
-        out_step or 0., out_zero, q_type, out_type, n, heads, pages, window, 0))
+        pq, po, 0 if lse is None else _lse(lse, n, heads), block_table.data_ptr() if pages else lengths, lengths, q0, q1, o0, o1,
+        strides[0] if n > 1 else 0, dim ** -0.5 if scale is None else scale, out_step or 0., out_zero, q_type, out_type, n, heads, pages,
+        window, 0))
 
 
 def _lse(lse, n, heads):
-    if lse is None:
-        return 0
     _need(lse.shape == (n, heads) and lse.is_contiguous() and _type(lse) == TYPE_F32, "lse is float32 [rows][heads] in one piece")
     return lse.data_ptr()
 
@@ -608,17 +618,18 @@ def pulpnn_attn_prompt(q, k, v, cu_q, out, cu_k=None, causal=True, window=0, sca
     nk, kv_heads = k.shape[0], k.shape[1]
     type_ = _type(q)
     out_type = _out_type(out, type_, out_step)
-    rows = [_rows(q, "q", n, heads, dim, type_), _rows(k, "k", nk, kv_heads, dim, type_), _rows(v, "v", nk, kv_heads, dim, type_),
-            _rows(out, "out", n, heads, dim, out_type, True)]
+    pq, q0, q1 = _rows(q, "q", n, heads, dim, type_)
+    pk, k0, k1 = _rows(k, "k", nk, kv_heads, dim, type_)
+    pv, v0, v1 = _rows(v, "v", nk, kv_heads, dim, type_)
+    po, o0, o1 = _rows(out, "out", n, heads, dim, out_type, True)
     seqs = cu_q.shape[0] - 1
     if cu_k is None:
         _need(nk == n, "other numbers of rows of keys than of queries, and no cu_k")
         cu_k = cu_q
     _prompt_call(_prompt_pack(
-        rows[0][0], rows[1][0], rows[2][0], rows[3][0], _lse(lse, n, heads), _vector(cu_q, "cu_q", seqs + 1, TYPE_S32),
-        _vector(cu_k, "cu_k", seqs + 1, TYPE_S32), rows[0][1], rows[0][2], rows[1][1], rows[1][2], rows[2][1], rows[2][2], rows[3][1],
-        rows[3][2], dim ** -0.5 if scale is None else scale, out_step or 0., out_zero, type_, out_type, n, nk, seqs, heads, kv_heads, dim,
-        1 if causal else 0, window, 0))
+        pq, pk, pv, po, 0 if lse is None else _lse(lse, n, heads), _vector(cu_q, "cu_q", seqs + 1, TYPE_S32),
+        _vector(cu_k, "cu_k", seqs + 1, TYPE_S32), q0, q1, k0, k1, v0, v1, o0, o1, dim ** -0.5 if scale is None else scale,
+        out_step or 0., out_zero, type_, out_type, n, nk, seqs, heads, kv_heads, dim, 1 if causal else 0, window, 0))
 
 
 # ---- network runner --------------------------------------------------------------------------

@@ -103,9 +103,9 @@ __device__ __forceinline__ unsigned code(float x, float inv) { return __float_as
 // pair, whichever way they are paired, and 32-bit rows are read without gaps between the lanes. Otherwise eight side by side, whose
 // mates come from another lane, or one by one where they are not eight side by side either.
 template <typename IN, typename WIDE, bool EIGHT, bool HALVES>
-__global__ void __launch_bounds__(WARPS * 32, Width<IN>::v == 2 ? 8 : 6) kv_append_kernel(const AppendProblem p)
+__global__ void __launch_bounds__(WARPS * 32, Width<IN>::v == 2 ? 10 : 8) kv_append_kernel(const AppendProblem p)
 {
-  constexpr int SIZE = Width<IN>::v, BATCH = SIZE == 2 ? 4 : 3;
+  constexpr int SIZE = Width<IN>::v, BATCH = SIZE == 2 ? 4 : 2;
   __shared__ __align__(16) float2 turns[MOST_TOKENS][MAX_HEAD_DIM / 2];
   __shared__ longlong2 where[MOST_TOKENS];      // of a token's head 0: its row's and its scale's place in the cache; -1: it is not stored
   const int which = blockIdx.x < p.blocks[0] ? 0 : (blockIdx.x < p.blocks[0] + p.blocks[1] ? 1 : 2);
@@ -283,7 +283,7 @@ template <typename IN, typename WIDE, bool EIGHT>
 cudaError_t append_go(AppendProblem &p, int sms, cudaStream_t s)
 {
   // tokens of a block: for BATCH rows a thread where there are blocks enough, else one
-  const int rows = WARPS * p.per_warp * (Width<IN>::v == 2 ? 4 : 3);
+  const int rows = WARPS * p.per_warp * (Width<IN>::v == 2 ? 4 : 2);
   unsigned blocks = 0;
   for (int i = 0; i < 3; i++) {
     p.tokens[i] = 1; p.blocks[i] = 0;
@@ -321,7 +321,7 @@ struct GatherProblem {
 template <typename WIDE, bool EIGHT>
 __global__ void __launch_bounds__(THREADS) kv_gather_kernel(const GatherProblem p)
 {
-  constexpr int BATCH = 4;
+  constexpr int BATCH = 2;                 // of 100003 rows of 8 heads: 106 us; one 114, four 114
   const int sub = threadIdx.x / p.chunks, chunk = threadIdx.x - sub * p.chunks, which = p.out[0] ? blockIdx.y : 1;
   const char *from = which == 0 ? p.cache.k : p.cache.v;
   const float *scales = which == 0 ? p.cache.k_scale : p.cache.v_scale;
@@ -377,7 +377,7 @@ cudaError_t gather_go(GatherProblem &p, cudaStream_t s)
   p.whole = 1;
   for (int i = 0; i < 2; i++)
     if (p.out[i] && (!aligned(p.out[i], 32) || p.out_token[i] % 32 || p.out_head[i] % 32)) p.whole = 0;
-  const int64_t rows = (int64_t)p.n * p.heads, per = 4 * p.per_block;
+  const int64_t rows = (int64_t)p.n * p.heads, per = 2 * p.per_block;
   const dim3 grid((unsigned)((rows + per - 1) / per), p.out[0] && p.out[1] ? 2 : 1);
   return launch_pdl(kv_gather_kernel<WIDE, EIGHT>, grid, dim3(THREADS), 0, s, p);
 }
