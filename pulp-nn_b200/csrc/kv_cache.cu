@@ -46,7 +46,7 @@ struct AppendProblem {
   CacheView cache;
   int n, heads[3], tokens[3], blocks[3];                 // of q, k, v: heads; tokens of a block; blocks
   FastDiv by_heads[3];
-  int dim, half, interleaved, chunks, pow2, per_warp;                       // chunks of 8 channels in a row; rows of a warp
+  int dim, half, interleaved, chunks, pow2, narrow, per_warp;                       // chunks of 8 channels in a row; rows of a warp
 };
 
 struct S32 {};
@@ -102,7 +102,12 @@ __device__ __forceinline__ unsigned code(float x, float inv) { return __float_as
 // HALVES (all channels rotate, or none): a lane's eight channels are four of each half of the row, so that it has both of every
 // pair, whichever way they are paired, and 32-bit rows are read without gaps between the lanes. Otherwise eight side by side, whose
 // mates come from another lane, or one by one where they are not eight side by side either.
-template <typename IN, typename WIDE, bool EIGHT, bool HALVES>
+// NARROW: what a block's rows lie apart fits 32 bits, as it nearly always does; products of 64 bits were a fifth of the instructions.
+template <bool NARROW> __device__ __forceinline__ int64_t apart(int a, int64_t sa, int b, int64_t sb)
+{
+  return NARROW ? (int64_t)(a * (int)sa + b * (int)sb) : a * sa + b * sb;
+}
+template <typename IN, typename WIDE, bool EIGHT, bool HALVES, bool NARROW>
 __global__ void __launch_bounds__(WARPS * 32, Width<IN>::v == 2 ? 10 : 8) kv_append_kernel(const AppendProblem p)
 {
   constexpr int SIZE = Width<IN>::v, BATCH = SIZE == 2 ? 4 : 2;
@@ -133,7 +138,7 @@ __global__ void __launch_bounds__(WARPS * 32, Width<IN>::v == 2 ? 10 : 8) kv_app
       live[b] = sub < p.per_warp && row < rows;
       token[b] = by_heads.div(row); head[b] = row - token[b] * heads;
       if (live[b]) {
-        const char *src = in + token[b] * in_token + head[b] * in_head;
+        const char *src = in + apart<NARROW>(token[b], in_token, head[b], in_head);
         if (!HALVES && SIZE == 2) {
           const uint4 both = *reinterpret_cast<const uint4 *>(src + c0 * SIZE);
           reinterpret_cast<uint2 &>(lo[b]) = make_uint2(both.x, both.y); reinterpret_cast<uint2 &>(hi[b]) = make_uint2(both.z, both.w);
@@ -235,11 +240,11 @@ __global__ void __launch_bounds__(WARPS * 32, Width<IN>::v == 2 ? 10 : 8) kv_app
           *reinterpret_cast<uint4 *>(row + c0 * 2) = make_uint4(wide0.x, wide0.y, wide1.x, wide1.y);
         }
       };
-      if (live[b] && out) put(out + token[b] * out_token + head[b] * out_head);
+      if (live[b] && out) put(out + apart<NARROW>(token[b], out_token, head[b], out_head));
       if (which == 0) continue;
       const longlong2 at = where[k];
       const bool stored = live[b] && at.x >= 0;
-      const int64_t place = at.x + head[b] * p.cache.head_stride;
+      const int64_t place = at.x + apart<NARROW>(head[b], p.cache.head_stride, 0, 0);
       if (EIGHT) {
         float most = 0.f;
 #pragma unroll
@@ -293,8 +298,10 @@ cudaError_t append_go(AppendProblem &p, int sms, cudaStream_t s)
     p.blocks[i] = (p.n + p.tokens[i] - 1) / p.tokens[i];
     blocks += (unsigned)p.blocks[i];
   }
-  return p.half == 0 || 2 * p.half == p.dim ? launch_pdl(kv_append_kernel<IN, WIDE, EIGHT, true>, dim3(blocks), dim3(WARPS * 32), 0, s, p)
-                                            : launch_pdl(kv_append_kernel<IN, WIDE, EIGHT, false>, dim3(blocks), dim3(WARPS * 32), 0, s, p);
+  const bool halves = p.half == 0 || 2 * p.half == p.dim;
+  auto k = p.narrow ? (halves ? kv_append_kernel<IN, WIDE, EIGHT, true, true> : kv_append_kernel<IN, WIDE, EIGHT, false, true>)
+                    : (halves ? kv_append_kernel<IN, WIDE, EIGHT, true, false> : kv_append_kernel<IN, WIDE, EIGHT, false, false>);
+  return launch_pdl(k, dim3(blocks), dim3(WARPS * 32), 0, s, p);
 }
 template <typename WIDE, bool EIGHT>
 cudaError_t append_in(int in_type, AppendProblem &p, int sms, cudaStream_t s)
@@ -437,6 +444,14 @@ extern "C" int pulpnn_kv_append(const pulpnn_kv_cache_t *cache, const pulpnn_kv_
   p.cache = view_of(*cache);
   p.n = a->n_tokens; p.heads[0] = a->q ? a->n_q_heads : 0; p.heads[1] = p.heads[2] = cache->n_heads; p.dim = cache->head_dim;
   p.half = a->rotary_dim / 2; p.interleaved = a->interleaved != 0;
+  // the furthest apart that rows of a block can be
+  auto near = [](int64_t token, int64_t head, int heads) {
+    auto size = [](int64_t x) { return (double)(x < 0 ? -x : x); };
+    return size(token) * MOST_TOKENS + size(head) * heads < 2147483647.0;
+  };
+  p.narrow = near(0, cache->head_stride, cache->n_heads);
+  for (int i = 0; i < 3; i++)
+    p.narrow = p.narrow && near(p.in_token[i], p.in_head[i], p.heads[i]) && (!p.out[i] || near(p.out_token[i], p.out_head[i], p.heads[i]));
   p.chunks = p.dim / 8; p.pow2 = (p.chunks & (p.chunks - 1)) == 0; p.per_warp = 32 / p.chunks;
   const bool f16 = a->out_type == PULPNN_TYPE_F16;
   const cudaError_t e = cache->type == PULPNN_TYPE_S8

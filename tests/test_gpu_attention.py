@@ -163,6 +163,28 @@ def test_append_in_place_and_without_queries():
     assert torch.equal(c.rows(0, slots), k1.double())
 
 
+def test_append_and_gather_with_strides_beyond_32_bits():
+    """Tokens 1 GB apart, in what is read and in what is written."""
+    g = gen(16)
+    n, far = 5, 2 ** 29
+    wide = torch.empty(n * far, dtype=BF16, device="cuda")
+    view = lambda at: wide[at:].as_strided((n, 2, 64), (far, 64, 1))  # noqa: E731
+    q, k, v, k_out = (view(at) for at in (0, 256, 512, 768))
+    for t in (q, k, v):
+        t.copy_(normal(g, n, 2, 64))
+    q0, k0, v0 = (t.double().clone() for t in (q, k, v))
+    pos = torch.arange(n, device="cuda", dtype=torch.int32) + 70000
+    slots = torch.arange(n, device="cuda") + 3
+    c = Cache(g, BF16, 1, 8, 2, 64, False)
+    api.pulpnn_kv_append(c.handle, slots, k, v, positions=pos, inv_freq=freqs(64), q=q, q_out=q)
+    api.pulpnn_kv_gather(c.handle, slots, k_out)
+    torch.cuda.synchronize()
+    for got, raw in ((q, q0), (k_out, k0), (c.rows(0, slots), k0)):
+        want = rotate(raw, pos, freqs(64), False)
+        assert ((got.double() - want).abs() <= eps(BF16) / 2 * want.abs() + 2.0 ** -19 * raw.abs().amax()).all()
+    assert torch.equal(c.rows(1, slots), v0) and torch.equal(v.double(), v0)
+
+
 def test_append_rows_that_8_bits_cannot_hold():
     """Zeros and the smallest rows become 0, a row with an infinity or a NaN becomes NaN, the next row is unaffected."""
     g = gen(4)
