@@ -33,25 +33,8 @@ inline bool is_wide(int type) { return type == PULPNN_TYPE_F16 || type == PULPNN
     }                                       \
   } while (0)
 
-// A kernel that reads a host pointer faults, and one that reads another GPU's memory may: neither is launched.
-inline bool on_device(const Context &c, const char *who, std::initializer_list<const void *> pointers)
-{
-  for (const void *p : pointers) {
-    if (!p) continue;
-    cudaPointerAttributes a;
-    if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
-      cudaGetLastError();
-      set_error(PULPNN_ERR_INVALID_ARG, "%s: %p is not an address CUDA knows", who, p);
-      return false;
-    }
-    if (a.type == cudaMemoryTypeManaged) continue;
-    if (a.type != cudaMemoryTypeDevice || a.device != c.device) {
-      set_error(PULPNN_ERR_INVALID_ARG, "%s: %p is not memory of GPU %d", who, p, c.device);
-      return false;
-    }
-  }
-  return true;
-}
+// A kernel that reads a host pointer faults, and one that reads another GPU's memory may: neither is launched. (In kv_cache.cu.)
+bool on_device(const Context &c, const char *who, std::initializer_list<const void *> pointers);
 
 inline bool aligned(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (unsigned)(bytes - 1)) == 0; }
 // rows of `size`-byte elements at these strides begin on 16-byte boundaries

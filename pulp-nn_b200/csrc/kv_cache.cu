@@ -4,10 +4,54 @@
 // Both move bytes: 48 rows of 128 channels a token at 32 query and 8 key heads, some 4 operations a channel. A warp of the
 // append holds whole rows, as many as fit at 8 channels a lane (3 of 80 channels), so that it loads and stores them in
 // 16-byte pieces and a row's largest value is 4 shuffles away.
+#include <cuda.h>
+
 #include "attention.cuh"
 
 namespace pulpnn {
 namespace attn {
+
+typedef CUresult (*PointerAttributeFn)(void *, CUpointer_attribute, CUdeviceptr);
+
+bool on_device(const Context &c, const char *who, std::initializer_list<const void *> pointers)
+{
+  // one attribute of the driver's takes half the time of the runtime's whole answer, and a call has up to thirteen pointers
+  static PointerAttributeFn attribute = [] {
+    void *f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuPointerGetAttribute", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      f = nullptr;
+    }
+    return reinterpret_cast<PointerAttributeFn>(f);
+  }();
+  static const int devices = [] {
+    int n = 0;
+    if (cudaGetDeviceCount(&n) != cudaSuccess) cudaGetLastError();
+    return n;
+  }();
+  for (const void *p : pointers) {
+    if (!p) continue;
+    unsigned type = 0;
+    int device = c.device;
+    const CUdeviceptr at = reinterpret_cast<CUdeviceptr>(p);
+    if (attribute && attribute(&type, CU_POINTER_ATTRIBUTE_MEMORY_TYPE, at) == CUDA_SUCCESS && type == CU_MEMORYTYPE_DEVICE &&
+        (devices == 1 || (attribute(&device, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, at) == CUDA_SUCCESS && device == c.device)))
+      continue;
+    cudaPointerAttributes a;
+    if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
+      cudaGetLastError();
+      set_error(PULPNN_ERR_INVALID_ARG, "%s: %p is not an address CUDA knows", who, p);
+      return false;
+    }
+    if (a.type == cudaMemoryTypeManaged) continue;
+    if (a.type != cudaMemoryTypeDevice || a.device != c.device) {
+      set_error(PULPNN_ERR_INVALID_ARG, "%s: %p is not memory of GPU %d", who, p, c.device);
+      return false;
+    }
+  }
+  return true;
+}
 
 int check_cache(const char *who, const pulpnn_kv_cache_t *c)
 {
