@@ -51,6 +51,7 @@ struct PromptProblem {
   const int *cu_q, *cu_k;
   int64_t v_row, v_head, out_row, out_head;       // bytes
   FastDiv by_group;
+  int units;                                      // of an item: 2, or 1 where there are fewer than half as many units as SMs
   int nq, nk, seqs, hq, group, dim, causal, window, out_type, out_zero;
   float scale_log2, out_inv_step;
   int *status;
@@ -175,10 +176,10 @@ __device__ __forceinline__ void make_work(Work &w, int q0, int lq, int k0, int l
   w.q0 = q0; w.k0 = k0; w.lk = lk; w.kvh = kvh;
   w.lo = 0x7fffffff; w.hi = 0;
   for (int x = 0; x < 2; x++) {
-    const int n = 2 * pair + x, rt = p.by_group.div(n);
+    const int n = p.units * pair + x, rt = p.by_group.div(n);
     Unit u;
     u.row0 = rt * BQ; u.head = kvh * p.group + n - rt * p.group;
-    u.rows = min(max(lq - u.row0, 0), BQ);
+    u.rows = x < p.units ? min(max(lq - u.row0, 0), BQ) : 0;
     u.pos = u.row0 + lk - lq;
     const int keys = u.rows == 0 ? 0 : (p.causal ? min(lk, max(u.pos + u.rows, 0)) : lk);       // it sees none from here on
     const int from = p.window > 0 ? max(0, u.pos - p.window + 1) : 0;
@@ -216,7 +217,7 @@ __device__ __forceinline__ bool find_item(const PromptProblem &p, int x, int y, 
 #pragma unroll
     for (int k = 0; k < 8; k++) {
       const int tiles = b0 + k < p.seqs ? (max(at[k + 1] - at[k], 0) + BQ - 1) / BQ : 0;
-      count[k] = (int)(((int64_t)tiles * p.group + 1) / 2);
+      count[k] = (int)(((int64_t)tiles * p.group + p.units - 1) >> (p.units - 1));
       sum += count[k];
     }
     int incl = sum;
@@ -878,8 +879,10 @@ extern "C" int pulpnn_attn_prompt(const pulpnn_attn_prompt_t *a)
   } else {
     mk = mv = mq;
   }
-  // at most this many pairs of units: a sequence's rows fill all its tiles but one, and a pair may be half empty
-  const int64_t pairs = (((int64_t)a->n_q_rows / BQ + a->n_seqs) * p.group + a->n_seqs + 1) / 2;
+  // at most so many units: a sequence's rows fill all its tiles but one; and items, of which a sequence's last may be half empty
+  const int64_t units = ((int64_t)a->n_q_rows / BQ + a->n_seqs) * p.group;
+  p.units = units * a->n_kv_heads <= c.sm_count ? 1 : 2;
+  const int64_t pairs = p.units == 1 ? units : (units + a->n_seqs + 1) / 2;
   ATTN_REQUIRE(pairs <= 0x3fffffff, PULPNN_ERR_UNSUPPORTED, "%s: %d rows in %d sequences", who, a->n_q_rows, a->n_seqs);
   const dim3 grid((unsigned)pairs, (unsigned)a->n_kv_heads);
   const bool f16 = a->type == PULPNN_TYPE_F16, narrow = a->head_dim <= 64;
