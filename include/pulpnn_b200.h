@@ -73,6 +73,7 @@ enum {
   PULPNN_OPT_FORCE_GENERIC = 1,   /* route contractions to the generic CUDA-core kernel      */
   PULPNN_OPT_MAXPOOL_CLOBBER = 2, /* also reproduce the reference's overwrite of Im_in       */
   PULPNN_OPT_SPLIT_K = 3,         /* 0 = choose automatically, n > 0 = force n K-slices      */
+                                  /* (pulpnn_attn_decode: n CTAs for a sequence)             */
   PULPNN_OPT_FUSE_DWPW = 4,       /* network runner: run a 3x3 stride-1 depthwise layer and   */
                                   /* the pointwise layer behind it as ONE kernel where a      */
                                   /* fused kernel exists (default 1); results are identical   */
@@ -335,7 +336,7 @@ typedef struct {
  * S8 codes rint(x * 127 / max|x|) with the scale max|x| / 127 (rows below 2^-100 become 0; a row with a NaN or an
  * infinity gets the scale NaN). k_out and v_out (may be NULL) receive the rows before they are cut to 8 bits.
  *
- *  - in_type: F16, BF16, F32 or S32. out_type: F16 or BF16, of q_out, k_out and v_out; a 16-bit cache has the same.
+ *  - in_type: F16, BF16, F32 or S32. out_type: F16 or BF16, of q_out, k_out and v_out, whatever the cache holds.
  *  - q may be NULL (with q_out); positions and inv_freq may be NULL where rotary_dim is 0 (even, at most head_dim).
  *  - q_out may be q (k_out k, v_out v) with the same strides and a type of the same size; other overlaps are undefined.
  *  - A token whose slot lies outside the cache (-1: padding) is not stored; its q_out, k_out, v_out are written.

@@ -506,15 +506,14 @@ def pulpnn_kv_append(cache, slots, k, v, positions=None, inv_freq=None, interlea
                      v_out=None, q_step=None, k_step=None, v_step=None):
     """Rotates q and k ([tokens][heads][dim]; float16, bfloat16, float32, or int32 with a float32 step per channel) by
     positions (int32) x inv_freq (float64, half as many as channels rotate), writes q to q_out and stores k and v in the
-    cache at slots (int64; one outside the cache stores nothing). k_out, v_out: the stored rows before a cut to 8 bits."""
+    cache at slots (int64; one outside the cache stores nothing). k_out, v_out: the stored rows before a cut to 8 bits.
+    The outputs are float16 or bfloat16, all of one type, which need not be the cache's."""
     n, heads, dim = k.shape[0], cache.n_heads, cache.head_dim
     if n == 0:
         return
     in_type = _type(k)
-    out_type = cache.type
-    if out_type == TYPE_S8:                     # the outputs' own; any, where nothing of that type is written
-        o = q_out if q_out is not None else k_out if k_out is not None else v_out
-        out_type = TYPE_BF16 if o is None else _type(o)
+    o = q_out if q_out is not None else k_out if k_out is not None else v_out
+    out_type = _type(o) if o is not None else cache.type if cache.type != TYPE_S8 else TYPE_BF16      # any, where no rows are written
     pk, pk0, pk1 = _rows(k, "k", n, heads, dim, in_type)
     pv, pv0, pv1 = _rows(v, "v", n, heads, dim, in_type)
     pq = pq0 = pq1 = oq = oq0 = oq1 = hq = ok = ok0 = ok1 = ov = ov0 = ov1 = sq = sk = sv = 0

@@ -9,7 +9,7 @@
 //
 // One CTA an SM. It begins with the item of its own block index and takes further ones from blocks that have not
 // started yet (clusterlaunchcontrol), so that nothing is set up twice and no SM waits at the end of a fixed share; a
-// sequence's last rows, which see the most keys, come first.
+// sequence's last rows, which see the most keys, come first. Where there are no more units than SMs, each is an item.
 //
 //   warps 0-3, 4-7  softmax of unit 0 and 1: a thread is a row. S comes from TMEM, the weights go back there as the 16-bit
 //                   operand of the second product. At an item's end they also write its rows.
@@ -30,6 +30,11 @@
 //     halves, so that the first half's product runs under the second half's exponentials.
 // The running maximum is a reference that has to be near the true one only: it is taken from an item's first tile, and raised
 // (O being rescaled in TMEM by the softmax warps themselves) when a weight comes out above 2^15, which is rare.
+//
+// Measured (one B200): 16384 causal tokens, 32 query and 8 key heads of 128 channels in bf16, 1860 us in a burst (1180 of the
+// 1670 TFLOP/s that a plain matrix product reaches), 2090 in a long run at the power limit; 24 packed prompts of 28 heads of 64
+// channels 245 us, where the exponentials alone take 82 and the matrix products 57; 300 tokens 12.9 us: the set-up, three
+// key tiles one after the other and the epilogue.
 #include "attention.cuh"
 #include "sm100_primitives.cuh"
 
@@ -51,7 +56,7 @@ struct PromptProblem {
   const int *cu_q, *cu_k;
   int64_t v_row, v_head, out_row, out_head;       // bytes
   FastDiv by_group;
-  int units;                                      // of an item: 2, or 1 where there are fewer than half as many units as SMs
+  int units;                                      // of an item: 2, or 1 where all of them find an SM at once
   int nq, nk, seqs, hq, group, dim, causal, window, out_type, out_zero;
   float scale_log2, out_inv_step;
   int *status;
@@ -334,7 +339,7 @@ __device__ __noinline__ bool wait_long(uint64_t *bar, uint32_t parity, volatile 
   return mbar_wait(bar, parity, abort_flag, status, code);
 }
 
-// Warp 17: issues the MMAs. The whole warp walks through the tiles, so that what the instructions take from uniform
+// Warp 9: issues the MMAs. The whole warp walks through the tiles, so that what the instructions take from uniform
 // registers is computed there; one lane issues and commits.
 template <typename T, int DP>
 __device__ __forceinline__ void mma_warp(Control &ct, uint32_t base, uint32_t tmem_, const PromptProblem &p)
@@ -881,6 +886,7 @@ extern "C" int pulpnn_attn_prompt(const pulpnn_attn_prompt_t *a)
   }
   // at most so many units: a sequence's rows fill all its tiles but one; and items, of which a sequence's last may be half empty
   const int64_t units = ((int64_t)a->n_q_rows / BQ + a->n_seqs) * p.group;
+  // one unit an item where that still fits the GPU at once: 300 tokens of 32 heads take 12.9 us, 13.9 in pairs
   p.units = units * a->n_kv_heads <= c.sm_count ? 1 : 2;
   const int64_t pairs = p.units == 1 ? units : (units + a->n_seqs + 1) / 2;
   ATTN_REQUIRE(pairs <= 0x3fffffff, PULPNN_ERR_UNSUPPORTED, "%s: %d rows in %d sequences", who, a->n_q_rows, a->n_seqs);

@@ -64,7 +64,8 @@ def test_append():
     refused(INVALID, call, c, n.to(S32), k, k)
     refused(INVALID, call, c, n[:2], k, k)
     refused(INVALID, call, c, n, k, k, q=rows(3, 4, 64))
-    refused(INVALID, call, c, n, k, k, q=rows(3, 4, 64), q_out=rows(3, 4, 64, F16))
+    refused(INVALID, call, c, n, k, k, q=rows(3, 4, 64), q_out=rows(3, 4, 64, F32))
+    refused(INVALID, call, c, n, k, k, q=rows(3, 4, 64), q_out=rows(3, 4, 64, F16), k_out=k)
     refused(INVALID, call, c, n, k, k, q=rows(3, 4, 64), q_out=rows(1, 4, 64).expand(3, 4, 64))
     refused(INVALID, call, c, n, k, k, inv_freq=torch.ones(32, dtype=torch.float64))
     refused(INVALID, call, c, n, k, k, inv_freq=torch.ones(32), positions=n.to(S32))
@@ -110,6 +111,12 @@ def test_decode():
     refused(INVALID, call, c, q, table, lens, q, lse=torch.zeros(3, 5))
     refused(INVALID, call, c, q, table, lens, q, lse=torch.zeros(3, 4, dtype=F16))
     call(c, q[:0], table[:0], lens[:0], q[:0])
+
+
+def test_decode_of_tables_for_2_31_tokens():
+    # 524273 pages of 4096 slots: 2^31 - 61440 tokens, which a few tiles more would carry beyond 31 bits
+    c, q = cache(pages=1, page=4096, heads=1, dim=8), rows(1, 1, 8)
+    refused(UNSUPPORTED, api.pulpnn_attn_decode, c, q, torch.zeros(1, 524273, dtype=S32), torch.zeros(1, dtype=S32), q.clone())
 
 
 def test_prompt():

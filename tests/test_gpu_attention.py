@@ -76,7 +76,7 @@ def freqs(rot):
 # ---- append and gather --------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("in_type,wide,cache", [(BF16, BF16, BF16), (F16, F16, S8), (F32, F16, F16), (S32, BF16, S8), (BF16, BF16, S8),
-                                                (S32, F16, F16), (F32, BF16, S8)])
+                                                (S32, F16, F16), (F32, BF16, S8), (S32, BF16, F16), (BF16, F16, BF16)])
 @pytest.mark.parametrize("n,hq,hkv,dim,rot,interleaved,heads_first,page", [
     (1, 4, 1, 128, 128, False, False, 16), (37, 3, 3, 80, 32, True, True, 20), (5, 7, 1, 64, 64, False, True, 1),
     (19, 2, 2, 112, 20, False, False, 7), (9, 1, 1, 16, 10, True, False, 16), (700, 4, 2, 32, 0, False, False, 33),
