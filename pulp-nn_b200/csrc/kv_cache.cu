@@ -6,7 +6,7 @@
 // 16-byte pieces and a row's largest value is 4 shuffles away.
 //
 // Measured (one B200; the copy rate is 6.56 TB/s): 32-bit accumulators of 4096 tokens, 32 query and 8 key heads of 128 channels,
-// into an 8-bit cache and 16-bit rows, 34.6 us (4.9 TB/s; 25 M instructions, issue slots 73 % busy); 32768 tokens of 16 heads of
+// into an 8-bit cache and 16-bit queries, 34.6 us (4.1 TB/s; 25 M instructions, issue slots 73 % busy); 32768 tokens of 16 heads of
 // 80 channels in 16 bits, 32 of them rotated, 92 us in a burst (5.5 TB/s, issue slots 81 % busy: what is left is the rotation
 // and the cut themselves); 8 tokens 2.2 us. The gather of 100003 tokens of 8 heads of 128 channels out of 8 bits 107 us (5.8 TB/s).
 #include <cuda.h>
