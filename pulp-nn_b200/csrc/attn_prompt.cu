@@ -33,7 +33,7 @@
 //
 // Measured (one B200): 16384 causal tokens, 32 query and 8 key heads of 128 channels in bf16, 1860 us in a burst (1180 of the
 // 1670 TFLOP/s that a plain matrix product reaches), 2090 in a long run at the power limit; 24 packed prompts of 28 heads of 64
-// channels 245 us, where the exponentials alone take 82 and the matrix products 57; 300 tokens 12.9 us: the set-up, three
+// channels 215 us, where the exponentials alone take 82 and the matrix products 57; 300 tokens 12.9 us: the set-up, three
 // key tiles one after the other and the epilogue.
 #include "attention.cuh"
 #include "sm100_primitives.cuh"
@@ -207,10 +207,13 @@ __device__ __forceinline__ bool guarded(const Work &w, int j, const PromptProble
   return (sees(w.u[0], j) && masked(w.u[0], j, w.lk, p)) || (sees(w.u[1], j) && masked(w.u[1], j, w.lk, p));
 }
 
-// Finds pair number x of the units of all sequences. The search goes on where the last one stopped: `before` pairs lie
-// ahead of sequence s0. A whole warp; false where there are not so many pairs.
+// Finds pair number x of the units of all sequences, the longest first where there are up to 256 sequences (24 packed prompts of
+// 1 to 2048 tokens: 230 us where the sequences' order took 247, SMs waiting for one that began a long item last). Beyond that in the
+// sequences' order: the search goes on where the last one stopped, `before` pairs lie ahead of sequence s0. A whole warp; false
+// where there are not so many pairs.
 __device__ __forceinline__ bool find_item(const PromptProblem &p, int x, int y, int lane, int &s0, int &before, Item &it)
 {
+  const bool merged = p.seqs > 1 && p.seqs <= 256;
   for (; s0 < p.seqs; s0 += 256) {              // eight sequences a lane
     int at[9], at_k[9], count[8], sum = 0;
     const int b0 = s0 + lane * 8;
@@ -225,20 +228,44 @@ __device__ __forceinline__ bool find_item(const PromptProblem &p, int x, int y, 
       count[k] = (int)(((int64_t)tiles * p.group + p.units - 1) >> (p.units - 1));
       sum += count[k];
     }
+    // Of up to 256 sequences, pair v of each before pair v - 1 of any: as many pairs lie ahead of those numbered v as there are beyond
+    // v in all sequences together.
+    int v = 0;
+    if (merged) {
+      if ((unsigned)x >= __reduce_add_sync(0xffffffffu, (unsigned)sum)) return false;
+      int most = 0;
+#pragma unroll
+      for (int k = 0; k < 8; k++) most = max(most, count[k]);
+      int hi = __reduce_max_sync(0xffffffffu, most);
+      unsigned ahead = 0;
+      while (hi - v > 1) {               // the largest v with x < pairs numbered v and beyond
+        const int mid = (v + hi) >> 1;
+        unsigned n = 0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) n += max(count[k] - mid, 0);
+        n = __reduce_add_sync(0xffffffffu, n);
+        if ((unsigned)x < n) v = mid;
+        else { hi = mid; ahead = n; }
+      }
+      x -= (int)ahead; sum = 0;
+#pragma unroll
+      for (int k = 0; k < 8; k++) sum += count[k] > v;
+    }
     int incl = sum;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += v;
+      const int n = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += n;
     }
     int off = before + incl - sum, q0 = 0, lq = 0, k0 = 0, lk = 0, pair = -1;
 #pragma unroll
     for (int k = 0; k < 8; k++) {
-      if (x >= off && x < off + count[k]) {
+      const int n = merged ? count[k] > v : count[k];
+      if (x >= off && x < off + n) {
         // the last rows of a causal sequence see the most keys: they begin first
-        q0 = at[k]; lq = at[k + 1] - at[k]; k0 = at_k[k]; lk = max(at_k[k + 1] - at_k[k], 0); pair = count[k] - 1 - (x - off);
+        q0 = at[k]; lq = at[k + 1] - at[k]; k0 = at_k[k]; lk = max(at_k[k + 1] - at_k[k], 0); pair = merged ? v : count[k] - 1 - (x - off);
       }
-      off += count[k];
+      off += n;
     }
     const unsigned hit = __ballot_sync(0xffffffffu, pair >= 0);
     if (hit) {
@@ -246,6 +273,7 @@ __device__ __forceinline__ bool find_item(const PromptProblem &p, int x, int y, 
       __syncwarp();
       return true;
     }
+    if (merged) return false;
     before += __shfl_sync(0xffffffffu, incl, 31);
   }
   return false;
@@ -535,10 +563,15 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
       if (j >= whole_hi || j < whole_lo) {
         const int a = first - j * BK, b = last - j * BK;
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (int k = 0; k < 4; k++) {
+          // bit c: whether the row sees key 32 k + c of the tile. One test of a bit a score; two comparisons took the packed
+          // prompts above from 215 to 230 us
+          const int from = a - k * 32, to = b - k * 32;
+          const unsigned seen = (from <= 0 ? 0xffffffffu : (from < 32 ? 0xffffffffu << from : 0u)) & (to >= 31 ? 0xffffffffu : (to >= 0 ? 0xffffffffu >> (31 - to) : 0u));
 #pragma unroll
           for (int c = 0; c < 32; c++)
-            if (k * 32 + c < a || k * 32 + c > b) s[k][c] = 0xff800000u;
+            if (!(seen & (1u << c))) s[k][c] = 0xff800000u;
+        }
       }
       // A new reference: the maximum so far. O is rescaled where it holds something (`has`); its products have ended.
       auto raise = [&](bool has) {
@@ -633,7 +666,7 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
     }
     const bool live = r < w.rows;
     const int64_t row = it.w.q0 + w.row0 + r;
-    const float inv = l == 0.f ? 0.f : 1.f / l;         // a row that sees nothing is zero
+    const float inv = l == 0.f ? 0.f : 1.f / l;         // a row that sees nothing is zero: its O is, the guards having been over V
     char *dst = p.out + row * p.out_row + (int64_t)w.head * p.out_head;
     const bool dirty = any && *reinterpret_cast<const volatile int *>(&it.dirty);
     // 16-bit rows go through shared memory, 64 channels at a time, and leave as whole rows: stored by their own threads, each
@@ -646,7 +679,7 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
         tmem_ld_16(t_o + c * 16, o);
         tmem_wait_ld();
 #pragma unroll
-        for (int k = 0; k < 16; k++) y[k] = inv == 0.f ? 0.f : __uint_as_float(o[k]) * inv;
+        for (int k = 0; k < 16; k++) y[k] = __uint_as_float(o[k]) * inv;
       } else {
 #pragma unroll
         for (int k = 0; k < 16; k++) y[k] = 0.f;

@@ -631,6 +631,14 @@ def test_prompt_many_sequences():
     prompt_case(9, lens, [0] * 1000, 1, 1, 64, BF16)
 
 
+@pytest.mark.parametrize("seqs", [2, 3, 33, 255, 256, 257])
+@pytest.mark.parametrize("hq,hkv", [(7, 1), (2, 2)])
+def test_prompt_sequences_taken_longest_first_or_in_order(seqs, hq, hkv):
+    lens = [(b * 37) % 61 if b % 3 else (b * 131) % 400 for b in range(seqs)]
+    lens[-1] = 390
+    prompt_case(seqs, lens, [0] * seqs, hq, hkv, 64, BF16, pad=2)
+
+
 def test_prompt_offsets_that_make_no_sense_stay_inside():
     g = gen(20)
     q, k, v = (normal(g, 200, 1, 64, dtype=BF16) for _ in range(3))
