@@ -24,9 +24,9 @@
 //
 // Measured (one B200; the copy rate is 6.56 TB/s): 64 ragged sequences of up to 8192 tokens, 32 query and 8 key heads of 128
 // channels in 16 bits, 166 us (6.6 TB/s); 8 of 128k in 8 bits 330 us (6.5 TB/s; 178 M instructions, issue slots 56 % busy),
-// 375 in a long run, where the power limit lowers the clock; 200 with a window, heads of 80 channels, pages of 20 slots
-// 152 us (5.4 TB/s: the 16-byte copies' instructions); one of 131072 tokens and 8 heads 90 us (6.0 TB/s); one of 1000 tokens
-// 6.3 us, a chain of six round trips to memory and two cluster barriers.
+// 375 in a long run, where the power limit lowers the clock; 200 with a window of 1024, 16 heads of 80 channels, pages of 20
+// slots, 139 us (5.9 TB/s: 64 tiles a sequence, so that the CTAs' starts and joins show); one of 131072 tokens and 8 heads
+// 90 us (6.0 TB/s); one of 1000 tokens 6.3 us, a chain of six round trips to memory and two cluster barriers.
 //
 // Running maximum: the reference m only has to be near the true maximum, not equal to it. It is raised (and the sums
 // rescaled) when some score is more than 2^LAG above it, which one vote per tile finds out; the weights stay
@@ -127,12 +127,15 @@ __device__ __forceinline__ float load_q(const char *p, int type)
 }
 
 // Rows of 128 bytes (a box of 64 16-bit channels or of up to 128 8-bit ones), whose 16-byte chunks are swizzled by their row the way
-// TMA does it: eight rows of one chunk lie in different banks.
+// TMA does it: eight rows of one chunk lie in different banks. DENSE: rows as long as they are, two of eight in the same banks,
+// where a second box of 64 channels would be mostly empty: 41 KB a CTA instead of 66, five of them an SM instead of three
+// (the 200 sequences above: 139 us, 153 in two boxes).
 template <int DP, bool EIGHT> struct Tile {
   static constexpr int SIZE = EIGHT ? 1 : 2;
   static constexpr int TOKENS = EIGHT || DP <= 64 ? 32 : 16;
-  static constexpr int BOXES = EIGHT || DP <= 64 ? 1 : 2;
-  static constexpr int BOX = TOKENS * 128;                   // bytes
+  static constexpr bool DENSE = !EIGHT && DP == 80;
+  static constexpr int BOXES = EIGHT || DP <= 64 || DENSE ? 1 : 2;
+  static constexpr int BOX = TOKENS * (DENSE ? DP * 2 : 128);    // bytes
   static constexpr int CHUNKS = DP * SIZE / 16;              // of a row
   static constexpr int STAGE = 2 * BOXES * BOX;              // keys, values
   static constexpr int PIPE = WARPS * STAGES * STAGE;
@@ -140,6 +143,7 @@ template <int DP, bool EIGHT> struct Tile {
   // address of a 16-byte chunk of a token's row, from the tile's first byte
   static __device__ __forceinline__ uint32_t at(int token, int chunk)
   {
+    if (DENSE) return token * (DP * 2) + chunk * 16;
     return (BOXES > 1 ? (chunk >> 3) * BOX : 0) + token * 128 + (((chunk & 7) ^ (token & 7)) << 4);
   }
 };
@@ -369,9 +373,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       // a page's rows that are not this sequence's tokens: a weight of 0 does not keep an infinity or a NaN out of the sum
       if (!((live >> lane) & 1u) && lane < TL::TOKENS) {
 #pragma unroll
-        for (int b = 0; b < TL::BOXES; b++)
-#pragma unroll
-          for (int c = 0; c < 8; c++) sm100::sts128(vbase + b * TL::BOX + lane * 128 + c * 16, 0, 0, 0, 0);
+        for (int c = 0; c < TL::CHUNKS; c++) sm100::sts128(vbase + TL::at(lane, c), 0, 0, 0, 0);
       }
       sm100::fence_proxy_async();
       __syncwarp();
@@ -588,8 +590,9 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   cluster.sync();          // no CTA leaves while another reads its sums
 }
 
-// [n_pages][n_heads][page_size][dim] at the cache's strides, boxes of 128 bytes of `box` slots of one head, 128-byte swizzle
-bool make_cache_map(CUtensorMap *map, const pulpnn_kv_cache_t &c, const void *base, int box)
+// [n_pages][n_heads][page_size][dim] at the cache's strides, boxes of `box` slots of one head: of 128 bytes, 128-byte swizzle, or of
+// `dense` channels as they lie
+bool make_cache_map(CUtensorMap *map, const pulpnn_kv_cache_t &c, const void *base, int box, int dense)
 {
   sm100::EncodeTiledFn enc = sm100::encode_tiled_fn();
   if (!enc) { set_error(PULPNN_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver"); return false; }
@@ -599,9 +602,9 @@ bool make_cache_map(CUtensorMap *map, const pulpnn_kv_cache_t &c, const void *ba
   const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.page_size, (cuuint64_t)c.n_heads, (cuuint64_t)c.n_pages};
   const cuuint64_t strides[3] = {c.page_size > 1 ? (cuuint64_t)c.slot_stride * size : any, c.n_heads > 1 ? (cuuint64_t)c.head_stride * size : any,
                                  c.n_pages > 1 ? (cuuint64_t)c.page_stride * size : any};
-  const cuuint32_t boxes[4] = {(cuuint32_t)(eight ? 128 : 64), (cuuint32_t)box, 1, 1}, step[4] = {1, 1, 1, 1};
+  const cuuint32_t boxes[4] = {(cuuint32_t)(dense ? dense : eight ? 128 : 64), (cuuint32_t)box, 1, 1}, step[4] = {1, 1, 1, 1};
   const CUresult r = enc(map, eight ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, strides,
-                         boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                         boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE, dense ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) { set_error(PULPNN_ERR_CUDA, "cuTensorMapEncodeTiled (cache) failed with code %d", (int)r); return false; }
   return true;
@@ -674,6 +677,7 @@ bool decode_tiles(Context &c, const DecodeLaunch &d)
 template <typename T, bool EIGHT>
 bool decode_dim(Context &c, const DecodeLaunch &d)
 {
+  if (!EIGHT && d.p.dim > 64 && d.p.dim <= 80) return decode_tiles<T, 80, false>(c, d);
   return d.p.dim <= 64 ? decode_tiles<T, 64, EIGHT>(c, d) : (d.p.dim <= 96 ? decode_tiles<T, 96, EIGHT>(c, d) : decode_tiles<T, 128, EIGHT>(c, d));
 }
 
@@ -735,7 +739,8 @@ extern "C" int pulpnn_attn_decode(const pulpnn_kv_cache_t *cache, const pulpnn_a
   p.status = nullptr; p.sums = nullptr;
   if (tma) {
     if (!ctx_status_word_unless_capturing(c, &p.status)) return c.err;
-    if (!make_cache_map(&mk, *cache, cache->k, p.box) || !make_cache_map(&mv, *cache, cache->v, p.box)) return c.err;
+    const int dense = !eight && p.dim > 64 && p.dim <= 80 ? 80 : 0;
+    if (!make_cache_map(&mk, *cache, cache->k, p.box, dense) || !make_cache_map(&mv, *cache, cache->v, p.box, dense)) return c.err;
   }
   const DecodeLaunch d = {p, mk, mv, pairs, longest, tile, tma};
   const bool ok = eight ? decode_dim<__half, true>(c, d)

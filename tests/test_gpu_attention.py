@@ -301,6 +301,14 @@ def test_decode(q_type, cache, hq, hkv, dim, page, heads_first):
     decode_case(dim + hq, LENS, hq, hkv, dim, q_type, cache, page, heads_first)
 
 
+@pytest.mark.parametrize("dim", [72, 80, 88])
+@pytest.mark.parametrize("hq,hkv,page,heads_first,window", [(4, 4, 16, False, 0), (10, 1, 32, True, 0), (6, 2, 48, False, 77), (20, 2, 20, False, 0),
+                                                            (2, 2, 9, True, 130)])
+def test_decode_rows_as_long_as_they_are(dim, hq, hkv, page, heads_first, window):
+    """65 to 80 channels lie in shared memory without gaps, more in boxes of 64."""
+    decode_case(dim * 3 + hq, LENS, hq, hkv, dim, F16, F16, page, heads_first, window=window, extra_pages=1)
+
+
 @pytest.mark.parametrize("cache", [BF16, S8])
 @pytest.mark.parametrize("window", [1, 16, 100, 10 ** 9])
 def test_decode_window(cache, window):
