@@ -80,7 +80,7 @@ def freqs(rot):
 @pytest.mark.parametrize("n,hq,hkv,dim,rot,interleaved,heads_first,page", [
     (1, 4, 1, 128, 128, False, False, 16), (37, 3, 3, 80, 32, True, True, 20), (5, 7, 1, 64, 64, False, True, 1),
     (19, 2, 2, 112, 20, False, False, 7), (9, 1, 1, 16, 10, True, False, 16), (700, 4, 2, 32, 0, False, False, 33),
-    (3, 33, 2, 128, 126, False, False, 16)])
+    (3, 33, 2, 128, 126, False, False, 16), (5003, 5, 1, 32, 32, False, True, 64), (3001, 2, 3, 48, 14, True, False, 20)])
 def test_append(in_type, wide, cache, n, hq, hkv, dim, rot, interleaved, heads_first, page):
     g = gen(n * 131 + dim)
     pages = (n + 5) // page + 2
@@ -140,6 +140,12 @@ def test_append(in_type, wide, cache, n, hq, hkv, dim, rot, interleaved, heads_f
         rest[slots[stored]] = False
         now = c.rows(i - 1, torch.arange(pages * page, device="cuda"))
         assert torch.equal(now[rest], before[i - 1][rest])
+
+
+@pytest.mark.parametrize("in_type,wide,cache", [(BF16, BF16, BF16), (S32, F16, F16)])
+@pytest.mark.parametrize("dim,rot,interleaved", [(72, 72, False), (72, 72, True), (72, 24, True), (8, 8, False), (8, 0, False), (104, 2, True), (24, 16, False)])
+def test_append_an_odd_number_of_octets(in_type, wide, cache, dim, rot, interleaved):
+    test_append(in_type, wide, cache, 37, 3, 2, dim, rot, interleaved, True, 5)
 
 
 def test_append_in_place_and_without_queries():
