@@ -33,7 +33,7 @@
 //
 // Measured (one B200): 16384 causal tokens, 32 query and 8 key heads of 128 channels in bf16, 1860 us in a burst (1180 of the
 // 1670 TFLOP/s that a plain matrix product reaches), 2090 in a long run at the power limit; 24 packed prompts of 28 heads of 64
-// channels 215 us, where the exponentials alone take 82 and the matrix products 57; 300 tokens 12.9 us: the set-up, three
+// channels 209 us, where the exponentials alone take 82 and the matrix products 57; 300 tokens 12.0 us: the set-up, three
 // key tiles one after the other and the epilogue.
 #include "attention.cuh"
 #include "sm100_primitives.cuh"
@@ -672,7 +672,43 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
     // 16-bit rows go through shared memory, 64 channels at a time, and leave as whole rows: stored by their own threads, each
     // instruction would touch 32 rows (300 tokens of 32 heads: 4900 of 24000 cycles)
     const uint32_t stage = staging + warp * SH::STAGING;
-    for (int c = 0; c < groups; c++) {
+    // eight lanes write 64 channels of a row: rows 4 k + lane / 8 of the warp's 32
+    const int chunk = lane & 7;
+    auto store = [&](int c) {
+      const int channel = (c & ~3) * 16 + chunk * 8;
+      char *to = p.out + ((int64_t)it.w.q0 + w.row0 + (warp & 3) * 32) * p.out_row + (int64_t)w.head * p.out_head + channel * 2;
+      __syncwarp();
+      uint4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const int n = k * 4 + (lane >> 3);
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[k].x), "=r"(v[k].y), "=r"(v[k].z), "=r"(v[k].w) : "r"(stage + n * 128 + ((chunk ^ (n & 7)) << 4)) : "memory");
+      }
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const int n = k * 4 + (lane >> 3);
+        if ((warp & 3) * 32 + n < w.rows && channel < p.dim) *reinterpret_cast<uint4 *>(to + n * p.out_row) = v[k];
+      }
+      __syncwarp();
+    };
+    // By far the most items, without the tests below: packed prompts 209 us, 215 without this loop. (Two or four groups at a time cost
+    // the main loop its registers: 222, 272.)
+    const bool plain = any && !dirty && p.out_type != PULPNN_TYPE_U8;
+#pragma unroll 1
+    for (int c = 0; plain && c < groups; c++) {
+      uint32_t o[16];
+      tmem_ld_16(t_o + c * 16, o);
+      tmem_wait_ld();
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        uint32_t w4[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) w4[e] = pack2<T>(__uint_as_float(o[8 * k + 2 * e]) * inv, __uint_as_float(o[8 * k + 2 * e + 1]) * inv);
+        sts128(stage + lane * 128 + ((((c & 3) * 2 + k) ^ (lane & 7)) << 4), w4[0], w4[1], w4[2], w4[3]);
+      }
+      if ((c & 3) == 3 || c == groups - 1) store(c);
+    }
+    for (int c = plain ? groups : 0; c < groups; c++) {
       float y[16];
       if (any) {
         uint32_t o[16];
@@ -714,21 +750,9 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
       for (int k = 0; k < 2; k++)
         sts128(stage + lane * 128 + ((((c & 3) * 2 + k) ^ (lane & 7)) << 4), pack2<T>(y[8 * k], y[8 * k + 1]), pack2<T>(y[8 * k + 2], y[8 * k + 3]),
                pack2<T>(y[8 * k + 4], y[8 * k + 5]), pack2<T>(y[8 * k + 6], y[8 * k + 7]));
-      if ((c & 3) == 3 || c == groups - 1) {
-        __syncwarp();
-        const int chunk = lane & 7, channel = (c & ~3) * 16 + chunk * 8;
-        char *to = p.out + ((int64_t)it.w.q0 + w.row0 + (warp & 3) * 32) * p.out_row + (int64_t)w.head * p.out_head + channel * 2;
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-          const int n = k * 4 + (lane >> 3);
-          uint4 v;
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(stage + n * 128 + ((chunk ^ (n & 7)) << 4)) : "memory");
-          if ((warp & 3) * 32 + n < w.rows && channel < p.dim) *reinterpret_cast<uint4 *>(to + n * p.out_row) = v;
-        }
-        __syncwarp();
-      }
+      if ((c & 3) == 3 || c == groups - 1) store(c);
     }
-    if (live && p.lse) p.lse[row * p.hq + w.head] = (m + log2f(l)) * 0.69314718055994530942f;
+    if (live && p.lse) p.lse[row * p.hq + w.head] = (m + __log2f(l)) * 0.69314718055994530942f;      // l is about 1 or more, or 0: off by 2^-22
     tc_fence_before();          // O has been read: the next item's first P, behind this, lets it be written over
     __syncwarp();
     if (lane == 0) mbar_arrive(&ct.item_empty[i % ITEMS]);
@@ -919,7 +943,7 @@ extern "C" int pulpnn_attn_prompt(const pulpnn_attn_prompt_t *a)
   }
   // at most so many units: a sequence's rows fill all its tiles but one; and items, of which a sequence's last may be half empty
   const int64_t units = ((int64_t)a->n_q_rows / BQ + a->n_seqs) * p.group;
-  // one unit an item where that still fits the GPU at once: 300 tokens of 32 heads take 12.9 us, 13.9 in pairs
+  // one unit an item where that still fits the GPU at once: 300 tokens of 32 heads took 12.9 us, 13.9 in pairs
   p.units = units * a->n_kv_heads <= c.sm_count ? 1 : 2;
   const int64_t pairs = p.units == 1 ? units : (units + a->n_seqs + 1) / 2;
   ATTN_REQUIRE(pairs <= 0x3fffffff, PULPNN_ERR_UNSUPPORTED, "%s: %d rows in %d sequences", who, a->n_q_rows, a->n_seqs);
