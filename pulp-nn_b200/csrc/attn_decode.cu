@@ -25,7 +25,7 @@
 // Measured (one B200; the copy rate is 6.56 TB/s): 64 ragged sequences of up to 8192 tokens, 32 query and 8 key heads of 128
 // channels in 16 bits, 166 us (6.6 TB/s); 8 of 128k in 8 bits 330 us (6.5 TB/s; 178 M instructions, issue slots 56 % busy),
 // 375 in a long run, where the power limit lowers the clock; 200 with a window of 1024, 16 heads of 80 channels, pages of 20
-// slots, 139 us (5.9 TB/s: 64 tiles a sequence, so that the CTAs' starts and joins show); one of 131072 tokens and 8 heads
+// slots, 136 us (6.1 TB/s: 64 tiles a sequence, so that the CTAs' starts and joins show); one of 131072 tokens and 8 heads
 // 90 us (6.0 TB/s); one of 1000 tokens 6.3 us, a chain of six round trips to memory and two cluster barriers.
 //
 // Running maximum: the reference m only has to be near the true maximum, not equal to it. It is raised (and the sums
@@ -556,7 +556,9 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     *reinterpret_cast<float4 *>(cta_sums + head * JN::PITCH + ch) = acc;
     if (ch == 0) { cta_stats[head] = M; cta_stats[JN::HEADS + head] = L; cta_stats[2 * JN::HEADS + head] = R; }
   }
-  cluster.sync();
+  // a cluster's barrier, for a CTA alone, is 2 to 5 % of a call with many short sequences
+  if (p.splits > 1) cluster.sync();
+  else __syncthreads();
   // each CTA writes its share of the outputs, from every CTA's sums
   for (int i = threadIdx.x + rank * WARPS * 32; i < heads * (p.dim / 4); i += p.splits * WARPS * 32) {
     const int head = i / (p.dim / 4), ch = i % (p.dim / 4) * 4;
@@ -587,7 +589,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     store4(dst, ch, p.out_type, y, p.out_inv_step, p.out_zero);
     if (p.lse && ch == 0) p.lse[(int64_t)seq * p.hq + h0 + head] = (M + log2f(L)) * 0.69314718055994530942f;
   }
-  cluster.sync();          // no CTA leaves while another reads its sums
+  if (p.splits > 1) cluster.sync();          // no CTA leaves while another reads its sums
 }
 
 // [n_pages][n_heads][page_size][dim] at the cache's strides, boxes of `box` slots of one head: of 128 bytes, 128-byte swizzle, or of
@@ -656,7 +658,7 @@ bool decode_go(Context &c, const DecodeLaunch &d)
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = (unsigned)d.p.splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr; cfg.numAttrs = 2;
+  cfg.attrs = attr; cfg.numAttrs = d.p.splits > 1 ? 2 : 1;
   bool ok = cuda_ok(cudaLaunchKernelEx(&cfg, k, d.k, d.v, d.p), "pulpnn_attn_decode");
   if (ok) count_launch("attn_decode_kernel");
   if (d.p.parts > 1) {
