@@ -57,6 +57,7 @@ struct PromptProblem {
   int64_t v_row, v_head, out_row, out_head;       // bytes
   FastDiv by_group;
   int units;                                      // of an item: 2, or 1 where all of them find an SM at once
+  int merged;                                     // items come longest first
   int nq, nk, seqs, hq, group, dim, causal, window, out_type, out_zero;
   float scale_log2, out_inv_step;
   int *status;
@@ -207,13 +208,11 @@ __device__ __forceinline__ bool guarded(const Work &w, int j, const PromptProble
   return (sees(w.u[0], j) && masked(w.u[0], j, w.lk, p)) || (sees(w.u[1], j) && masked(w.u[1], j, w.lk, p));
 }
 
-// Finds pair number x of the units of all sequences, the longest first where there are up to 256 sequences (24 packed prompts of
-// 1 to 2048 tokens: 230 us where the sequences' order took 247, SMs waiting for one that began a long item last). Beyond that in the
-// sequences' order: the search goes on where the last one stopped, `before` pairs lie ahead of sequence s0. A whole warp; false
-// where there are not so many pairs.
+// Finds pair number x of the units of all sequences: the longest first (`merged`), or in the sequences' order, where the search goes
+// on where the last one stopped, `before` pairs lying ahead of sequence s0. A whole warp; false where there are not so many pairs.
 __device__ __forceinline__ bool find_item(const PromptProblem &p, int x, int y, int lane, int &s0, int &before, Item &it)
 {
-  const bool merged = p.seqs > 1 && p.seqs <= 256;
+  const bool merged = p.merged;
   for (; s0 < p.seqs; s0 += 256) {              // eight sequences a lane
     int at[9], at_k[9], count[8], sum = 0;
     const int b0 = s0 + lane * 8;
@@ -228,7 +227,7 @@ __device__ __forceinline__ bool find_item(const PromptProblem &p, int x, int y, 
       count[k] = (int)(((int64_t)tiles * p.group + p.units - 1) >> (p.units - 1));
       sum += count[k];
     }
-    // Of up to 256 sequences, pair v of each before pair v - 1 of any: as many pairs lie ahead of those numbered v as there are beyond
+    // merged: pair v of each sequence before pair v - 1 of any: as many pairs lie ahead of those numbered v as there are beyond
     // v in all sequences together.
     int v = 0;
     if (merged) {
@@ -946,6 +945,10 @@ extern "C" int pulpnn_attn_prompt(const pulpnn_attn_prompt_t *a)
   // one unit an item where that still fits the GPU at once: 300 tokens of 32 heads took 12.9 us, 13.9 in pairs
   p.units = units * a->n_kv_heads <= c.sm_count ? 1 : 2;
   const int64_t pairs = p.units == 1 ? units : (units + a->n_seqs + 1) / 2;
+  // Longest first, so that no SM begins a long item last: 24 packed prompts of 1 to 2048 tokens 230 us, 247 in the sequences' order; 250
+  // of 300 tokens 549 and 633. A warp looks through up to 256 sequences at once, which takes longer than to go on from the last one
+  // and shows where an SM has few items: two prompts of 500 tokens 16.7 us, 14.4 in order.
+  p.merged = a->n_seqs > 1 && a->n_seqs <= 256 && pairs * a->n_kv_heads >= 12 * (int64_t)c.sm_count;
   ATTN_REQUIRE(pairs <= 0x3fffffff, PULPNN_ERR_UNSUPPORTED, "%s: %d rows in %d sequences", who, a->n_q_rows, a->n_seqs);
   const dim3 grid((unsigned)pairs, (unsigned)a->n_kv_heads);
   const bool f16 = a->type == PULPNN_TYPE_F16, narrow = a->head_dim <= 64;

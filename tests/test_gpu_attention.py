@@ -645,8 +645,8 @@ def test_prompt_many_sequences():
     prompt_case(9, lens, [0] * 1000, 1, 1, 64, BF16)
 
 
-@pytest.mark.parametrize("seqs", [2, 3, 33, 255, 256, 257])
-@pytest.mark.parametrize("hq,hkv", [(7, 1), (2, 2)])
+@pytest.mark.parametrize("seqs", [2, 33, 180, 256, 257])
+@pytest.mark.parametrize("hq,hkv", [(14, 2), (8, 8)])
 def test_prompt_sequences_taken_longest_first_or_in_order(seqs, hq, hkv):
     lens = [(b * 37) % 61 if b % 3 else (b * 131) % 400 for b in range(seqs)]
     lens[-1] = 390
