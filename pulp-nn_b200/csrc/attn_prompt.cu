@@ -387,22 +387,21 @@ __device__ __forceinline__ void mma_warp(Control &ct, uint32_t base, uint32_t tm
   const uint32_t id_s = idesc16(Kind<T>::BF16, false, BK), id_o = idesc16(Kind<T>::BF16, true, (p.dim + 15) / 16 * 16);
   int i = -1, np[2] = {0, 0}, nq[2] = {0, 0}, ns[2] = {0, 0}, e = 0;        // e: the ring's number of the current key tile
   struct Range { int lo, hi, ulo[2], uhi[2]; } cur, nxt;      // key tiles of an item and of its units
-  // the next item that has key tiles; those without need nothing here. False: there is none, or an error (ok)
+  // Looks at the next item. TILES: it has key tiles; NONE: it needs nothing here; END: there is none, or an error (ok).
+  enum Next { END, NONE, TILES };
   auto next_item = [&](Range &r) {
-    while (true) {
-      i++;
-      wait(&ct.item_full[i % ITEMS], (i / ITEMS) & 1);
-      if (__any_sync(0xffffffffu, !ok) || __any_sync(0xffffffffu, ct.item[i % ITEMS].end)) return false;
-      const Work &w = ct.item[i % ITEMS].w;
-      r.lo = __shfl_sync(0xffffffffu, w.lo, 0); r.hi = __shfl_sync(0xffffffffu, w.hi, 0);
+    i++;
+    wait(&ct.item_full[i % ITEMS], (i / ITEMS) & 1);
+    if (__any_sync(0xffffffffu, !ok) || __any_sync(0xffffffffu, ct.item[i % ITEMS].end)) return END;
+    const Work &w = ct.item[i % ITEMS].w;
+    r.lo = __shfl_sync(0xffffffffu, w.lo, 0); r.hi = __shfl_sync(0xffffffffu, w.hi, 0);
 #pragma unroll
-      for (int x = 0; x < 2; x++) {
-        r.ulo[x] = __shfl_sync(0xffffffffu, w.u[x].lo, 0); r.uhi[x] = __shfl_sync(0xffffffffu, w.u[x].hi, 0);
-      }
-      __syncwarp();
-      if (leader) mbar_arrive(&ct.item_empty[i % ITEMS]);
-      if (r.lo < r.hi) return true;
+    for (int x = 0; x < 2; x++) {
+      r.ulo[x] = __shfl_sync(0xffffffffu, w.u[x].lo, 0); r.uhi[x] = __shfl_sync(0xffffffffu, w.u[x].hi, 0);
     }
+    __syncwarp();
+    if (leader) mbar_arrive(&ct.item_empty[i % ITEMS]);
+    return r.lo < r.hi ? TILES : NONE;
   };
   auto wait_kv = [&](int k) { wait(&ct.kv_full[k % ST], (k / ST) & 1); };
   // S of unit x with tile j, K being number k of the ring, which has landed
@@ -426,65 +425,71 @@ __device__ __forceinline__ void mma_warp(Control &ct, uint32_t base, uint32_t tm
     umma_commit_by(leader, &ct.s_full[x]);
     if (j == hi - 1) umma_commit_by(leader, &ct.q_empty[x]);
   };
-  bool more = next_item(cur);
-  int j = 0;
-  if (more) {
-    j = cur.lo;
-    wait_kv(0);
+  Next next = next_item(cur);
+  while (true) {
+    // the first S of an item behind which no product is left to issue
+    while (next == NONE) next = next_item(cur);
+    if (next == END) break;
+    int j = cur.lo;
+    wait_kv(e);
+    if (__any_sync(0xffffffffu, !ok)) break;
     tc_fence_after();
 #pragma unroll
     for (int x = 0; x < 2; x++)
-      if (j >= cur.ulo[x] && j < cur.uhi[x]) issue_s(x, cur.ulo[x], cur.uhi[x], j, 0);
-    umma_commit_by(leader, &ct.kv_empty[0]);
-  }
-  while (more) {
-    // the tile after this one, of this item or the next
-    const bool same = j + 1 < cur.hi;
-    int jn = j + 1;
-    if (!same) {
-      more = next_item(nxt);
-      jn = nxt.lo;
-    }
-    wait_kv(e + 1);
-    wait(&ct.clean[((e + 1) % ST) >> 1], ((e + 1) / ST) & 1);
-    if (more) wait_kv(e + 2);
-    if (__any_sync(0xffffffffu, !ok)) break;
-    const uint32_t b = v_low + ((e + 1) % ST) * (SH::TILE >> 4);
-    auto next_s = [&](int x) {
-      const int lo_n = same ? cur.ulo[x] : nxt.ulo[x], hi_n = same ? cur.uhi[x] : nxt.uhi[x];
-      if (more && jn >= lo_n && jn < hi_n) issue_s(x, lo_n, hi_n, jn, e + 2);
-    };
-    if (SH::APART) {
+      if (j >= cur.ulo[x] && j < cur.uhi[x]) issue_s(x, cur.ulo[x], cur.uhi[x], j, e);
+    umma_commit_by(leader, &ct.kv_empty[e % ST]);
+    bool more = true;                          // S of a next tile has been issued, too
+    while (more) {
+      // The tile after this one, of this item or the next. Where the next item has none, this tile's P V goes out before a further
+      // item is looked at: items come as earlier ones are done (ITEMS at a time), and this one is not before its last P V.
+      const bool same = j + 1 < cur.hi;
+      int jn = j + 1;
+      if (!same) {
+        next = next_item(nxt);
+        more = next == TILES;
+        jn = nxt.lo;
+      }
+      wait_kv(e + 1);
+      wait(&ct.clean[((e + 1) % ST) >> 1], ((e + 1) / ST) & 1);
+      if (more) wait_kv(e + 2);
+      if (__any_sync(0xffffffffu, !ok)) { next = END; break; }
+      const uint32_t b = v_low + ((e + 1) % ST) * (SH::TILE >> 4);
+      auto next_s = [&](int x) {
+        const int lo_n = same ? cur.ulo[x] : nxt.ulo[x], hi_n = same ? cur.uhi[x] : nxt.uhi[x];
+        if (more && jn >= lo_n && jn < hi_n) issue_s(x, lo_n, hi_n, jn, e + 2);
+      };
+      if (SH::APART) {
 #pragma unroll
-      for (int x = 0; x < 2; x++) next_s(x);
-    }
+        for (int x = 0; x < 2; x++) next_s(x);
+      }
 #pragma unroll
-    for (int x = 0; x < 2; x++) {
-      if (j >= cur.ulo[x] && j < cur.uhi[x]) {
-        const bool begun = j > cur.ulo[x], last = j == cur.uhi[x] - 1;
-        const uint32_t o = tmem + SH::O_AT + x * DP, w = tmem + SH::P_AT + x * SH::P_STEP;
-        if (!SH::APART) {
-          wait(&ct.p_half[x], np[x] & 1);
+      for (int x = 0; x < 2; x++) {
+        if (j >= cur.ulo[x] && j < cur.uhi[x]) {
+          const bool begun = j > cur.ulo[x], last = j == cur.uhi[x] - 1;
+          const uint32_t o = tmem + SH::O_AT + x * DP, w = tmem + SH::P_AT + x * SH::P_STEP;
+          if (!SH::APART) {
+            wait(&ct.p_half[x], np[x] & 1);
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++) umma_ts(leader, o, w + kk * 8, desc_of(b + kk * (2048 >> 4)), id_o, begun || kk > 0);
+            umma_commit_by(leader, &ct.pv_done[x]);         // of the first half
+          }
+          wait(&ct.p_full[x], np[x] & 1);
+          np[x]++;
           tc_fence_after();
 #pragma unroll
-          for (int kk = 0; kk < 4; kk++) umma_ts(leader, o, w + kk * 8, desc_of(b + kk * (2048 >> 4)), id_o, begun || kk > 0);
-          umma_commit_by(leader, &ct.pv_done[x]);         // of the first half
+          for (int kk = SH::APART ? 0 : 4; kk < 8; kk++) umma_ts(leader, o, w + kk * 8, desc_of(b + kk * (2048 >> 4)), id_o, begun || kk > 0);
+          if (SH::APART) umma_commit_by(leader, &ct.pv_done[x]);
+          if (last) umma_commit_by(leader, &ct.o_full[x]);
         }
-        wait(&ct.p_full[x], np[x] & 1);
-        np[x]++;
-        tc_fence_after();
-#pragma unroll
-        for (int kk = SH::APART ? 0 : 4; kk < 8; kk++) umma_ts(leader, o, w + kk * 8, desc_of(b + kk * (2048 >> 4)), id_o, begun || kk > 0);
-        if (SH::APART) umma_commit_by(leader, &ct.pv_done[x]);
-        if (last) umma_commit_by(leader, &ct.o_full[x]);
+        if (!SH::APART) next_s(x);
       }
-      if (!SH::APART) next_s(x);
+      umma_commit_by(leader, &ct.kv_empty[(e + 1) % ST]);
+      if (more) umma_commit_by(leader, &ct.kv_empty[(e + 2) % ST]);
+      e += 2;
+      j = jn;
+      if (!same) cur = nxt;
     }
-    umma_commit_by(leader, &ct.kv_empty[(e + 1) % ST]);
-    if (more) umma_commit_by(leader, &ct.kv_empty[(e + 2) % ST]);
-    e += 2;
-    j = jn;
-    if (!same) cur = nxt;
   }
   // the MMAs issued so far end before TMEM is given back
   volatile int never = 0;
