@@ -51,7 +51,7 @@ namespace cg = cooperative_groups;
 // the cache holds 8 bits. Three stages and two CTAs: 171 instead of 165 us for 64 ragged sequences of up to 8192 tokens in
 // 16 bits, 189 instead of 151 for 200 of 80 channels.
 constexpr int WARPS = 4, STAGES = 2, MOST_SPLITS = 8;
-constexpr float LAG = 8.f, NOTHING = -1e30f;
+constexpr float LAG = 8.f, NOTHING = -3.402823466e38f;       // the lowest number: any score is at least that
 
 struct DecodeProblem {
   const char *q;

@@ -46,7 +46,7 @@ using namespace sm100;
 
 constexpr int BQ = 128, BK = 128, THREADS = 384;
 constexpr int WARP_LOAD = 8, WARP_MMA = 9, WARP_GUARD = 10, GUARD_THREADS = 64;
-constexpr float NOTHING = -1e30f;
+constexpr float NOTHING = -3.402823466e38f;       // the lowest number: any score is at least that
 enum { ST_LOAD = 1 << 20, ST_MMA = 1 << 21, ST_SOFTMAX = 1 << 22, ST_GUARD = 1 << 23, ST_EPI = 1 << 24 };
 
 struct PromptProblem {
@@ -585,7 +585,7 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
 #pragma unroll
           for (int k = 0; k < 4; k++) top[k] = max3(top[k], __uint_as_float(s[k][c]), __uint_as_float(s[k][c + 1]));
         const float most = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * p.scale_log2;
-        if (!(most <= 3e38f)) l = __int_as_float(0x7fffffff);        // a NaN or an infinity among the scores
+        if (!(most <= 3.402823466e38f)) l = __int_as_float(0x7fffffff);        // a NaN or an infinity among the scores
         const float to = fmaxf(m, most), f = ex2(m - to);
         m = to;
         l *= f;

@@ -5,7 +5,8 @@ from conftest import pulpnn
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
-from test_gpu_attention import BF16, F16, _settled, prompt_case  # noqa: E402, F401
+from attention_cases import eps  # noqa: E402
+from test_gpu_attention import BF16, F16, S8, _settled, gen, prompt_case  # noqa: E402, F401
 
 api = pulpnn.api
 
@@ -38,3 +39,46 @@ def test_prompt_with_fewer_keys_than_queries(dtype, dim):
 def test_prompt_all_at_once_and_without_keys():
     """No more units than SMs, each an item of its own."""
     prompt_case(25, [1, 140] * 20, [-1, -140, 3, 0] * 10, 2, 2, 64, BF16)
+
+
+# ---- scores and weights at the ends of the types ----------------------------------------------------------
+
+def one_sequence(cache_type, k, v, page=16, k_scale=1.0, v_scale=1.0):
+    """A cache of one sequence's rows ([n][dim] each), in order, with its table."""
+    n, dim = k.shape
+    pages = -(-n // page)
+    rows = [torch.zeros(pages * page, dim, dtype=cache_type, device="cuda") for _ in range(2)]
+    for r, x in zip(rows, (k, v)):
+        r[:n] = x.to(cache_type)
+    scales = [None, None]
+    if cache_type == S8:
+        scales = [torch.zeros(pages * page, device="cuda") for _ in range(2)]
+        for s, x in zip(scales, (k_scale, v_scale)):
+            s[:n] = x
+        scales = [s.view(pages, page, 1) for s in scales]
+    cache = api.KVCache(*(r.view(pages, page, 1, dim) for r in rows), *scales)
+    return cache, torch.arange(pages, dtype=torch.int32, device="cuda")[None], torch.tensor([n], dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("how", ["decode", "decode s8", "decode window", "prompt 64", "prompt 128"])
+def test_scores_of_a_large_negative_number(how):
+    """Scores of about -10^37, all equal: an average of the values, and not the zeros of a row without keys."""
+    n, dim = 300, 128 if how == "prompt 128" else 64
+    g = gen(28)
+    q, k = torch.full((1, 1, dim), -2.0 ** 60, device="cuda", dtype=BF16), torch.full((n, dim), 2.0 ** 60, device="cuda", dtype=BF16)
+    v = torch.randint(-100, 100, (n, dim), generator=g, device="cuda").to(BF16)
+    out, lse = torch.empty(1, 1, dim, dtype=BF16, device="cuda"), torch.empty(1, 1, device="cuda")
+    window = 130 if how == "decode window" else 0
+    if how.startswith("decode"):
+        cache = one_sequence(S8, torch.full_like(k, 64), v, k_scale=2.0 ** 54) if how.endswith("s8") else one_sequence(BF16, k, v)
+        api.pulpnn_attn_decode(cache[0], q, cache[1], cache[2], out, lse=lse, window=window)
+    else:
+        cu_q, cu_k = (torch.tensor([0, m], dtype=torch.int32, device="cuda") for m in (1, n))
+        api.pulpnn_attn_prompt(q, k[:, None], v[:, None], cu_q, out, cu_k=cu_k, lse=lse)
+    torch.cuda.synchronize()
+    seen = v[-window:].double()
+    want = seen.mean(0)
+    # equal weights of one: their sum and the products are whole numbers; divided in 32 bits, rounded to bf16 once
+    assert ((out[0, 0].double() - want).abs() <= (eps(BF16) / 2 + 2.0 ** -20) * want.abs()).all()
+    score = -2.0 ** 120 * dim * dim ** -0.5
+    assert abs(lse[0, 0].double() / score - 1) <= (dim + 8) * 2.0 ** -23
