@@ -516,6 +516,12 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
 {
   uint64_t r;
@@ -538,7 +544,6 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
   const uint32_t rowbase = tmem + ((uint32_t)((warp & 3) * 32) << 16);
   const uint32_t t_s = rowbase + x * 128, t_o = rowbase + SH::O_AT + x * DP, t_p = rowbase + SH::P_AT + x * SH::P_STEP;
   const int groups = (p.dim + 15) / 16;
-  const uint64_t scale2 = pair2(p.scale_log2, p.scale_log2);
   uint32_t done = 0, o_phase = 0;              // tiles of this unit; item ends
   bool ok = true;
   for (int i = 0; ok; i++) {
@@ -552,6 +557,7 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
     // every row sees every key of the tiles whole_lo .. whole_hi - 1
     const int whole_hi = (p.causal ? min(lk, max(w.pos + 1, 0)) : lk) / BK, whole_lo = p.window > 0 ? (max(w.pos + w.rows - p.window, 0) + BK - 1) / BK : 0;
     float m = NOTHING, l = 0.f;
+    bool far = false;                          // some row's reference is beyond 2^24
     for (int j = w.lo; j < w.hi; j++, done++) {
       if (!(ok = mbar_wait(&ct.s_full[x], done & 1, abort_flag, p.status, ST_SOFTMAX))) break;
       tc_fence_after();
@@ -577,6 +583,7 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
             if (!(seen & (1u << c))) s[k][c] = 0xff800000u;
         }
       }
+      float scale = p.scale_log2;
       // A new reference: the maximum so far. O is rescaled where it holds something (`has`); its products have ended.
       auto raise = [&](bool has) {
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -584,10 +591,11 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
         for (int c = 0; c < 32; c += 2)
 #pragma unroll
           for (int k = 0; k < 4; k++) top[k] = max3(top[k], __uint_as_float(s[k][c]), __uint_as_float(s[k][c + 1]));
-        const float most = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * p.scale_log2;
+        const float most = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * scale;
         if (!(most <= 3.402823466e38f)) l = __int_as_float(0x7fffffff);        // a NaN or an infinity among the scores
         const float to = fmaxf(m, most), f = ex2(m - to);
         m = to;
+        far = __any_sync(0xffffffffu, fabsf(m) > 16777216.f && m > NOTHING);
         l *= f;
         if (has) {
           for (int c = 0; c < groups; c++) {
@@ -600,9 +608,33 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
           }
         }
       };
+      // Scores are scaled within the subtraction of the reference, which is rounded once. Against a reference that is itself a rounded
+      // product, beyond 2^24 that leaves whole units of its last place, of either sign, for weights to be 2 to the power of.
+      // There (`far`) the scores are scaled and rounded first, as the reference was. At 64 channels a scale that changes costs
+      // registers (215 us instead of 207 for the packed prompts above): the differences, in units of the score, take the scores' place;
+      // at 128 channels that and its second maximum take longer (300 tokens 11.7 us, so 11.3).
+      auto scale_first = [&] {
+        if (SH::APART) {
+          const float back = 1.f / p.scale_log2;
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int c = 0; c < 32; c++) s[k][c] = __float_as_uint((__fmul_rn(__uint_as_float(s[k][c]), p.scale_log2) - m) * back);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+              const float2 v = both(mul2(pair2(__uint_as_float(s[k][c]), __uint_as_float(s[k][c + 1])), pair2(scale, scale)));
+              s[k][c] = __float_as_uint(v.x); s[k][c + 1] = __float_as_uint(v.y);
+            }
+          scale = 1.f;
+        }
+      };
       // the weights of 32 keys, as the second product wants them, and their sum
       auto weights = [&](int k, uint64_t off2) {
         uint64_t sum = 0;
+        const uint64_t scale2 = pair2(scale, scale);
         uint32_t w16[16];
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
@@ -622,23 +654,26 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
       };
       // With the reference as it is; with a new one where there is none yet, or where the weights' sum shows that one of them is
       // beyond 2^15 (or no number). In between, the scores' maximum is not looked for: that took a fifth of the time.
-      bool raised = j == w.lo;
-      if (raised) raise(false);
       if (SH::APART) {
         if (done > 0 && !(ok = mbar_wait(&ct.pv_done[x], (done - 1) & 1, abort_flag, p.status, ST_SOFTMAX))) break;
         tc_fence_after();
+        bool raised = false, need = j == w.lo || far;
         while (true) {
-          const uint64_t off2 = pair2(-m, -m);
+          if (need) { raise(j > w.lo); raised = true; if (far) scale_first(); }
+          const float off = far ? 0.f : -m;
+          const uint64_t off2 = pair2(off, off);
           uint64_t sum[4];
 #pragma unroll
           for (int k = 0; k < 4; k++) sum[k] = weights(k, off2);
           const float2 v = both(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
           if (raised || !__any_sync(0xffffffffu, !(v.x + v.y < 32768.f))) { l += v.x + v.y; break; }
-          raised = true;
-          raise(true);
+          need = true;
         }
         hand_over(&ct.p_full[x]);
       } else {
+        bool raised = j == w.lo;
+        if (raised) raise(false);
+        if (far) scale_first();
 #pragma unroll
         for (int h = 0; h < 2; h++) {
           while (true) {
@@ -653,6 +688,7 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
               tc_fence_after();
             }
             raise(h == 1 || j > w.lo);
+            if (far) scale_first();
           }
           if (!ok) break;
           hand_over(h == 0 ? &ct.p_half[x] : &ct.p_full[x]);

@@ -1,4 +1,6 @@
 """Attention over a paged cache where it is easily wrong: work without keys, values at the ends of the types, rarely taken paths."""
+import math
+
 import pytest
 
 from conftest import pulpnn
@@ -82,3 +84,29 @@ def test_scores_of_a_large_negative_number(how):
     assert ((out[0, 0].double() - want).abs() <= (eps(BF16) / 2 + 2.0 ** -20) * want.abs()).all()
     score = -2.0 ** 120 * dim * dim ** -0.5
     assert abs(lse[0, 0].double() / score - 1) <= (dim + 8) * 2.0 ** -23
+
+
+@pytest.mark.parametrize("dtype,u,w", [(F16, 1.0, 64.0), (BF16, 2.0 ** 17, 2.0 ** 30)])
+@pytest.mark.parametrize("how", ["decode", "prompt 64", "prompt 128"])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_far_apart(how, dtype, u, w, sign):
+    """Scores of up to 2^33 and 2^75, far apart: the value of the largest one, or the mean of two where it comes twice."""
+    n, dim, rows = 300, 128 if how == "prompt 128" else 64, 12
+    g = gen(31)
+    order = (torch.randperm(n, generator=g, device="cuda") % 250 + 1).float()        # the largest one once, the smallest ones twice
+    k = (order[:, None].expand(n, dim) * w).to(dtype)
+    q = (torch.tensor([sign * m for m in (3, 37, 513, 1025, 1027, 4099, 8199, 10001, 12347, 20011, 30011, 31013)], device="cuda")[:, None, None].expand(rows, 1, dim) * u).to(dtype)
+    v = torch.randint(-100, 100, (n, dim), generator=g, device="cuda").to(dtype)
+    out = torch.empty(rows, 1, dim, dtype=dtype, device="cuda")
+    if how == "decode":
+        cache = one_sequence(dtype, k, v)
+        api.pulpnn_attn_decode(cache[0], q, cache[1].expand(rows, -1).contiguous(), cache[2].expand(rows).contiguous(), out)
+    else:
+        cu_q, cu_k = (torch.tensor([0, m], dtype=torch.int32, device="cuda") for m in (rows, n))
+        api.pulpnn_attn_prompt(q.contiguous(), k[:, None].contiguous(), v[:, None], cu_q, out, cu_k=cu_k, causal=False)
+    torch.cuda.synchronize()
+    x = sign * k[:, 0].double()
+    best = x == x.max()
+    # the next score is at least 3 x 64 / 8 below: e^-24 of a value of up to 100, which a result of 0 shows by itself
+    want = v[best].double().mean(0)
+    assert ((out[:, 0].double() - want).abs() <= eps(dtype) / 2 * want.abs() + 300 * 100 * math.exp(-24)).all()
