@@ -301,8 +301,8 @@ int pulpnn_selftest_wait_timeout(unsigned int limit_us);
  *  - Each call enqueues ONE kernel (pulpnn_attn_decode at most two) on the calling thread's stream, returns
  *    a status (PULPNN_OK or an error code, also recorded for pulpnn_last_error) and may be captured
  *    into a CUDA graph. The batch setting does not apply.
- *  - Every buffer is device (or managed) memory of the context's GPU. Strides count elements; the channels of
- *    a row lie side by side, and rows of queries, keys, values and outputs begin on 16-byte boundaries (uint8
+ *  - Every buffer is device (or managed) memory of the context's GPU. Strides count elements and, but for
+ *    pulpnn_attn_prompt's, may be negative; the channels of a row lie side by side, and rows of queries, keys, values and outputs begin on 16-byte boundaries (uint8
  *    outputs of the attentions: on 4-byte ones).
  *  - head_dim: a multiple of 8 up to 128; of 16 where the cache holds 8 bits.
  *  - Sizes come from the host; slots, positions, block tables, lengths and offsets are read from device

@@ -156,6 +156,7 @@ template <bool NARROW> __device__ __forceinline__ int64_t apart(int a, int64_t s
 {
   return NARROW ? (int64_t)(a * (int)sa + b * (int)sb) : a * sa + b * sb;
 }
+constexpr int64_t NOWHERE = INT64_MIN;       // no place is that; others may be below zero, where strides are
 // What the cache holds: the outputs' type, the other 16-bit type, or 8 bits.
 enum Held { SAME, OTHER, CODES };
 template <typename T> struct OtherType { typedef __half type; };
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(WARPS * 32, Width<IN>::v == 2 ? 10 : 8) kv_app
 {
   constexpr int SIZE = Width<IN>::v, BATCH = (SIZE == 2 ? 4 : 2) / OCTS;
   __shared__ __align__(16) float2 turns[MOST_TOKENS][MAX_HEAD_DIM / 2];
-  __shared__ longlong2 where[MOST_TOKENS];      // of a token's head 0: its row's and its scale's place in the cache; -1: it is not stored
+  __shared__ longlong2 where[MOST_TOKENS];      // of a token's head 0: its row's and its scale's place in the cache; NOWHERE: it is not stored
   const int which = blockIdx.x < p.blocks[0] ? 0 : (blockIdx.x < p.blocks[0] + p.blocks[1] ? 1 : 2);
   const int block = blockIdx.x - (which > 0 ? p.blocks[0] : 0) - (which > 1 ? p.blocks[1] : 0);
   const int token0 = block * p.tokens[which], tokens = min(p.tokens[which], p.n - token0);
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(WARPS * 32, Width<IN>::v == 2 ? 10 : 8) kv_app
         const long long slot = __ldg(p.slots + token0 + threadIdx.x);
         const bool stored = slot >= 0 && slot < p.cache.n_slots;
         const int page = stored ? p.cache.by_page.div((int)slot) : 0, at = stored ? (int)slot - page * p.cache.page_size : 0;
-        where[threadIdx.x] = stored ? make_longlong2(row_of(p.cache, page, at, 0), scale_of(p.cache, page, at, 0)) : make_longlong2(-1, -1);
+        where[threadIdx.x] = stored ? make_longlong2(row_of(p.cache, page, at, 0), scale_of(p.cache, page, at, 0)) : make_longlong2(NOWHERE, 0);
       }
       __syncthreads();
     }
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(WARPS * 32, Width<IN>::v == 2 ? 10 : 8) kv_app
       if (live[b] && out) put(out + apart<NARROW>(token[b], out_token, head[b], out_head));
       if (which == 0) continue;
       const longlong2 at = where[k];
-      const bool stored = live[b] && at.x >= 0;
+      const bool stored = live[b] && at.x != NOWHERE;
       const int64_t place = at.x + apart<NARROW>(head[b], p.cache.head_stride, 0, 0);
       if (HELD == CODES) {
         float most = 0.f;
@@ -438,7 +439,7 @@ __global__ void __launch_bounds__(THREADS) kv_gather_kernel(const GatherProblem 
 #pragma unroll
   for (int b = 0; b < BATCH; b++) {
     const int row = (blockIdx.x * BATCH + b) * p.per_block + sub;
-    to[b] = -1;
+    to[b] = NOWHERE;
     w[b] = make_uint4(0, 0, 0, 0);
     scale[b] = 0.f;
     const int token = p.by_heads.div(row), head = row - token * p.heads;
@@ -452,7 +453,7 @@ __global__ void __launch_bounds__(THREADS) kv_gather_kernel(const GatherProblem 
   }
 #pragma unroll
   for (int b = 0; b < BATCH; b++) {
-    if (to[b] < 0) continue;
+    if (to[b] == NOWHERE) continue;
     uint4 *dst = reinterpret_cast<uint4 *>(p.out[which] + to[b]);
     if (!EIGHT) { *dst = w[b]; continue; }
     const unsigned q[4] = {w[b].x, w[b].y, w[b].z, w[b].w};

@@ -1,5 +1,6 @@
 """Attention over a paged cache where it is easily wrong: work without keys, values at the ends of the types, rarely taken paths."""
 import math
+from types import SimpleNamespace
 
 import pytest
 
@@ -7,8 +8,8 @@ from conftest import pulpnn
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
-from attention_cases import eps  # noqa: E402
-from test_gpu_attention import BF16, F16, S8, _settled, gen, prompt_case  # noqa: E402, F401
+from attention_cases import Fenced, attend, eps, tolerance  # noqa: E402
+from test_gpu_attention import BF16, F16, S8, Cache, _settled, gen, normal, prompt_case  # noqa: E402, F401
 
 api = pulpnn.api
 
@@ -41,6 +42,58 @@ def test_prompt_with_fewer_keys_than_queries(dtype, dim):
 def test_prompt_all_at_once_and_without_keys():
     """No more units than SMs, each an item of its own."""
     prompt_case(25, [1, 140] * 20, [-1, -140, 3, 0] * 10, 2, 2, 64, BF16)
+
+
+# ---- strides that go backwards (the C interface has them; torch does not) ------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF16, S8])
+def test_caches_and_rows_at_negative_strides(dtype):
+    g = gen(27)
+    pages, page, hkv, dim = 5, 16, 3, 64
+    c = Cache(g, dtype, pages, page, hkv, dim, False)
+    kept = [x.wide for x in (c.k, c.v)] + ([x.wide for x in c.s] if c.s else [])
+    before = [t.clone() for t in kept]
+    # the same memory with its pages, slots and heads counted from the last
+    flip = lambda x: sum((n - 1) * s for n, s in zip(x.shape[:3], x.stride()[:3])) * x.element_size()  # noqa: E731
+    s = [t.view for t in c.s] if c.s else [None, None]
+    base = [t.data_ptr() + flip(t) if t is not None else 0 for t in (c.k.view, c.v.view, *s)]
+    a, b = c.k.view.stride(), s[0].stride() if c.s else (0, 0, 0)
+    block = api.KVCache._pack(*base, -a[0], -a[1], -a[2], -b[0], -b[1], -b[2], c.handle.type, pages, page, hkv, dim, 0)
+    back = SimpleNamespace(block=block, type=c.handle.type, n_pages=pages, page_size=page, n_heads=hkv, head_dim=dim)
+    n = 40
+    slots = torch.randperm(pages * page, generator=g, device="cuda")[:n]
+    mirrored = pages * page - 1 - slots
+    k, v = normal(g, n, hkv, dim, dtype=BF16), normal(g, n, hkv, dim, dtype=BF16)
+    api.pulpnn_kv_append(c.handle, mirrored, k.flip(1).contiguous(), v.flip(1).contiguous())
+    torch.cuda.synchronize()
+    want = [t.clone() for t in kept]
+    for t, old in zip(kept, before):
+        t.copy_(old)
+    api.pulpnn_kv_append(back, slots, k, v)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(kept, want)) and c.intact()
+    # read back, into rows whose tokens and heads go backwards
+    straight, turned = ([Fenced((n, hkv, dim), BF16) for _ in range(2)] for _ in range(2))
+    api.pulpnn_kv_gather(back, slots, straight[0].view, straight[1].view)
+    o = [x.view for x in turned]
+    api._gather_call(block, api._gather_pack(slots.data_ptr(), *(x[-1, -1].data_ptr() for x in o), *[-o[0].stride(0), -o[0].stride(1)] * 2, n, api.TYPE_BF16))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert straight[i].intact() and turned[i].intact()
+        stored = c.rows(i, mirrored).flip(1)
+        assert ((straight[i].view.double() - stored).abs() <= (eps(BF16) / 2 + 2.0 ** -23) * stored.abs()).all()
+        assert torch.equal(o[i].flip(0, 1), straight[i].view)
+    # one token reads the same cache
+    q, lens = normal(g, 1, 6, dim, dtype=BF16), torch.tensor([pages * page], dtype=torch.int32, device="cuda")
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    out = torch.empty_like(q)
+    api.pulpnn_attn_decode(back, q, table, lens, out)
+    torch.cuda.synchronize()
+    at = torch.arange(pages * page - 1, -1, -1, device="cuda")
+    kk, vv = (c.rows(i, at).flip(1) for i in range(2))
+    for h in range(6):
+        w, _, sums, product = attend(q[0, h:h + 1].double(), kk[:, h // 2], vv[:, h // 2], torch.ones(1, len(at), dtype=torch.bool, device="cuda"), dim ** -0.5)
+        assert ((out[0, h].double() - w[0]).abs() <= tolerance(w, sums, product, len(at), dim, BF16, F16 if dtype == S8 else BF16)[0]).all()
 
 
 # ---- scores and weights at the ends of the types ----------------------------------------------------------
