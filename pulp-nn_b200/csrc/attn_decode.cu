@@ -330,9 +330,11 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      // the power of two at or below the row's maximum (1 for a row of zeros, infinities or the smallest numbers)
+      // the power of two at or below the row's maximum (1 for a row of zeros, infinities or the smallest numbers); one over it is
+      // 2^-127 for the largest, a number below the normal ones
       const unsigned e = (__float_as_uint(most) >> 23) & 255u;
-      const float up = e >= 1 && e <= 253 ? __uint_as_float((254u - e) << 23) : 1.f, down = e >= 1 && e <= 253 ? __uint_as_float(e << 23) : 1.f;
+      const bool fits = e >= 1 && e <= 254;
+      const float up = fits ? __uint_as_float(e < 254 ? (254u - e) << 23 : 1u << 22) : 1.f, down = fits ? __uint_as_float(e << 23) : 1.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ks++)
 #pragma unroll

@@ -163,3 +163,22 @@ def test_scores_far_apart(how, dtype, u, w, sign):
     # the next score is at least 3 x 64 / 8 below: e^-24 of a value of up to 100, which a result of 0 shows by itself
     want = v[best].double().mean(0)
     assert ((out[:, 0].double() - want).abs() <= eps(dtype) / 2 * want.abs() + 300 * 100 * math.exp(-24)).all()
+
+
+@pytest.mark.parametrize("top", [126, 127])
+def test_decode_8_bits_with_queries_at_the_end_of_bf16(top):
+    """Queries of up to 2^127 on keys of 2^-126: scores that are ordinary numbers."""
+    g = gen(top)
+    n, dim, hq = 100, 64, 2
+    q = normal(g, 1, hq, dim) * 2.0 ** 120
+    q[..., 3], q[..., 9] = 2.0 ** top, -1.5 * 2.0 ** top
+    q = q.to(BF16)
+    codes = torch.randint(-127, 128, (2, n, dim), generator=g, device="cuda")
+    cache = one_sequence(S8, codes[0], codes[1], k_scale=2.0 ** -126, v_scale=0.01)
+    out = torch.empty_like(q)
+    api.pulpnn_attn_decode(cache[0], q, cache[1], cache[2], out)
+    torch.cuda.synchronize()
+    k, v = codes[0].double() * 2.0 ** -126, codes[1].double() * float(torch.tensor(0.01))
+    want, _, sums, product = attend(q[0].double(), k, v, torch.ones(hq, n, dtype=torch.bool, device="cuda"), dim ** -0.5)
+    # a key's product with q, scaled to a largest value of 1 .. 2, may fall below 2^-126 times its scale: off by 2^-149 x 2^127 there
+    assert ((out[0].double() - want).abs() <= tolerance(want, sums, product + 1, n, dim, BF16, F16)).all()
