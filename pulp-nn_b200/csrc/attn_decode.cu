@@ -428,7 +428,8 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 #pragma unroll
           for (int c = 0; c < 2; c++) {
             float &x = s[mt][nt][2 * r + c];
-            x = ok ? x * (EIGHT ? q_scale[nt][c] * ks_ : q_scale[nt][c]) : -INFINITY;
+            // the key's scale first: codes of zero give a zero, whatever the two scales are together
+            x = ok ? (EIGHT ? x * ks_ : x) * q_scale[nt][c] : -INFINITY;
             over |= x > m[nt][c] + LAG;
             if (EIGHT) over |= x + lvs[mt][r] > ref[nt][c] + LAG;
           }

@@ -182,3 +182,21 @@ def test_decode_8_bits_with_queries_at_the_end_of_bf16(top):
     want, _, sums, product = attend(q[0].double(), k, v, torch.ones(hq, n, dtype=torch.bool, device="cuda"), dim ** -0.5)
     # a key's product with q, scaled to a largest value of 1 .. 2, may fall below 2^-126 times its scale: off by 2^-149 x 2^127 there
     assert ((out[0].double() - want).abs() <= tolerance(want, sums, product + 1, n, dim, BF16, F16)).all()
+
+
+def test_decode_8_bits_rows_of_zeros_whatever_their_scale():
+    """A row of codes of zero has the score 0, also where its scale times the query's size is beyond 32 bits."""
+    g = gen(29)
+    n, dim = 100, 64
+    q = (normal(g, 1, 2, dim) * 2.0 ** 100).to(BF16)
+    codes = torch.randint(-127, 128, (2, n, dim), generator=g, device="cuda")
+    codes[0, ::3] = 0
+    scale = torch.full((n,), 2.0 ** -104, device="cuda")
+    scale[::3] = 2.0 ** 40
+    cache = one_sequence(S8, codes[0], codes[1], k_scale=scale, v_scale=0.01)
+    out = torch.empty_like(q)
+    api.pulpnn_attn_decode(cache[0], q, cache[1], cache[2], out)
+    torch.cuda.synchronize()
+    k, v = codes[0].double() * scale.double()[:, None], codes[1].double() * float(torch.tensor(0.01))
+    want, _, sums, product = attend(q[0].double(), k, v, torch.ones(2, n, dtype=torch.bool, device="cuda"), dim ** -0.5)
+    assert ((out[0].double() - want).abs() <= tolerance(want, sums, product + 1, n, dim, BF16, F16)).all()
