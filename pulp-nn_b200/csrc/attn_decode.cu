@@ -29,8 +29,10 @@
 // 90 us (6.0 TB/s); one of 1000 tokens 6.3 us, a chain of six round trips to memory and two cluster barriers.
 //
 // Running maximum: the reference m only has to be near the true maximum, not equal to it. It is raised (and the sums
-// rescaled) when some score is more than 2^LAG above it, which one vote per tile finds out; the weights stay
-// below 2^LAG, far from the end of the 16-bit types' range, and the sums are kept in 32 bits.
+// rescaled) when some weight would be above 2^LAG, which one vote per tile finds out; the weights stay
+// below that, which the 16-bit types hold, and the sums are kept in 32 bits. fp16 ends at 2^-24 on the other side, and many small
+// weights make a sum: there the reference is set 2^UNDER below the maximum, so that weights down to 2^-21 of the largest one keep
+// all their bits, and each is off by 2^-32 of it at most. It is raised as often as with 8 and 0, bf16's.
 //
 // 8-bit caches: codes are exact in fp16, so K's product is exact but for q, whose rows are scaled by a power of two
 // to a maximum of 1 .. 2 (bf16 queries lose nothing that matters: 2^-24 of the row's maximum). The key's scale
@@ -51,7 +53,9 @@ namespace cg = cooperative_groups;
 // the cache holds 8 bits. Three stages and two CTAs: 171 instead of 165 us for 64 ragged sequences of up to 8192 tokens in
 // 16 bits, 189 instead of 151 for 200 of 80 channels.
 constexpr int WARPS = 4, STAGES = 2, MOST_SPLITS = 8;
-constexpr float LAG = 8.f, NOTHING = -3.402823466e38f;       // the lowest number: any score is at least that
+constexpr float NOTHING = -3.402823466e38f;       // the lowest number: any score is at least that
+template <typename T> struct Room { static constexpr float LAG = 15.f, UNDER = 7.f; };
+template <> struct Room<__nv_bfloat16> { static constexpr float LAG = 8.f, UNDER = 0.f; };
 
 struct DecodeProblem {
   const char *q;
@@ -201,6 +205,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   using TL = Tile<DP, EIGHT>;
   using JN = Join<DP, NT>;
   constexpr int KS = DP / 16, MT = TL::TOKENS / 16;
+  constexpr float LAG = Room<T>::LAG, UNDER = Room<T>::UNDER;
   extern __shared__ char raw[];
   __shared__ uint64_t full[WARPS][STAGES];
   __shared__ int abort_flag;
@@ -439,7 +444,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int c = 0; c < 2; c++) {
-          float a = m[nt][c], b = ref[nt][c];
+          float a = -INFINITY, b = -INFINITY;
 #pragma unroll
           for (int mt = 0; mt < MT; mt++)
 #pragma unroll
@@ -452,7 +457,9 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
             if (EIGHT) b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, d));
           }
-          if (!EIGHT) b = a;
+          // the sum of the weights is 32 bits wide wherever its reference lies; an 8-bit cache's has one of its own
+          a = fmaxf(m[nt][c], EIGHT ? a : a - UNDER);
+          b = EIGHT ? fmaxf(ref[nt][c], b - UNDER) : a;
           l[nt][c] *= ex2(m[nt][c] - a);
           const float f = ex2(ref[nt][c] - b);
           m[nt][c] = a; ref[nt][c] = b;

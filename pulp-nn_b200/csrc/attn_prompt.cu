@@ -29,7 +29,9 @@
 //   128 channels: P has to lie in columns that S had, and the next S comes behind P V. The weights are handed over in two
 //     halves, so that the first half's product runs under the second half's exponentials.
 // The running maximum is a reference that has to be near the true one only: it is taken from an item's first tile, and raised
-// (O being rescaled in TMEM by the softmax warps themselves) when a weight comes out above 2^15, which is rare.
+// (O being rescaled in TMEM by the softmax warps themselves) when a weight comes out above 2^15, which is rare. fp16 ends at
+// 2^-24 on the other side, and many small weights make a sum: there the reference lies 2^UNDER below the maximum when it is set, so that
+// each weight is off by 2^-30 of the largest one at most. (128 weights of a tile that all are the largest come to 2^12.)
 //
 // Measured (one B200): 16384 causal tokens, 32 query and 8 key heads of 128 channels in bf16, 1860 us in a burst (1180 of the
 // 1670 TFLOP/s that a plain matrix product reaches), 2090 in a long run at the power limit; 24 packed prompts of 28 heads of 64
@@ -174,8 +176,8 @@ __device__ __forceinline__ float ex2(float x)
   return y;
 }
 template <typename T> struct Kind;
-template <> struct Kind<__half> { static constexpr bool BF16 = false; static constexpr unsigned EXP = 0x7c00u; };
-template <> struct Kind<__nv_bfloat16> { static constexpr bool BF16 = true; static constexpr unsigned EXP = 0x7f80u; };
+template <> struct Kind<__half> { static constexpr bool BF16 = false; static constexpr unsigned EXP = 0x7c00u; static constexpr float UNDER = 5.f; };
+template <> struct Kind<__nv_bfloat16> { static constexpr bool BF16 = true; static constexpr unsigned EXP = 0x7f80u; static constexpr float UNDER = 0.f; };
 
 __device__ __forceinline__ void make_work(Work &w, int q0, int lq, int k0, int lk, int pair, int kvh, const PromptProblem &p)
 {
@@ -593,7 +595,7 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
           for (int k = 0; k < 4; k++) top[k] = max3(top[k], __uint_as_float(s[k][c]), __uint_as_float(s[k][c + 1]));
         const float most = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * scale;
         if (!(most <= 3.402823466e38f)) l = __int_as_float(0x7fffffff);        // a NaN or an infinity among the scores
-        const float to = fmaxf(m, most), f = ex2(m - to);
+        const float to = fmaxf(m, most - Kind<T>::UNDER), f = ex2(m - to);
         m = to;
         far = __any_sync(0xffffffffu, fabsf(m) > 16777216.f && m > NOTHING);
         l *= f;

@@ -115,6 +115,39 @@ def one_sequence(cache_type, k, v, page=16, k_scale=1.0, v_scale=1.0):
     return cache, torch.arange(pages, dtype=torch.int32, device="cuda")[None], torch.tensor([n], dtype=torch.int32, device="cuda")
 
 
+@pytest.mark.parametrize("how", ["decode", "decode s8", "prompt 64", "prompt 128"])
+def test_many_small_weights_beside_a_large_one(how):
+    """4095 weights of 2^-27 of the largest one each. In fp16, which holds nothing below 2^-24, they must not vanish from the sum over
+    the values: the largest weight is held at 2^5 or more, and each of the small ones is then off by 2^-25 at most."""
+    n, dim = 4096, 128 if how == "prompt 128" else 64
+    q, k, v = torch.zeros(1, 1, dim, device="cuda"), torch.zeros(n, dim, device="cuda"), torch.zeros(n, dim, device="cuda")
+    q[..., 0] = 8
+    k[0, 0], v[1:] = 117 / 50, 1016.0
+    out = torch.empty(1, 1, dim, dtype=F16, device="cuda")
+    lse = torch.empty(1, 1, device="cuda")
+    if how.startswith("decode"):
+        eight = how.endswith("s8")
+        cache = one_sequence(S8, k * 50, v / 8, k_scale=0.02, v_scale=8.0) if eight else one_sequence(F16, k, v)
+        kept = (k * 50).to(S8).double() * float(torch.tensor(0.02)) if eight else k.to(F16)      # as it lies in the cache
+        api.set_option(api.OPT_SPLIT_K, 1)
+        try:
+            api.pulpnn_attn_decode(cache[0], q.to(F16), cache[1], cache[2], out, scale=1.0, lse=lse)
+        finally:
+            api.set_option(api.OPT_SPLIT_K, 0)
+    else:
+        cu_q, cu_k = (torch.tensor([0, m], dtype=torch.int32, device="cuda") for m in (1, n))
+        kept = k.to(F16)
+        api.pulpnn_attn_prompt(q.to(F16), kept[:, None], v.to(F16)[:, None], cu_q, out, cu_k=cu_k, scale=1.0, lse=lse)
+    torch.cuda.synchronize()
+    score = 8 * kept[0, 0].double()
+    small = (n - 1) * (-score).exp()
+    want = 1016 * small / (1 + small)
+    # rounded to fp16 once; each small weight by half of fp16's smallest step where the largest is 2^5; sums and exponents in 32 bits
+    tol = eps(F16) / 2 * want + n * 2.0 ** -25 * 2.0 ** -5 * 1016 + 2.0 ** -16 * want
+    assert ((out.double() - want).abs() <= tol).all(), (out[0, 0, 0], want)
+    assert abs(lse.double() - (score + torch.log1p(small))) <= 2.0 ** -16
+
+
 @pytest.mark.parametrize("how", ["decode", "decode s8", "decode window", "prompt 64", "prompt 128"])
 def test_scores_of_a_large_negative_number(how):
     """Scores of about -10^37, all equal: an average of the values, and not the zeros of a row without keys."""
