@@ -547,9 +547,14 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
   const uint32_t t_s = rowbase + x * 128, t_o = rowbase + SH::O_AT + x * DP, t_p = rowbase + SH::P_AT + x * SH::P_STEP;
   const int groups = (p.dim + 15) / 16;
   uint32_t done = 0, o_phase = 0;              // tiles of this unit; item ends
+  // A whole warp goes on or gives up, since loads and stores of TMEM want all its lanes: a lane's wait that fails is looked at where
+  // the warp votes, at the next S, rows or item. Until then its tile is stale and its results are void.
+  bool mine = true;
+  auto wait = [&](uint64_t *bar, uint32_t parity, int code) { mine = mbar_wait(bar, parity, abort_flag, p.status, code) && mine; };
+  auto waited = [&](uint64_t *bar, uint32_t parity, int code) { wait(bar, parity, code); return __all_sync(0xffffffffu, mine); };
   bool ok = true;
   for (int i = 0; ok; i++) {
-    if (!(ok = mbar_wait(&ct.item_full[i % ITEMS], (i / ITEMS) & 1, abort_flag, p.status, ST_SOFTMAX))) break;
+    if (!(ok = waited(&ct.item_full[i % ITEMS], (i / ITEMS) & 1, ST_SOFTMAX))) break;
     const Item &it = ct.item[i % ITEMS];
     if (it.end) break;
     const Unit w = it.w.u[x];
@@ -561,7 +566,7 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
     float m = NOTHING, l = 0.f;
     bool far = false;                          // some row's reference is beyond 2^24
     for (int j = w.lo; j < w.hi; j++, done++) {
-      if (!(ok = mbar_wait(&ct.s_full[x], done & 1, abort_flag, p.status, ST_SOFTMAX))) break;
+      if (!(ok = waited(&ct.s_full[x], done & 1, ST_SOFTMAX))) break;
       tc_fence_after();
       uint32_t s[4][32];
 #pragma unroll
@@ -657,7 +662,8 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
       // With the reference as it is; with a new one where there is none yet, or where the weights' sum shows that one of them is
       // beyond 2^15 (or no number). In between, the scores' maximum is not looked for: that took a fifth of the time.
       if (SH::APART) {
-        if (done > 0 && !(ok = mbar_wait(&ct.pv_done[x], (done - 1) & 1, abort_flag, p.status, ST_SOFTMAX))) break;
+        wait(&ct.pv_done[x], (done - 1) & 1, ST_SOFTMAX);      // of the tile before; there is none to wait for before the first
+        __syncwarp();
         tc_fence_after();
         bool raised = false, need = j == w.lo || far;
         while (true) {
@@ -686,23 +692,22 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
             raised = true;
             // the second half: the first half's product must have ended before O is rescaled
             if (h == 1) {
-              if (!(ok = mbar_wait(&ct.pv_done[x], done & 1, abort_flag, p.status, ST_SOFTMAX))) break;
+              wait(&ct.pv_done[x], done & 1, ST_SOFTMAX);
+              __syncwarp();
               tc_fence_after();
             }
             raise(h == 1 || j > w.lo);
             if (far) scale_first();
           }
-          if (!ok) break;
           hand_over(h == 0 ? &ct.p_half[x] : &ct.p_full[x]);
         }
-        if (!ok) break;
       }
     }
     if (!ok) break;
     // ---- the rows ----
     const bool any = w.hi > w.lo;
     if (any) {
-      if (!(ok = mbar_wait(&ct.o_full[x], o_phase, abort_flag, p.status, ST_EPI))) break;
+      if (!(ok = waited(&ct.o_full[x], o_phase, ST_EPI))) break;
       o_phase ^= 1;
       tc_fence_after();
     }
@@ -777,6 +782,7 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
           }
         }
       }
+      __syncwarp();             // the rows' keys differ; the next group's load wants the whole warp
       if (p.out_type == PULPNN_TYPE_U8) {
         if (live) {
 #pragma unroll

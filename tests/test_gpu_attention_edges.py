@@ -233,3 +233,29 @@ def test_decode_8_bits_rows_of_zeros_whatever_their_scale():
     k, v = codes[0].double() * scale.double()[:, None], codes[1].double() * float(torch.tensor(0.01))
     want, _, sums, product = attend(q[0].double(), k, v, torch.ones(2, n, dtype=torch.bool, device="cuda"), dim ** -0.5)
     assert ((out[0].double() - want).abs() <= tolerance(want, sums, product + 1, n, dim, BF16, F16)).all()
+
+
+# ---- what is masked, beside rarely taken paths ------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64), (BF16, 80)])
+def test_prompt_infinities_and_uint8_output(dtype, dim):
+    """Infinities in V that some rows of a tile see and others do not, and an output of uint8: 255 and 0 for those that do, the
+    zero point for infinities of both signs together, what the finite values give for the others."""
+    g = gen(32)
+    n, step, zero = 200, 0.02, 100
+    q, k, v = (normal(g, n, 1, dim, dtype=dtype) for _ in range(3))
+    v[150, 0, ::2], v[170, 0, 1::2], v[190, 0, 0] = math.inf, -math.inf, -math.inf
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    out = torch.empty(n, 1, dim, dtype=torch.uint8, device="cuda")
+    api.pulpnn_attn_prompt(q, k, v, cu, out, out_step=step, out_zero=zero)
+    torch.cuda.synchronize()
+    finite = v[:, 0].double().where(v[:, 0].isfinite(), torch.zeros_like(v[:, 0], dtype=torch.float64))
+    seen = torch.tril(torch.ones(n, n, dtype=torch.bool, device="cuda"))
+    want, _, sums, product = attend(q[:, 0].double(), k[:, 0].double(), finite, seen, dim ** -0.5)
+    tol = tolerance(want, sums, product, n, dim, None, dtype) / step
+    got, want = out[:, 0].double(), (want / step + zero).clamp(0, 255)
+    row, channel = torch.arange(n, device="cuda")[:, None], torch.arange(dim, device="cuda")[None]
+    up, down = (row >= 150) & (channel % 2 == 0), (row >= 170) & (channel % 2 == 1)
+    both = (row >= 190) & (channel == 0)
+    assert (got[up & ~both] == 255).all() and (got[down] == 0).all() and (got[both] == zero).all()
+    assert ((got - want).abs() <= 0.5 + tol + 1e-4)[~up & ~down].all()
