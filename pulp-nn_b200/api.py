@@ -426,7 +426,7 @@ def _need(ok, what):
 
 def _rows(x, name, n, heads, dim, type_, out=False):
     """Address, token and head stride of [n][heads][dim] rows; an axis of one has the stride 0."""
-    a, b, c = x.stride()
+    a, b, c = x.stride()                  # of another rank: a ValueError, which the entry points turn into their error
     if x.shape != (n, heads, dim) or _type_of.get(x.dtype) != type_ or c != 1:
         raise PulpNNError(ERR_INVALID_ARG, "%s: %s %s with strides %s, where rows of %s are wanted" % (
             name, x.dtype, tuple(x.shape), x.stride(), (n, heads, dim)))
@@ -459,6 +459,14 @@ class _StructCall:
             f = self.f = proto(C.cast(getattr(_lib.load_library(), self.name), C.c_void_p).value)
         if f(*blocks):
             _check()
+
+
+# What unpacking a shape and packing a struct raise for tensors of another rank and numbers that the struct does not hold.
+_MALFORMED = (struct.error, ValueError, IndexError, OverflowError)
+
+
+def _malformed(name, e):
+    return PulpNNError(ERR_INVALID_ARG, "%s: a tensor of another rank, or a number beyond its range (%s)" % (name, e))
 
 
 class KVCache:
@@ -508,59 +516,65 @@ def pulpnn_kv_append(cache, slots, k, v, positions=None, inv_freq=None, interlea
     positions (int32) x inv_freq (float64, half as many as channels rotate), writes q to q_out and stores k and v in the
     cache at slots (int64; one outside the cache stores nothing). k_out, v_out: the stored rows before a cut to 8 bits.
     The outputs are float16 or bfloat16, all of one type, which need not be the cache's."""
-    n, heads, dim = k.shape[0], cache.n_heads, cache.head_dim
-    if n == 0:
-        return
-    in_type = _type(k)
-    o = q_out if q_out is not None else k_out if k_out is not None else v_out
-    out_type = _type(o) if o is not None else cache.type if cache.type != TYPE_S8 else TYPE_BF16      # any, where no rows are written
-    pk, pk0, pk1 = _rows(k, "k", n, heads, dim, in_type)
-    pv, pv0, pv1 = _rows(v, "v", n, heads, dim, in_type)
-    pq = pq0 = pq1 = oq = oq0 = oq1 = hq = ok = ok0 = ok1 = ov = ov0 = ov1 = sq = sk = sv = 0
-    if q is not None:
-        hq = q.shape[1]
-        pq, pq0, pq1 = _rows(q, "q", n, hq, dim, in_type)
-        _need(q_out is not None, "q and q_out come together")
-        oq, oq0, oq1 = _rows(q_out, "q_out", n, hq, dim, out_type, True)
-    elif q_out is not None:
-        _need(False, "q and q_out come together")
-    if k_out is not None:
-        ok, ok0, ok1 = _rows(k_out, "k_out", n, heads, dim, out_type, True)
-    if v_out is not None:
-        ov, ov0, ov1 = _rows(v_out, "v_out", n, heads, dim, out_type, True)
-    if in_type == TYPE_S32:
-        _need(k_step is not None and v_step is not None and (q is None or q_step is not None), "int32 rows have steps")
-        sq, sk, sv = (_vector(q_step, "q_step", hq * dim, TYPE_F32), _vector(k_step, "k_step", heads * dim, TYPE_F32),
-                      _vector(v_step, "v_step", heads * dim, TYPE_F32))
-    elif q_step is not None or k_step is not None or v_step is not None:
-        _need(False, "steps are for int32 rows")
-    at = angles = half = 0
-    if inv_freq is not None:
-        half = inv_freq.shape[0]
-        _need(positions is not None or half == 0, "a rotation has positions")
-        angles = _vector(inv_freq, "inv_freq", half, _TYPE_F64)
-    if positions is not None:
-        at = _vector(positions, "positions", n, TYPE_S32)
-    _append_call(cache.block, _append_pack(
-        pq, pk, pv, oq, ok, ov, sq, sk, sv, _vector(slots, "slots", n, _TYPE_S64), at, angles, pq0, pq1, pk0, pk1, pv0, pv1,
-        oq0, oq1, ok0, ok1, ov0, ov1, n, hq, 2 * half, 1 if interleaved else 0, in_type, out_type))
+    try:
+        n, heads, dim = k.shape[0], cache.n_heads, cache.head_dim
+        if n == 0:
+            return
+        in_type = _type(k)
+        o = q_out if q_out is not None else k_out if k_out is not None else v_out
+        out_type = _type(o) if o is not None else cache.type if cache.type != TYPE_S8 else TYPE_BF16      # any, where no rows are written
+        pk, pk0, pk1 = _rows(k, "k", n, heads, dim, in_type)
+        pv, pv0, pv1 = _rows(v, "v", n, heads, dim, in_type)
+        pq = pq0 = pq1 = oq = oq0 = oq1 = hq = ok = ok0 = ok1 = ov = ov0 = ov1 = sq = sk = sv = 0
+        if q is not None:
+            hq = q.shape[1]
+            pq, pq0, pq1 = _rows(q, "q", n, hq, dim, in_type)
+            _need(q_out is not None, "q and q_out come together")
+            oq, oq0, oq1 = _rows(q_out, "q_out", n, hq, dim, out_type, True)
+        elif q_out is not None:
+            _need(False, "q and q_out come together")
+        if k_out is not None:
+            ok, ok0, ok1 = _rows(k_out, "k_out", n, heads, dim, out_type, True)
+        if v_out is not None:
+            ov, ov0, ov1 = _rows(v_out, "v_out", n, heads, dim, out_type, True)
+        if in_type == TYPE_S32:
+            _need(k_step is not None and v_step is not None and (q is None or q_step is not None), "int32 rows have steps")
+            sq, sk, sv = (_vector(q_step, "q_step", hq * dim, TYPE_F32), _vector(k_step, "k_step", heads * dim, TYPE_F32),
+                          _vector(v_step, "v_step", heads * dim, TYPE_F32))
+        elif q_step is not None or k_step is not None or v_step is not None:
+            _need(False, "steps are for int32 rows")
+        at = angles = half = 0
+        if inv_freq is not None:
+            half = inv_freq.shape[0]
+            _need(positions is not None or half == 0, "a rotation has positions")
+            angles = _vector(inv_freq, "inv_freq", half, _TYPE_F64)
+        if positions is not None:
+            at = _vector(positions, "positions", n, TYPE_S32)
+        _append_call(cache.block, _append_pack(
+            pq, pk, pv, oq, ok, ov, sq, sk, sv, _vector(slots, "slots", n, _TYPE_S64), at, angles, pq0, pq1, pk0, pk1, pv0, pv1,
+            oq0, oq1, ok0, ok1, ov0, ov1, n, hq, 2 * half, 1 if interleaved else 0, in_type, out_type))
+    except _MALFORMED as e:
+        raise _malformed("pulpnn_kv_append", e) from None
 
 
 def pulpnn_kv_gather(cache, slots, k_out, v_out=None):
     """Rows `slots` (int64) of the cache into k_out and v_out ([tokens][heads][dim], float16 or bfloat16; either may be
     None). A slot outside the cache gives zeros."""
-    n = slots.shape[0]
-    if n == 0:
-        return
-    first = k_out if k_out is not None else v_out
-    _need(first is not None, "neither k_out nor v_out")
-    out_type, heads, dim = _type(first), cache.n_heads, cache.head_dim
-    a = a0 = a1 = b = b0 = b1 = 0
-    if k_out is not None:
-        a, a0, a1 = _rows(k_out, "k_out", n, heads, dim, out_type, True)
-    if v_out is not None:
-        b, b0, b1 = _rows(v_out, "v_out", n, heads, dim, out_type, True)
-    _gather_call(cache.block, _gather_pack(_vector(slots, "slots", n, _TYPE_S64), a, b, a0, a1, b0, b1, n, out_type))
+    try:
+        n = slots.shape[0]
+        if n == 0:
+            return
+        first = k_out if k_out is not None else v_out
+        _need(first is not None, "neither k_out nor v_out")
+        out_type, heads, dim = _type(first), cache.n_heads, cache.head_dim
+        a = a0 = a1 = b = b0 = b1 = 0
+        if k_out is not None:
+            a, a0, a1 = _rows(k_out, "k_out", n, heads, dim, out_type, True)
+        if v_out is not None:
+            b, b0, b1 = _rows(v_out, "v_out", n, heads, dim, out_type, True)
+        _gather_call(cache.block, _gather_pack(_vector(slots, "slots", n, _TYPE_S64), a, b, a0, a1, b0, b1, n, out_type))
+    except _MALFORMED as e:
+        raise _malformed("pulpnn_kv_gather", e) from None
 
 
 _decode_pack = struct.Struct("=5Q5q2f8i").pack
@@ -579,23 +593,26 @@ def pulpnn_attn_decode(cache, q, block_table, seq_lens, out, scale=None, window=
     """Attention of one new token per sequence: q and out [sequences][heads][dim], block_table int32 [sequences][pages],
     seq_lens int32 [sequences]. scale: dim ** -0.5 unless given. window > 0: the last `window` tokens only. lse: float32
     [sequences][heads]. out has q's type, or uint8 with out_step (and out_zero)."""
-    n, heads, dim = q.shape
-    if n == 0:
-        return
-    q_type = _type(q)
-    out_type = _out_type(out, q_type, out_step)
-    if dim != cache.head_dim:
-        _need(False, "q and the cache have different numbers of channels")
-    pq, q0, q1 = _rows(q, "q", n, heads, dim, q_type)
-    po, o0, o1 = _rows(out, "out", n, heads, dim, out_type, True)
-    shape, strides = block_table.shape, block_table.stride()
-    if len(shape) != 2 or shape[0] != n or _type(block_table) != TYPE_S32 or (strides[1] != 1 and shape[1] > 1):
-        _need(False, "block_table is int32 [sequences][pages], the pages of a sequence side by side")
-    pages, lengths = shape[1], _vector(seq_lens, "seq_lens", n, TYPE_S32)
-    _decode_call(cache.block, _decode_pack(
-        pq, po, 0 if lse is None else _lse(lse, n, heads), block_table.data_ptr() if pages else lengths, lengths, q0, q1, o0, o1,
-        strides[0] if n > 1 else 0, dim ** -0.5 if scale is None else scale, out_step or 0., out_zero, q_type, out_type, n, heads, pages,
-        window, 0))
+    try:
+        n, heads, dim = q.shape
+        if n == 0:
+            return
+        q_type = _type(q)
+        out_type = _out_type(out, q_type, out_step)
+        if dim != cache.head_dim:
+            _need(False, "q and the cache have different numbers of channels")
+        pq, q0, q1 = _rows(q, "q", n, heads, dim, q_type)
+        po, o0, o1 = _rows(out, "out", n, heads, dim, out_type, True)
+        shape, strides = block_table.shape, block_table.stride()
+        if len(shape) != 2 or shape[0] != n or _type(block_table) != TYPE_S32 or (strides[1] != 1 and shape[1] > 1):
+            _need(False, "block_table is int32 [sequences][pages], the pages of a sequence side by side")
+        pages, lengths = shape[1], _vector(seq_lens, "seq_lens", n, TYPE_S32)
+        _decode_call(cache.block, _decode_pack(
+            pq, po, 0 if lse is None else _lse(lse, n, heads), block_table.data_ptr() if pages else lengths, lengths, q0, q1, o0, o1,
+            strides[0] if n > 1 else 0, dim ** -0.5 if scale is None else scale, out_step or 0., out_zero, q_type, out_type, n, heads, pages,
+            window, 0))
+    except _MALFORMED as e:
+        raise _malformed("pulpnn_attn_decode", e) from None
 
 
 def _lse(lse, n, heads):
@@ -611,24 +628,27 @@ def pulpnn_attn_prompt(q, k, v, cu_q, out, cu_k=None, causal=True, window=0, sca
     """Attention over whole prompts: sequence b holds rows cu_q[b] .. cu_q[b+1] of q and out ([rows][heads][dim]) and rows
     cu_k[b] .. cu_k[b+1] (cu_q's unless given) of k and v. Its last query and its last key have the same position.
     causal: no query sees a later position; window > 0 (causal only): nor one `window` or more before its own."""
-    n, heads, dim = q.shape
-    if n == 0:
-        return
-    nk, kv_heads = k.shape[0], k.shape[1]
-    type_ = _type(q)
-    out_type = _out_type(out, type_, out_step)
-    pq, q0, q1 = _rows(q, "q", n, heads, dim, type_)
-    pk, k0, k1 = _rows(k, "k", nk, kv_heads, dim, type_)
-    pv, v0, v1 = _rows(v, "v", nk, kv_heads, dim, type_)
-    po, o0, o1 = _rows(out, "out", n, heads, dim, out_type, True)
-    seqs = cu_q.shape[0] - 1
-    if cu_k is None:
-        _need(nk == n, "other numbers of rows of keys than of queries, and no cu_k")
-        cu_k = cu_q
-    _prompt_call(_prompt_pack(
-        pq, pk, pv, po, 0 if lse is None else _lse(lse, n, heads), _vector(cu_q, "cu_q", seqs + 1, TYPE_S32),
-        _vector(cu_k, "cu_k", seqs + 1, TYPE_S32), q0, q1, k0, k1, v0, v1, o0, o1, dim ** -0.5 if scale is None else scale,
-        out_step or 0., out_zero, type_, out_type, n, nk, seqs, heads, kv_heads, dim, 1 if causal else 0, window, 0))
+    try:
+        n, heads, dim = q.shape
+        if n == 0:
+            return
+        nk, kv_heads = k.shape[0], k.shape[1]
+        type_ = _type(q)
+        out_type = _out_type(out, type_, out_step)
+        pq, q0, q1 = _rows(q, "q", n, heads, dim, type_)
+        pk, k0, k1 = _rows(k, "k", nk, kv_heads, dim, type_)
+        pv, v0, v1 = _rows(v, "v", nk, kv_heads, dim, type_)
+        po, o0, o1 = _rows(out, "out", n, heads, dim, out_type, True)
+        seqs = cu_q.shape[0] - 1
+        if cu_k is None:
+            _need(nk == n, "other numbers of rows of keys than of queries, and no cu_k")
+            cu_k = cu_q
+        _prompt_call(_prompt_pack(
+            pq, pk, pv, po, 0 if lse is None else _lse(lse, n, heads), _vector(cu_q, "cu_q", seqs + 1, TYPE_S32),
+            _vector(cu_k, "cu_k", seqs + 1, TYPE_S32), q0, q1, k0, k1, v0, v1, o0, o1, dim ** -0.5 if scale is None else scale,
+            out_step or 0., out_zero, type_, out_type, n, nk, seqs, heads, kv_heads, dim, 1 if causal else 0, window, 0))
+    except _MALFORMED as e:
+        raise _malformed("pulpnn_attn_prompt", e) from None
 
 
 # ---- network runner --------------------------------------------------------------------------
