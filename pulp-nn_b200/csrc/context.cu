@@ -199,7 +199,10 @@ bool ctx_status_word_unless_capturing(Context &c, int **word)
   if (!c.status_word) {
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     if (cudaStreamIsCapturing(c.stream, &cap) != cudaSuccess) { cudaGetLastError(); cap = cudaStreamCaptureStatusActive; }
-    if (cap == cudaStreamCaptureStatusNone && !ctx_status_word(c)) return false;
+    if (cap == cudaStreamCaptureStatusNone) {
+      RelaxedCapture relaxed;              // another thread's capture goes on
+      if (!ctx_status_word(c)) return false;
+    }
   }
   *word = c.status_word;
   return true;

@@ -1,5 +1,6 @@
 """Attention over a paged cache where it is easily wrong: work without keys, values at the ends of the types, rarely taken paths."""
 import math
+import threading
 from types import SimpleNamespace
 
 import pytest
@@ -233,6 +234,57 @@ def test_decode_8_bits_rows_of_zeros_whatever_their_scale():
     k, v = codes[0].double() * scale.double()[:, None], codes[1].double() * float(torch.tensor(0.01))
     want, _, sums, product = attend(q[0].double(), k, v, torch.ones(2, n, dtype=torch.bool, device="cuda"), dim ** -0.5)
     assert ((out[0].double() - want).abs() <= tolerance(want, sums, product + 1, n, dim, BF16, F16)).all()
+
+
+# ---- beside a capture of another thread -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("first", ["decode", "prompt"])
+def test_a_threads_first_call_beside_a_capture_of_another(first):
+    """A thread's first attention, which gets the word its waits report into, while another thread captures a graph."""
+    g = gen(30)
+    p = normal(g, 40, 4, 64, dtype=BF16)
+    cu, out = torch.tensor([0, 40], dtype=torch.int32, device="cuda"), torch.empty_like(p)
+    c = Cache(g, BF16, 4, 16, 2, 64, False)
+    table, lens = torch.arange(3, dtype=torch.int32, device="cuda")[None], torch.tensor([40], dtype=torch.int32, device="cuda")
+    mark = torch.ones(8, device="cuda")
+
+    def call():
+        if first == "decode":
+            api.pulpnn_attn_decode(c.handle, p[:1], table, lens, out[:1])
+        else:
+            api.pulpnn_attn_prompt(p, p[:, :2], p[:, 2:], cu, out)
+
+    call()                                                   # loads the kernel
+    torch.cuda.synchronize()
+    want, errors = out.clone(), []
+    out.zero_()
+
+    def work():
+        try:
+            torch.cuda.set_device(0)
+            api.set_device(0)
+            api.set_stream(stream)
+            ready.set()
+            capturing.wait(60)
+            call()
+        except BaseException as e:
+            errors.append(e)
+
+    ready, capturing = threading.Event(), threading.Event()
+    stream, side, graph = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    t = threading.Thread(target=work)
+    t.start()
+    assert ready.wait(60)
+    with torch.cuda.graph(graph, stream=side):
+        mark.zero_()
+        capturing.set()
+        t.join()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    rows = slice(0, 1) if first == "decode" else slice(None)
+    assert not mark.any() and torch.equal(out[rows], want[rows])
 
 
 # ---- what is masked, beside rarely taken paths ------------------------------------------------------------------
