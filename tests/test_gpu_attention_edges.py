@@ -10,7 +10,7 @@ from conftest import pulpnn
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 from attention_cases import Fenced, attend, eps, tolerance  # noqa: E402
-from test_gpu_attention import BF16, F16, S8, Cache, _settled, gen, normal, prompt_case  # noqa: E402, F401
+from test_gpu_attention import BF16, F16, S8, Cache, _settled, freqs, gen, normal, prompt_case  # noqa: E402, F401
 
 api = pulpnn.api
 
@@ -43,6 +43,48 @@ def test_prompt_with_fewer_keys_than_queries(dtype, dim):
 def test_prompt_all_at_once_and_without_keys():
     """No more units than SMs, each an item of its own."""
     prompt_case(25, [1, 140] * 20, [-1, -140, 3, 0] * 10, 2, 2, 64, BF16)
+
+
+# ---- rows of 8 bits ----------------------------------------------------------------------------------------
+
+def test_append_writes_rows_that_8_bits_cannot_hold_as_they_are():
+    """k_out and v_out get a row before it is cut to 8 bits: infinities, NaN and the smallest values among them."""
+    g = gen(26)
+    x = normal(g, 6, 2, 64)
+    x[1] = 0
+    x[2] *= 1e-36
+    x[3, 0, 5], x[3, 1, 6] = math.inf, -math.inf
+    x[4, 0, 63] = math.nan
+    c = Cache(g, S8, 1, 8, 2, 64, False)
+    outs = [torch.empty(6, 2, 64, dtype=BF16, device="cuda") for _ in range(2)]
+    api.pulpnn_kv_append(c.handle, torch.arange(6, device="cuda"), x, -x, k_out=outs[0], v_out=outs[1])
+    torch.cuda.synchronize()
+    for out, want in zip(outs, (x, -x)):
+        torch.testing.assert_close(out, want.to(BF16), rtol=0, atol=0, equal_nan=True)
+
+
+# ---- append in place ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim,rot,interleaved", [(112, 20, False), (128, 126, False), (80, 32, False), (128, 128, False), (80, 32, True), (48, 14, True),
+                                                 (72, 72, False), (72, 70, False)])
+def test_append_in_place_is_append(dtype, dim, rot, interleaved):
+    """Every way the rotation takes its pairs, several batches of rows a warp: the same bits as in buffers of their own."""
+    g = gen(rot)
+    n, hq, hkv = 700, 37, 9
+    c = [Cache(gen(1), dtype, 50, 16, hkv, dim, False) for _ in range(2)]
+    slots = torch.randperm(800, generator=g, device="cuda")[:n]
+    pos = torch.randint(0, 100000, (n,), generator=g, device="cuda").to(torch.int32)
+    packed = normal(g, n, hq + 2 * hkv, dim, dtype=dtype)
+    cut = lambda x: (x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:])  # noqa: E731
+    out = torch.empty_like(packed)
+    (q, k, v), (qo, ko, vo) = cut(packed), cut(out)
+    api.pulpnn_kv_append(c[0].handle, slots, k, v, positions=pos, inv_freq=freqs(rot), interleaved=interleaved, q=q, q_out=qo, k_out=ko, v_out=vo)
+    api.pulpnn_kv_append(c[1].handle, slots, k, v, positions=pos, inv_freq=freqs(rot), interleaved=interleaved, q=q, q_out=q, k_out=k, v_out=v)
+    torch.cuda.synchronize()
+    assert torch.equal(packed, out)
+    at = torch.arange(800, device="cuda")
+    assert all(torch.equal(c[0].rows(i, at), c[1].rows(i, at)) for i in range(2))
 
 
 # ---- strides that go backwards (the C interface has them; torch does not) ------------------------------------
