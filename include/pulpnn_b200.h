@@ -405,7 +405,7 @@ int pulpnn_attn_decode(const pulpnn_kv_cache_t *cache, const pulpnn_attn_decode_
  *  - What a query does not see does not reach its result, infinities and NaN there included.
  *  - out overlaps no input; strides are positive and below 2^38. Offsets ascend; what lies beyond the rows there are is cut
  *    off, and a sequence that ends before it begins is empty. Rows of out and lse that no sequence holds are left as
- *    they were.
+ *    they were. At most 2^24 sequences, and 2^26 of sequences times query heads.
  *  - Scores, sums and the softmax are held in 32 bits; weights are rounded to 16 bits for their product with v.
  */
 typedef struct {

@@ -603,7 +603,8 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 }
 
 // [n_pages][n_heads][page_size][dim] at the cache's strides, boxes of `box` slots of one head: of 128 bytes, 128-byte swizzle, or of
-// `dense` channels as they lie
+// `dense` channels as they lie. Axes in this order also where heads lie inside slots: a map wants strides that are multiples of 16 below
+// 2^40, in any order (heads as the second axis there: 168.6 us instead of 166.4 for 64 ragged sequences).
 bool make_cache_map(CUtensorMap *map, const pulpnn_kv_cache_t &c, const void *base, int box, int dense)
 {
   sm100::EncodeTiledFn enc = sm100::encode_tiled_fn();

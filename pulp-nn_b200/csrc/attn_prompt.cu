@@ -953,6 +953,9 @@ extern "C" int pulpnn_attn_prompt(const pulpnn_attn_prompt_t *a)
   ATTN_REQUIRE(a->head_dim > 0 && a->head_dim <= MAX_HEAD_DIM && a->head_dim % 8 == 0, PULPNN_ERR_UNSUPPORTED,
                "%s: head_dim %d is not a multiple of 8 up to %d", who, a->head_dim, MAX_HEAD_DIM);
   ATTN_REQUIRE(a->n_q_rows <= 0x3fffffff && a->n_k_rows <= 0x3fffffff, PULPNN_ERR_UNSUPPORTED, "%s: 2^30 rows or more", who);
+  // The grid is made for the most items that so many sequences may have. What empty ones leave of it is taken over block by block, at 0.33 us a
+  // block and SM, and sequences are looked through 256 at a time, while the other warps wait: 0.4 s within these bounds; the waits end after 1 s.
+  ATTN_REQUIRE(a->n_seqs <= 1 << 24 && (int64_t)a->n_seqs * a->n_heads <= 1 << 26, PULPNN_ERR_UNSUPPORTED, "%s: %d sequences of %d heads", who, a->n_seqs, a->n_heads);
   ATTN_REQUIRE(a->window >= 0 && (a->window == 0 || a->causal), PULPNN_ERR_INVALID_ARG, "%s: window %d%s", who, a->window, a->causal ? "" : " of a call that is not causal");
   if (const int e = check_scale(who, a->scale)) return e;
   if (const int e = check_out(who, a->out_type, a->out_step, a->out_zero)) return e;

@@ -2,7 +2,7 @@
 import pytest
 
 from conftest import pulpnn
-from test_attention_refusals import BF16, INVALID, S32, S8, cache, refused, rows
+from test_attention_refusals import BF16, INVALID, S32, S8, UNSUPPORTED, cache, refused, rows
 
 torch = pytest.importorskip("torch")
 api = pulpnn.api
@@ -75,3 +75,9 @@ def test_sizes_beyond_the_structs():
     slots = torch.zeros(1, dtype=torch.int64).expand(n)
     refused(INVALID, api.pulpnn_kv_append, cache(), slots, far, far)
     refused(INVALID, prompt, k=far, v=far, cu_k=torch.tensor([0, 7], dtype=S32))
+
+
+def test_prompts_of_too_many_sequences():
+    refused(UNSUPPORTED, prompt, cu=torch.zeros(2 ** 24 + 2, dtype=S32), q=rows(7, 1, 64), k=rows(7, 1, 64), v=rows(7, 1, 64), out=rows(7, 1, 64))
+    q, k = rows(7, 64, 64), rows(7, 8, 64)
+    refused(UNSUPPORTED, prompt, cu=torch.zeros(2 ** 20 + 2, dtype=S32), q=q, k=k, v=k, out=q)
