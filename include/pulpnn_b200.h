@@ -332,8 +332,9 @@ typedef struct {
  * Token t of head h: x = in (F16, BF16, F32) or in * step[h * head_dim + c] (S32). The first rotary_dim channels of
  * q and k turn by the angle positions[t] * inv_freq[i], i < rotary_dim / 2: (a, b) -> (a cos - b sin,
  * b cos + a sin) of the channels (i, i + rotary_dim / 2), or (2i, 2i + 1) where interleaved is set. The angle is
- * computed in 64 bits. q_out receives q; row slots[t] of the cache receives k and v, rounded to its 16-bit type, or as
- * S8 codes rint(x * 127 / max|x|) with the scale max|x| / 127 (rows below 2^-100 become 0; a row with a NaN or an
+ * computed in 64 bits; its part of a turn is then rounded to 24 bits. q_out receives q; row slots[t] of the cache receives k
+ * and v, rounded to its 16-bit type, or as S8 codes: the whole numbers nearest to x * (127 / max|x|) in 32 bits (within 2^-15
+ * of halfway between two of them, either), with the scale max|x| / 127 (rows below 2^-100 become 0; a row with a NaN or an
  * infinity gets the scale NaN). k_out and v_out (may be NULL) receive the rows before they are cut to 8 bits.
  *
  *  - in_type: F16, BF16, F32 or S32. out_type: F16 or BF16, of q_out, k_out and v_out, whatever the cache holds.
@@ -356,7 +357,7 @@ typedef struct {
 int pulpnn_kv_append(const pulpnn_kv_cache_t *cache, const pulpnn_kv_append_t *args);
 
 /*
- * pulpnn_kv_gather -- rows slots[0 .. n_tokens) of the cache as 16-bit rows (S8: code * scale, rounded once). A slot
+ * pulpnn_kv_gather -- rows slots[0 .. n_tokens) of the cache as 16-bit rows (S8: code * scale in 32 bits, then rounded). A slot
  * outside the cache gives a row of zeros. out_type: F16 or BF16; a 16-bit cache has the same. k_out or v_out may be NULL.
  */
 typedef struct {
@@ -375,12 +376,17 @@ int pulpnn_kv_gather(const pulpnn_kv_cache_t *cache, const pulpnn_kv_gather_t *a
  * lse (may be NULL, [n_seqs][n_heads]) receives the natural logarithm of the softmax's sum. A sequence without tokens
  * gives zeros, and minus infinity in lse.
  *
- *  - q_type: F16 or BF16, the cache's where that is 16 bits wide. out_type: q_type, or U8: rint(out / out_step) + out_zero,
- *    cut to 0 .. 255.
+ *  - q_type: F16 or BF16, the cache's where that is 16 bits wide. out_type: q_type, or U8: out * (1 / out_step) in 32 bits,
+ *    rounded to the nearest, plus out_zero, cut to 0 .. 255; a NaN gives out_zero.
  *  - out overlaps no input. A long sequence of a call with few of them is read by several groups of CTAs, whose sums are
  *    joined by a second kernel through memory allocated in the stream's order (in a capture: owned by the graph).
  *  - Lengths are cut to 0 .. max_pages * page_size. A token whose page lies outside the cache is left out, as if masked.
- *  - Scores, sums and the softmax are held in 32 bits; a token's weight is rounded to 16 bits for its product with v.
+ *    How many CTAs share a sequence goes by max_pages, since lengths are not known on the host: a table much wider than the
+ *    sequences costs time (64 of 1000 tokens: 51 us, 75 with a table for 131072).
+ *  - Scores, sums and the softmax are held in 32 bits; a token's weight is rounded to q_type for its product with v. fp16
+ *    weights are off by 2^-32 of the largest at most where that is more than half a step.
+ *  - S8 caches: the weight times the value's scale is what is rounded, to fp16, and q is, after a power of two that brings its
+ *    largest value to 1 .. 2: bf16 queries lose what lies below 2^-24 of that.
  */
 typedef struct {
   const void *q;                            /* [n_seqs][n_heads][head_dim] */
@@ -406,7 +412,9 @@ int pulpnn_attn_decode(const pulpnn_kv_cache_t *cache, const pulpnn_attn_decode_
  *  - out overlaps no input; strides are positive and below 2^38. Offsets ascend; what lies beyond the rows there are is cut
  *    off, and a sequence that ends before it begins is empty. Rows of out and lse that no sequence holds are left as
  *    they were. At most 2^24 sequences, and 2^26 of sequences times query heads.
- *  - Scores, sums and the softmax are held in 32 bits; weights are rounded to 16 bits for their product with v.
+ *  - Scores, sums and the softmax are held in 32 bits; weights are rounded to `type` for their product with v (fp16 weights: off
+ *    by 2^-30 of the largest at most where that is more than half a step). lse: its logarithm is off by 2^-22 or 2 units in
+ *    its last place.
  */
 typedef struct {
   const void *q, *k, *v;                    /* [rows][heads][head_dim] */

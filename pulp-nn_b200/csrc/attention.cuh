@@ -127,7 +127,7 @@ __device__ __forceinline__ unsigned widen(unsigned biased, unsigned select)
   const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&w), *reinterpret_cast<const __half2 *>(&off));
   return *reinterpret_cast<const unsigned *>(&r);
 }
-// four adjacent channels of an output row; uint8: rint(y / step) + zero, cut to 0 .. 255 (a NaN gives the zero point)
+// four adjacent channels of an output row; uint8: rint(y * (1 / step)) + zero, cut to 0 .. 255 (a NaN gives the zero point)
 __device__ __forceinline__ unsigned to_u8(float y, float inv_step, int zero)
 {
   const float x = fminf(fmaxf(y * inv_step, -1e6f), 1e6f);

@@ -33,9 +33,10 @@
 // 2^-24 on the other side, and many small weights make a sum: there the reference lies 2^UNDER below the maximum when it is set, so that
 // each weight is off by 2^-30 of the largest one at most. (128 weights of a tile that all are the largest come to 2^12.)
 //
-// Measured (one B200): 16384 causal tokens, 32 query and 8 key heads of 128 channels in bf16, 1860 us in a burst (1180 of the
-// 1670 TFLOP/s that a plain matrix product reaches), 2090 in a long run at the power limit; 24 packed prompts of 28 heads of 64
-// channels 209 us, where the exponentials alone take 82 and the matrix products 57; 300 tokens 12.0 us: the set-up, three
+// Measured (one B200): 16384 causal tokens, 32 query and 8 key heads of 128 channels in bf16, 1960 us (1120 of the 1670 TFLOP/s
+// that a plain matrix product reaches), 2030 in a long run, where the power limit lowers the clock to 1665 of 1965 MHz; of 8192 tokens
+// the tensor cores and the special function units are busy for 62 % of the cycles each. 24 packed prompts of 28 heads of 64
+// channels 213 us, where the exponentials alone take 82 and the matrix products 57; 300 tokens 11.0 us: the set-up, three
 // key tiles one after the other and the epilogue.
 #include "attention.cuh"
 #include "sm100_primitives.cuh"
@@ -738,7 +739,7 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
       }
       __syncwarp();
     };
-    // By far the most items, without the tests below: packed prompts 209 us, 215 without this loop. (Two or four groups at a time cost
+    // By far the most items, without the tests below: packed prompts 209 us with it, 215 without. (Two or four groups at a time cost
     // the main loop its registers: 222, 272.)
     const bool plain = any && !dirty && p.out_type != PULPNN_TYPE_U8;
 #pragma unroll 1
@@ -800,7 +801,7 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
                pack2<T>(y[8 * k + 4], y[8 * k + 5]), pack2<T>(y[8 * k + 6], y[8 * k + 7]));
       if ((c & 3) == 3 || c == groups - 1) store(c);
     }
-    if (live && p.lse) p.lse[row * p.hq + w.head] = (m + __log2f(l)) * 0.69314718055994530942f;      // l is about 1 or more, or 0: off by 2^-22
+    if (live && p.lse) p.lse[row * p.hq + w.head] = (m + __log2f(l)) * 0.69314718055994530942f;      // log2 l: off by 2^-22 or 2 units in its last place
     tc_fence_before();          // O has been read: the next item's first P, behind this, lets it be written over
     __syncwarp();
     if (lane == 0) mbar_arrive(&ct.item_empty[i % ITEMS]);

@@ -142,7 +142,9 @@ __device__ __forceinline__ float larger(float a, float b)
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
   return r;
 }
-// x * inv to the nearest integer, ties to even, in the low byte: 1.5 * 2^23 leaves the sum no bits below one
+// x * inv to the nearest integer, ties to even, in the low byte: 1.5 * 2^23 leaves the sum no bits below one. inv = (1 / most) * 127 is
+// rounded twice, so that next to a tie (127 * 1.5 * 2^-23, below 2^-15) the neighbour may come out; a division a value would cost more
+// than all the rest.
 __device__ __forceinline__ unsigned code(float x, float inv) { return __float_as_uint(fmaf(x, inv, 12582912.f)); }
 
 // One block: the queries, the keys or the values of a few tokens, as many as give each thread about BATCH rows, so that
