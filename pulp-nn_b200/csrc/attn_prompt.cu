@@ -33,10 +33,10 @@
 // 2^-24 on the other side, and many small weights make a sum: there the reference lies 2^UNDER below the maximum when it is set, so that
 // each weight is off by 2^-30 of the largest one at most. (128 weights of a tile that all are the largest come to 2^12.)
 //
-// Measured (one B200): 16384 causal tokens, 32 query and 8 key heads of 128 channels in bf16, 1960 us (1120 of the 1670 TFLOP/s
+// Measured (one B200): 16384 causal tokens, 32 query and 8 key heads of 128 channels in bf16, 1990 us (1105 of the 1670 TFLOP/s
 // that a plain matrix product reaches), 2030 in a long run, where the power limit lowers the clock to 1665 of 1965 MHz; of 8192 tokens
 // the tensor cores and the special function units are busy for 62 % of the cycles each. 24 packed prompts of 28 heads of 64
-// channels 213 us, where the exponentials alone take 82 and the matrix products 57; 300 tokens 11.0 us: the set-up, three
+// channels 210 us, where the exponentials alone take 82 and the matrix products 57; 300 tokens 11.2 us: the set-up, three
 // key tiles one after the other and the epilogue.
 #include "attention.cuh"
 #include "sm100_primitives.cuh"
@@ -537,6 +537,26 @@ __device__ __forceinline__ float max3(float a, float b, float c)
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// mbar_wait of a whole warp, which goes on or gives up as one. The vote is the loop's own condition, so that the lanes never part: 24 packed
+// prompts 209.6 us, 215 with lanes that wait each by themselves and vote then.
+__device__ __forceinline__ bool wait_together(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *status, int code)
+{
+  unsigned long long t0 = 0;
+  for (unsigned spin = 1; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); spin++) {
+    if ((spin & 255u) == 0) {
+      const unsigned long long now = global_ns();
+      if (t0 == 0) t0 = now;
+      const bool late = now - t0 > WAIT_LIMIT_NS;
+      if (late) {
+        *abort_flag = 1;
+        if (status) atomicOr(status, code);
+      }
+      if (__any_sync(0xffffffffu, late || *abort_flag)) return false;
+    }
+  }
+  return true;
+}
+
 // Warps 0 to 7: the softmax of a unit, a row a thread.
 template <typename T, int DP>
 __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uint32_t tmem, const PromptProblem &p)
@@ -548,11 +568,8 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
   const uint32_t t_s = rowbase + x * 128, t_o = rowbase + SH::O_AT + x * DP, t_p = rowbase + SH::P_AT + x * SH::P_STEP;
   const int groups = (p.dim + 15) / 16;
   uint32_t done = 0, o_phase = 0;              // tiles of this unit; item ends
-  // A whole warp goes on or gives up, since loads and stores of TMEM want all its lanes: a lane's wait that fails is looked at where
-  // the warp votes, at the next S, rows or item. Until then its tile is stale and its results are void.
-  bool mine = true;
-  auto wait = [&](uint64_t *bar, uint32_t parity, int code) { mine = mbar_wait(bar, parity, abort_flag, p.status, code) && mine; };
-  auto waited = [&](uint64_t *bar, uint32_t parity, int code) { wait(bar, parity, code); return __all_sync(0xffffffffu, mine); };
+  // A whole warp goes on or gives up, since loads and stores of TMEM want all its lanes.
+  auto waited = [&](uint64_t *bar, uint32_t parity, int code) { return wait_together(bar, parity, abort_flag, p.status, code); };
   bool ok = true;
   for (int i = 0; ok; i++) {
     if (!(ok = waited(&ct.item_full[i % ITEMS], (i / ITEMS) & 1, ST_SOFTMAX))) break;
@@ -663,8 +680,7 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
       // With the reference as it is; with a new one where there is none yet, or where the weights' sum shows that one of them is
       // beyond 2^15 (or no number). In between, the scores' maximum is not looked for: that took a fifth of the time.
       if (SH::APART) {
-        wait(&ct.pv_done[x], (done - 1) & 1, ST_SOFTMAX);      // of the tile before; there is none to wait for before the first
-        __syncwarp();
+        if (!(ok = waited(&ct.pv_done[x], (done - 1) & 1, ST_SOFTMAX))) break;      // of the tile before; there is none to wait for before the first
         tc_fence_after();
         bool raised = false, need = j == w.lo || far;
         while (true) {
@@ -693,15 +709,16 @@ __device__ __forceinline__ void softmax_warps(Control &ct, uint32_t staging, uin
             raised = true;
             // the second half: the first half's product must have ended before O is rescaled
             if (h == 1) {
-              wait(&ct.pv_done[x], done & 1, ST_SOFTMAX);
-              __syncwarp();
+              if (!(ok = waited(&ct.pv_done[x], done & 1, ST_SOFTMAX))) break;
               tc_fence_after();
             }
             raise(h == 1 || j > w.lo);
             if (far) scale_first();
           }
+          if (!ok) break;
           hand_over(h == 0 ? &ct.p_half[x] : &ct.p_full[x]);
         }
+        if (!ok) break;
       }
     }
     if (!ok) break;
