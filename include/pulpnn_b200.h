@@ -305,6 +305,8 @@ int pulpnn_selftest_wait_timeout(unsigned int limit_us);
  *    pulpnn_attn_prompt's, may be negative; the channels of a row lie side by side, and rows of queries, keys, values and outputs begin on 16-byte boundaries (uint8
  *    outputs of the attentions: on 4-byte ones).
  *  - head_dim: a multiple of 8 up to 128; of 16 where the cache holds 8 bits.
+ *  - A wait inside a kernel that runs out leaves that call's rows void and shows in pulpnn_device_status(), unless the
+ *    call was captured ahead of all its thread's calls outside a capture: then there is no word yet to report into.
  *  - Sizes come from the host; slots, positions, block tables, lengths and offsets are read from device
  *    memory when the kernel runs. Values among them that point outside the buffers read and write nothing:
  *    what each call does instead stands beside it.

@@ -33,8 +33,8 @@
 // 2^-24 on the other side, and many small weights make a sum: there the reference lies 2^UNDER below the maximum when it is set, so that
 // each weight is off by 2^-30 of the largest one at most. (128 weights of a tile that all are the largest come to 2^12.)
 //
-// Measured (one B200): 16384 causal tokens, 32 query and 8 key heads of 128 channels in bf16, 1990 us (1105 of the 1670 TFLOP/s
-// that a plain matrix product reaches), 2030 in a long run, where the power limit lowers the clock to 1665 of 1965 MHz; of 8192 tokens
+// Measured (one B200): 16384 causal tokens, 32 query and 8 key heads of 128 channels in bf16, 2000 us (1100 of the 1670 TFLOP/s
+// that a plain matrix product reaches), up to 2085 in a long run, where the power limit lowers the clock to 1665 of 1965 MHz; of 8192 tokens
 // the tensor cores and the special function units are busy for 62 % of the cycles each. 24 packed prompts of 28 heads of 64
 // channels 210 us, where the exponentials alone take 82 and the matrix products 57; 300 tokens 11.2 us: the set-up, three
 // key tiles one after the other and the epilogue.
